@@ -978,6 +978,21 @@ int run_problem(const f64e_problem* p, const double* A, const double* B, double*
 
 int report_error(int code, const char* msg) { return fail(code, "%s", msg); }
 
+// For the other entry points of the library: a fresh error message, the
+// current device's SM count (an error unless it is an sm_100 part) and the
+// limit of device-side waits.
+int begin_call() {
+  g_err.clear();
+  return F64E_OK;
+}
+int device_sms(int* sms) {
+  Dev d;
+  const int rc = device_info(&d);
+  *sms = d.sms;
+  return rc;
+}
+uint64_t wait_limit_ns() { return g_wait_limit.load(); }
+
 }  // namespace f64e
 
 extern "C" {

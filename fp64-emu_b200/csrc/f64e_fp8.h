@@ -1,0 +1,65 @@
+// Host-side launchers of the 8-bit floating-point operators (block
+// quantisation, products of block-scaled codes).  All launches go to the
+// caller's stream; none allocates memory.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace f64e {
+
+constexpr int kFp8Block = 128;  // values that share one scale
+
+// ---- quantisation (f64e_fp8_quant.cu) ----
+struct Fp8QuantArgs {
+  const void* x;        // [rows, cols], row pitch ldx elements
+  int64_t rows, cols, ldx;
+  uint8_t* q;           // codes [rows][ldq]: blocks along the row (or square blocks)
+  uint8_t* s;           // scales [rows][ceil(cols / 128)], or [ceil(rows / 128)][ceil(cols / 128)]
+  uint8_t* qc;          // codes [rows][ldq]: blocks along the column
+  uint8_t* sc;          // scales [ceil(rows / 128)][cols]
+  int64_t ldq;          // row pitch of q and qc: a multiple of 16, at least cols
+};
+// x_type F64E_F32 / F16 / BF16, code F64E_E4M3 / E5M2.
+cudaError_t launch_fp8_quant_rows(const Fp8QuantArgs& a, int x_type, int code, cudaStream_t s);
+// 128 x 128 squares held in registers: tile != 0 writes q / s with one scale
+// per square; otherwise qc / sc, and q / s too when q is not null.
+cudaError_t launch_fp8_quant_squares(const Fp8QuantArgs& a, int x_type, int code, int tile, cudaStream_t s);
+
+struct Fp8DequantArgs {
+  const uint8_t* q;
+  const uint8_t* s;
+  int64_t rows, cols, ldq;
+  int64_t s_row, s_col;   // scale strides (bytes) per row block and per column block
+  int blocks;             // F64E_BLOCKS_*
+  void* out;              // [rows][cols], contiguous
+};
+cudaError_t launch_fp8_dequant(const Fp8DequantArgs& a, int code, int out_type, cudaStream_t s);
+
+// ---- products (f64e_fp8_gemm.cu) ----
+// One operand as the product sees it: `rows` output rows (or columns) by K
+// contracted values.  kmajor: codes [rows][ld], else [K][ld].  The scale of
+// (row r, contraction block kb) is s[(r >> s_shift) * s_row + kb * s_kb].
+struct Fp8Operand {
+  const uint8_t* q;
+  int64_t ld;
+  const uint8_t* s;
+  int64_t s_row, s_kb;
+  int s_shift;   // 0, or 7: one scale for 128 rows
+  int code;
+  int kmajor;
+};
+struct Fp8GemmArgs {
+  Fp8Operand a, b;
+  int64_t M, N, K;
+  void* out;      // [M][ldo]
+  int64_t ldo;
+  int out_type;
+  uint64_t wait_limit_ns;
+  int sms;
+};
+cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, cudaStream_t s);
+
+}  // namespace f64e

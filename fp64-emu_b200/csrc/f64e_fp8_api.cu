@@ -1,0 +1,182 @@
+// C ABI of the 8-bit floating-point operators (declared in include/f64e.h).
+#include <algorithm>
+
+#include "f64e.h"
+#include "f64e_fp8.h"
+
+namespace f64e {
+int report_error(int code, const char* msg);
+int begin_call();
+int device_sms(int* sms);
+uint64_t wait_limit_ns();
+}  // namespace f64e
+
+using namespace f64e;
+
+namespace {
+
+constexpr int64_t kMaxDim = (int64_t)1 << 30;   // tile coordinates are 32-bit
+
+int bad(const char* msg) { return report_error(F64E_ERR_ARGUMENT, msg); }
+int cuda_error(cudaError_t e) { return report_error(F64E_ERR_CUDA, cudaGetErrorString(e)); }
+int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+const char* check_types(int x_type, int code) {
+  if (x_type != F64E_F32 && x_type != F64E_F16 && x_type != F64E_BF16) return "fp8: element type must be F32, F16 or BF16";
+  if (code != F64E_E4M3 && code != F64E_E5M2) return "fp8: code must be E4M3 or E5M2";
+  return nullptr;
+}
+
+const char* check_matrix(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 0) return "fp8: negative dimension";
+  if (rows > kMaxDim || cols > kMaxDim) return "fp8: dimension too large";
+  // every launch covers the matrix with at most one CTA for 16 x 512, 128 x 128 or 4096 values
+  if (blocks_of(rows) * blocks_of(cols) > 0x7FFFFFFF || (rows + 15) / 16 * ((cols + 511) / 512) > 0x7FFFFFFF ||
+      rows * ((cols + 15) / 16) / 256 >= 0x7FFFFFFF)
+    return "fp8: matrix too large";
+  return nullptr;
+}
+
+const char* check_codes(const void* q, int64_t ldq, int64_t cols) {
+  if (ldq < cols) return "fp8: row pitch of the codes is below their columns";
+  if (ldq % 16 != 0 || (reinterpret_cast<uintptr_t>(q) & 15)) return "fp8: codes need 16-byte aligned rows";
+  return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+int f64e_fp8_quantize(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx, int32_t blocks,
+                      int32_t code, void* q, int64_t ldq, void* scale, void* stream) {
+  begin_call();
+  if (const char* m = check_types(x_type, code)) return bad(m);
+  if (blocks != F64E_BLOCKS_ROW && blocks != F64E_BLOCKS_COL && blocks != F64E_BLOCKS_TILE)
+    return bad("fp8: blocks must be ROW, COL or TILE");
+  if (const char* m = check_matrix(rows, cols)) return bad(m);
+  if (rows == 0 || cols == 0) return F64E_OK;
+  if (!x || !q || !scale) return bad("fp8: null pointer");
+  if (ldx < cols) return bad("fp8: row pitch of x is below its columns");
+  if (const char* m = check_codes(q, ldq, cols)) return bad(m);
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  Fp8QuantArgs a{};
+  a.x = x;
+  a.rows = rows;
+  a.cols = cols;
+  a.ldx = ldx;
+  a.ldq = ldq;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (blocks == F64E_BLOCKS_COL) {
+    a.qc = static_cast<uint8_t*>(q);
+    a.sc = static_cast<uint8_t*>(scale);
+    e = launch_fp8_quant_squares(a, x_type, code, 0, s);
+  } else {
+    a.q = static_cast<uint8_t*>(q);
+    a.s = static_cast<uint8_t*>(scale);
+    e = blocks == F64E_BLOCKS_ROW ? launch_fp8_quant_rows(a, x_type, code, s)
+                                  : launch_fp8_quant_squares(a, x_type, code, 1, s);
+  }
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx, int32_t code,
+                           void* q_row, void* scale_row, void* q_col, void* scale_col, int64_t ldq, void* stream) {
+  begin_call();
+  if (const char* m = check_types(x_type, code)) return bad(m);
+  if (const char* m = check_matrix(rows, cols)) return bad(m);
+  if (rows == 0 || cols == 0) return F64E_OK;
+  if (!x || !q_row || !scale_row || !q_col || !scale_col) return bad("fp8: null pointer");
+  if (ldx < cols) return bad("fp8: row pitch of x is below its columns");
+  if (const char* m = check_codes(q_row, ldq, cols)) return bad(m);
+  if (const char* m = check_codes(q_col, ldq, cols)) return bad(m);
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  Fp8QuantArgs a{};
+  a.x = x;
+  a.rows = rows;
+  a.cols = cols;
+  a.ldx = ldx;
+  a.ldq = ldq;
+  a.q = static_cast<uint8_t*>(q_row);
+  a.s = static_cast<uint8_t*>(scale_row);
+  a.qc = static_cast<uint8_t*>(q_col);
+  a.sc = static_cast<uint8_t*>(scale_col);
+  const cudaError_t e = launch_fp8_quant_squares(a, x_type, code, 0, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int64_t cols, int64_t ldq, int32_t blocks,
+                        const void* scale, int64_t scale_row, int64_t scale_col, void* out, int32_t out_type,
+                        void* stream) {
+  begin_call();
+  if (const char* m = check_types(out_type, code)) return bad(m);
+  if (blocks != F64E_BLOCKS_ROW && blocks != F64E_BLOCKS_COL && blocks != F64E_BLOCKS_TILE)
+    return bad("fp8: blocks must be ROW, COL or TILE");
+  if (const char* m = check_matrix(rows, cols)) return bad(m);
+  if (rows == 0 || cols == 0) return F64E_OK;
+  if (!q || !scale || !out) return bad("fp8: null pointer");
+  if (ldq < cols) return bad("fp8: row pitch of the codes is below their columns");
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  Fp8DequantArgs a{};
+  a.q = static_cast<const uint8_t*>(q);
+  a.s = static_cast<const uint8_t*>(scale);
+  a.rows = rows;
+  a.cols = cols;
+  a.ldq = ldq;
+  a.s_row = scale_row;
+  a.s_col = scale_col;
+  a.blocks = blocks;
+  a.out = out;
+  const cudaError_t e = launch_fp8_dequant(a, code, out_type, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B, const void* b_scale,
+                  void* out, void* stream) {
+  begin_call();
+  if (!p) return bad("fp8: null problem");
+  if (const char* m = check_types(p->out_type, p->a.code)) return bad(m);
+  if (const char* m = check_types(p->out_type, p->b.code)) return bad(m);
+  if (p->layout != F64E_FP8_NT && p->layout != F64E_FP8_NN && p->layout != F64E_FP8_TN)
+    return bad("fp8: layout must be NT, NN or TN");
+  if (p->M < 0 || p->N < 0 || p->K < 0) return bad("fp8: negative dimension");
+  if (p->M > kMaxDim || p->N > kMaxDim || p->K > kMaxDim) return bad("fp8: dimension too large");
+  if ((p->M + 63) / 64 * ((p->N + 63) / 64) > 0x7FFFFFFF) return bad("fp8: product too large");
+  if (p->M == 0 || p->N == 0) return F64E_OK;
+  if (p->K == 0) return bad("fp8: K must be at least 1");
+  if (!A || !a_scale || !B || !b_scale || !out) return bad("fp8: null pointer");
+  if (p->ldo < p->N) return bad("fp8: row pitch of the output is below its columns");
+  Fp8GemmArgs g{};
+  g.M = p->M;
+  g.N = p->N;
+  g.K = p->K;
+  const f64e_fp8_operand* in[2] = {&p->a, &p->b};
+  const void* q[2] = {A, B};
+  const void* sc[2] = {a_scale, b_scale};
+  Fp8Operand* o[2] = {&g.a, &g.b};
+  const int64_t rows[2] = {p->M, p->N};
+  for (int i = 0; i < 2; i++) {
+    o[i]->kmajor = i == 0 ? p->layout != F64E_FP8_TN : p->layout == F64E_FP8_NT;
+    if (const char* m = check_codes(q[i], in[i]->ld, o[i]->kmajor ? p->K : rows[i])) return bad(m);
+    if (in[i]->tile != 0 && in[i]->tile != 1) return bad("fp8: tile must be 0 or 1");
+    o[i]->q = static_cast<const uint8_t*>(q[i]);
+    o[i]->ld = in[i]->ld;
+    o[i]->s = static_cast<const uint8_t*>(sc[i]);
+    o[i]->s_row = in[i]->scale_row;
+    o[i]->s_kb = in[i]->scale_block;
+    o[i]->s_shift = in[i]->tile ? 7 : 0;
+    o[i]->code = in[i]->code;
+  }
+  g.out = out;
+  g.ldo = p->ldo;
+  g.out_type = p->out_type;
+  g.wait_limit_ns = wait_limit_ns();
+  if (const int rc = device_sms(&g.sms)) return rc;
+  const cudaError_t e = launch_fp8_gemm(g, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+}  // extern "C"

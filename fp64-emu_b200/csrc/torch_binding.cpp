@@ -9,8 +9,10 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <tuple>
 #include <vector>
 
 #include "f64e.h"
@@ -359,6 +361,288 @@ int64_t wait_selftest(at::Tensor& ws, int64_t limit_ns) {
   return st;
 }
 
+// ---- 8-bit floating-point operators ----
+
+int fp8_type(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return F64E_F32;
+    case at::kHalf: return F64E_F16;
+    case at::kBFloat16: return F64E_BF16;
+    default: return -1;
+  }
+}
+int fp8_code(at::ScalarType t) {
+  return t == at::kFloat8_e4m3fn ? F64E_E4M3 : t == at::kFloat8_e5m2 ? F64E_E5M2 : -1;
+}
+int64_t fp8_blocks(int64_t n) { return (n + 127) / 128; }
+
+void fp8_check_float(const at::Tensor& x, const char* what) {
+  TORCH_CHECK(fp8_type(x.scalar_type()) >= 0, what, " must be float32, float16 or bfloat16");
+}
+void fp8_check_cuda(const at::Tensor& t, const char* what) { TORCH_CHECK(t.is_cuda(), what, " must be a CUDA tensor"); }
+
+// Rows of x with unit stride (x itself, or a copy).
+at::Tensor fp8_rows(const at::Tensor& x) {
+  return (x.stride(1) == 1 || x.size(1) <= 1) && (x.stride(0) >= x.size(1) || x.size(0) <= 1) ? x : x.contiguous();
+}
+int64_t fp8_pitch(const at::Tensor& x) { return x.size(0) <= 1 ? std::max<int64_t>(x.size(1), 1) : x.stride(0); }
+
+// Codes [rows, cols] whose rows start on 16-byte boundaries.
+at::Tensor fp8_new_codes(const at::Tensor& x, int64_t rows, int64_t cols, at::ScalarType code) {
+  const int64_t ld = (cols + 15) / 16 * 16;
+  at::Tensor q = at::empty({rows, ld}, x.options().dtype(code));
+  return ld == cols ? q : q.as_strided({rows, cols}, {ld, 1});
+}
+int64_t fp8_code_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
+
+std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, int64_t blocks, at::ScalarType code) {
+  TORCH_CHECK(x.dim() == 2, "x must be a matrix");
+  fp8_check_float(x, "x");
+  TORCH_CHECK(fp8_code(code) >= 0, "the code must be float8_e4m3fn or float8_e5m2");
+  TORCH_CHECK(blocks >= F64E_BLOCKS_ROW && blocks <= F64E_BLOCKS_TILE, "blocks must be row, col or tile");
+  fp8_check_cuda(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t R = x.size(0), C = x.size(1);
+  const at::Tensor xr = fp8_rows(x);
+  at::Tensor q = fp8_new_codes(x, R, C, code);
+  at::Tensor s = at::empty({blocks == F64E_BLOCKS_ROW ? R : fp8_blocks(R), blocks == F64E_BLOCKS_COL ? C : fp8_blocks(C)},
+                           x.options().dtype(at::kFloat8_e8m0fnu));
+  check(f64e_fp8_quantize(xr.data_ptr(), fp8_type(x.scalar_type()), R, C, fp8_pitch(xr), (int32_t)blocks,
+                          fp8_code(code), q.data_ptr(), fp8_code_pitch(C), s.data_ptr(), stream_of()));
+  return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> fp8_quantize_both(const at::Tensor& x, at::ScalarType code) {
+  TORCH_CHECK(x.dim() == 2, "x must be a matrix");
+  fp8_check_float(x, "x");
+  TORCH_CHECK(fp8_code(code) >= 0, "the code must be float8_e4m3fn or float8_e5m2");
+  fp8_check_cuda(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t R = x.size(0), C = x.size(1);
+  const at::Tensor xr = fp8_rows(x);
+  at::Tensor q = fp8_new_codes(x, R, C, code), qc = fp8_new_codes(x, R, C, code);
+  const auto so = x.options().dtype(at::kFloat8_e8m0fnu);
+  at::Tensor s = at::empty({R, fp8_blocks(C)}, so), sc = at::empty({fp8_blocks(R), C}, so);
+  check(f64e_fp8_quantize_both(xr.data_ptr(), fp8_type(x.scalar_type()), R, C, fp8_pitch(xr), fp8_code(code),
+                               q.data_ptr(), s.data_ptr(), qc.data_ptr(), sc.data_ptr(), fp8_code_pitch(C),
+                               stream_of()));
+  return {q, s, qc, sc};
+}
+
+at::Tensor fp8_dequantize(const at::Tensor& q, const at::Tensor& s, int64_t blocks, at::ScalarType dtype) {
+  TORCH_CHECK(q.dim() == 2 && s.dim() == 2, "codes and scales must be matrices");
+  TORCH_CHECK(fp8_code(q.scalar_type()) >= 0, "codes must be float8_e4m3fn or float8_e5m2");
+  TORCH_CHECK(s.scalar_type() == at::kFloat8_e8m0fnu, "scales must be float8_e8m0fnu (powers of two)");
+  TORCH_CHECK(fp8_type(dtype) >= 0, "the result must be float32, float16 or bfloat16");
+  TORCH_CHECK(blocks >= F64E_BLOCKS_ROW && blocks <= F64E_BLOCKS_TILE, "blocks must be row, col or tile");
+  const int64_t R = q.size(0), C = q.size(1);
+  TORCH_CHECK(s.size(0) == (blocks == F64E_BLOCKS_ROW ? R : fp8_blocks(R)) &&
+                  s.size(1) == (blocks == F64E_BLOCKS_COL ? C : fp8_blocks(C)),
+              "scales do not have one entry per block");
+  fp8_check_cuda(q, "codes");
+  TORCH_CHECK(s.device() == q.device(), "codes and scales must be on one device");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor qr = fp8_rows(q);
+  at::Tensor out = at::empty({R, C}, q.options().dtype(dtype));
+  check(f64e_fp8_dequantize(qr.data_ptr(), fp8_code(q.scalar_type()), R, C, fp8_pitch(qr), (int32_t)blocks,
+                            s.data_ptr(), s.stride(0), s.stride(1), out.data_ptr(), fp8_type(dtype), stream_of()));
+  return out;
+}
+
+// One operand of a product: codes whose rows start on 16-byte boundaries (a
+// copy is made when they do not), scales as strides.  kdim: the contracted
+// dimension of q.
+struct Fp8Held {
+  at::Tensor q;
+  f64e_fp8_operand o;
+};
+void fp8_check_operand(const at::Tensor& q, const at::Tensor& s, int kdim, const char* name) {
+  TORCH_CHECK(q.dim() == 2 && s.dim() == 2, name, ": codes and scales must be matrices");
+  TORCH_CHECK(fp8_code(q.scalar_type()) >= 0, name, ": codes must be float8_e4m3fn or float8_e5m2");
+  TORCH_CHECK(s.scalar_type() == at::kFloat8_e8m0fnu, name, ": scales must be float8_e8m0fnu (powers of two)");
+  const int64_t r = q.size(1 - kdim), k = q.size(kdim), sr = s.size(1 - kdim), sk = s.size(kdim);
+  TORCH_CHECK(sk == fp8_blocks(k) && (sr == r || sr == fp8_blocks(r)), name, ": scales of shape ", s.sizes(),
+              " do not fit codes of shape ", q.sizes(), " with blocks of 128 along the contracted dimension");
+}
+Fp8Held fp8_hold(const at::Tensor& q, const at::Tensor& s, int kdim) {
+  Fp8Held h;
+  const int64_t r = q.size(1 - kdim), C = q.size(1);
+  h.q = q;
+  int64_t ld = q.size(0) <= 1 ? fp8_code_pitch(C) : q.stride(0);
+  if ((C > 1 && q.stride(1) != 1) || ld % 16 != 0 || ld < C || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15)) {
+    h.q = fp8_new_codes(q, q.size(0), C, q.scalar_type());
+    h.q.copy_(q);
+    ld = fp8_code_pitch(C);
+  }
+  h.o.ld = ld;
+  h.o.code = fp8_code(q.scalar_type());
+  h.o.tile = s.size(1 - kdim) == r ? 0 : 1;
+  h.o.scale_row = s.stride(1 - kdim);
+  h.o.scale_block = s.stride(kdim);
+  return h;
+}
+
+at::Tensor fp8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa, const at::Tensor& sb, int64_t layout,
+                  at::ScalarType dtype) {
+  TORCH_CHECK(layout >= F64E_FP8_NT && layout <= F64E_FP8_TN, "layout must be 0 (NT), 1 (NN) or 2 (TN)");
+  const int ka = layout == F64E_FP8_TN ? 0 : 1, kb = layout == F64E_FP8_NT ? 1 : 0;
+  fp8_check_operand(a, sa, ka, "A");
+  fp8_check_operand(b, sb, kb, "B");
+  TORCH_CHECK(a.size(ka) == b.size(kb), "inner dimensions differ");
+  TORCH_CHECK(a.size(ka) >= 1, "the inner dimension must be at least 1");
+  TORCH_CHECK(fp8_type(dtype) >= 0, "the result must be float32, float16 or bfloat16");
+  fp8_check_cuda(a, "A");
+  TORCH_CHECK(b.device() == a.device() && sa.device() == a.device() && sb.device() == a.device(),
+              "operands and scales must be on one device");
+  const c10::cuda::CUDAGuard guard(a.device());
+  const Fp8Held ha = fp8_hold(a, sa, ka), hb = fp8_hold(b, sb, kb);
+  f64e_fp8_problem p;
+  p.M = a.size(1 - ka);
+  p.N = b.size(1 - kb);
+  p.K = a.size(ka);
+  p.layout = (int32_t)layout;
+  p.out_type = fp8_type(dtype);
+  p.ldo = p.N;
+  p.a = ha.o;
+  p.b = hb.o;
+  at::Tensor out = at::empty({p.M, p.N}, a.options().dtype(dtype));
+  check(f64e_fp8_gemm(&p, ha.q.data_ptr(), sa.data_ptr(), hb.q.data_ptr(), sb.data_ptr(), out.data_ptr(), stream_of()));
+  return out;
+}
+
+// ---- a layer held in 8 bits ----
+void fp8_check_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2, "x must have at least one dimension and w two");
+  fp8_check_float(x, "x");
+  TORCH_CHECK(x.size(-1) == w.size(1), "x's last dimension and w's differ");
+  TORCH_CHECK(w.size(0) >= 1 && w.size(1) >= 1, "w must not be empty");
+  if (ws.has_value()) {
+    fp8_check_operand(w, *ws, 1, "w");
+    TORCH_CHECK(ws->size(0) == fp8_blocks(w.size(0)), "w: kept weights need one scale per 128 x 128 square");
+  } else {
+    fp8_check_float(w, "w");
+  }
+  fp8_check_cuda(x, "x");
+  TORCH_CHECK(w.device() == x.device() && (!ws.has_value() || ws->device() == x.device()),
+              "x, w and its scales must be on one device");
+}
+std::vector<int64_t> fp8_out_sizes(const at::Tensor& x, int64_t n) {
+  std::vector<int64_t> v = x.sizes().vec();
+  v.back() = n;
+  return v;
+}
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
+  fp8_check_linear(x, w, ws);
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  at::Tensor q, s, wq = w, wsc;
+  std::tie(q, s) = fp8_quantize(x2, F64E_BLOCKS_ROW, at::kFloat8_e4m3fn);
+  if (ws.has_value())
+    wsc = *ws;
+  else
+    std::tie(wq, wsc) = fp8_quantize(w, F64E_BLOCKS_TILE, at::kFloat8_e4m3fn);
+  at::Tensor y = fp8_mm(q, wq, s, wsc, F64E_FP8_NT, x.scalar_type());
+  return x.dim() == 2 ? y : y.view(fp8_out_sizes(x, w.size(0)));
+}
+
+// The same with gradients.  What the backward pass needs of x is kept in 8
+// bits with blocks along the rows of x (the tokens), the direction the weight
+// gradient contracts; the operators are called through the dispatcher, so a
+// tracer sees them.
+using Two = std::tuple<at::Tensor, at::Tensor>;
+using Four = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+Two call_quantize(const at::Tensor& x, int64_t blocks) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fp64_emu_b200::fp8_quantize", "")
+                       .typed<Two(const at::Tensor&, int64_t, at::ScalarType)>();
+  return op.call(x, blocks, at::kFloat8_e4m3fn);
+}
+Four call_quantize_both(const at::Tensor& x) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fp64_emu_b200::fp8_quantize_both", "")
+                       .typed<Four(const at::Tensor&, at::ScalarType)>();
+  return op.call(x, at::kFloat8_e4m3fn);
+}
+at::Tensor call_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa, const at::Tensor& sb,
+                   int64_t layout, at::ScalarType dtype) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fp64_emu_b200::fp8_mm", "")
+                       .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                         int64_t, at::ScalarType)>();
+  return op.call(a, b, sa, sb, layout, dtype);
+}
+at::Tensor call_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("fp64_emu_b200::fp8_linear", "")
+                       .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&)>();
+  return op.call(x, w, ws);
+}
+
+struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const std::optional<at::Tensor>& ws) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+    const bool want_w = w.requires_grad() && !ws.has_value();
+    at::Tensor q, s, qc, sc, wq = w, wsc;
+    if (want_w)
+      std::tie(q, s, qc, sc) = call_quantize_both(x2);
+    else
+      std::tie(q, s) = call_quantize(x2, F64E_BLOCKS_ROW);
+    if (ws.has_value())
+      wsc = *ws;
+    else
+      std::tie(wq, wsc) = call_quantize(w, F64E_BLOCKS_TILE);
+    at::Tensor y = call_mm(q, wq, s, wsc, F64E_FP8_NT, x.scalar_type());
+    const bool want_x = x.requires_grad();
+    ctx->save_for_backward({want_x ? wq : at::Tensor(), want_x ? wsc : at::Tensor(), qc, sc});
+    ctx->saved_data["x_sizes"] = x.sizes().vec();
+    ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
+    ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
+    return x.dim() == 2 ? y : y.view(fp8_out_sizes(x, w.size(0)));
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()),
+                "linear_fp8 has no second derivative");
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &wq = saved[0], &wsc = saved[1], &qc = saved[2], &sc = saved[3];
+    const bool want_x = wq.defined(), want_w = qc.defined();
+    at::Tensor dx, dw;
+    if (grads[0].defined() && (want_x || want_w)) {
+      const at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, grads[0].size(-1)});
+      at::Tensor q, s, gc, gsc;
+      if (want_x && want_w)
+        std::tie(q, s, gc, gsc) = call_quantize_both(g);
+      else if (want_x)
+        std::tie(q, s) = call_quantize(g, F64E_BLOCKS_ROW);
+      else
+        std::tie(gc, gsc) = call_quantize(g, F64E_BLOCKS_COL);
+      if (want_x) {
+        dx = call_mm(q, wq, s, wsc, F64E_FP8_NN, (at::ScalarType)ctx->saved_data["x_type"].toInt());
+        const auto sizes = ctx->saved_data["x_sizes"].toIntVector();
+        if (sizes.size() != 2) dx = dx.view(sizes);
+      }
+      if (want_w) {
+        const auto wt = (at::ScalarType)ctx->saved_data["w_type"].toInt();
+        dw = g.size(0) > 0 ? call_mm(gc, qc, gsc, sc, F64E_FP8_TN, wt)
+                           : at::zeros({g.size(1), qc.size(1)}, g.options().dtype(wt));
+      }
+    }
+    return {dx, dw, at::Tensor()};
+  }
+};
+
+at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (w.requires_grad() && !ws.has_value()))) {
+    fp8_check_linear(x, w, ws);
+    return Fp8Linear::apply(x, w, ws);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_linear(x, w, ws);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(fp64_emu_b200, ops) {
@@ -403,6 +687,11 @@ TORCH_LIBRARY(fp64_emu_b200, ops) {
       "-> Tensor");
   ops.def("fp64_emu_set_wait_limit_ns(int ns) -> ()");
   ops.def("fp64_emu_wait_selftest(Tensor! ws, int limit_ns) -> int");
+  ops.def("fp8_quantize(Tensor x, int blocks, ScalarType code) -> (Tensor, Tensor)");
+  ops.def("fp8_quantize_both(Tensor x, ScalarType code) -> (Tensor, Tensor, Tensor, Tensor)");
+  ops.def("fp8_dequantize(Tensor q, Tensor s, int blocks, ScalarType dtype) -> Tensor");
+  ops.def("fp8_mm(Tensor a, Tensor b, Tensor sa, Tensor sb, int layout, ScalarType dtype) -> Tensor");
+  ops.def("fp8_linear(Tensor x, Tensor w, Tensor? ws=None) -> Tensor");
   ops.impl("fp64_emu_maxp", &maxp);
   ops.impl("fp64_emu_workspace_bytes", &workspace_bytes);
   ops.impl("fp64_emu_set_wait_limit_ns", &set_wait_limit_ns);
@@ -424,4 +713,25 @@ TORCH_LIBRARY_IMPL(fp64_emu_b200, CUDA, ops) {
   ops.impl("fp64_emu_status", &status);
   ops.impl("fp64_emu_debug_fetch", &debug_fetch);
   ops.impl("fp64_emu_wait_selftest", &wait_selftest);
+}
+
+// The 8-bit operators check shapes and types before they ask for the device;
+// on the CPU they end with that refusal.
+#define F64E_FP8_IMPLS(ops)                        \
+  ops.impl("fp8_quantize", &fp8_quantize);         \
+  ops.impl("fp8_quantize_both", &fp8_quantize_both); \
+  ops.impl("fp8_dequantize", &fp8_dequantize);     \
+  ops.impl("fp8_mm", &fp8_mm);                     \
+  ops.impl("fp8_linear", &fp8_linear);
+TORCH_LIBRARY_IMPL(fp64_emu_b200, CUDA, ops) { F64E_FP8_IMPLS(ops) }
+TORCH_LIBRARY_IMPL(fp64_emu_b200, CPU, ops) { F64E_FP8_IMPLS(ops) }
+#undef F64E_FP8_IMPLS
+
+// Codes and scales carry no gradient; the layer has its own.
+TORCH_LIBRARY_IMPL(fp64_emu_b200, Autograd, ops) {
+  ops.impl("fp8_quantize", torch::CppFunction::makeFallthrough());
+  ops.impl("fp8_quantize_both", torch::CppFunction::makeFallthrough());
+  ops.impl("fp8_dequantize", torch::CppFunction::makeFallthrough());
+  ops.impl("fp8_mm", torch::CppFunction::makeFallthrough());
+  ops.impl("fp8_linear", &fp8_linear_autograd);
 }

@@ -227,6 +227,68 @@ F64E_API int f64e_mm_nt_noalloc(double* out, const double* A, const double* Bt, 
                                 const int32_t* primes, int32_t nprimes, int32_t exact, int64_t bits,
                                 int32_t use_corr, void* stream);
 
+/* ---- products of 8-bit floating-point codes with a scale per 128 values ----
+ *
+ * No counterpart in the reference.  A block of up to 128 values with largest
+ * finite magnitude amax is held as 8-bit codes and one scale 2^e, e the
+ * smallest integer >= -127 with amax <= FMAX * 2^e (FMAX = 448 in e4m3, 57344
+ * in e5m2; e = 0 for a block of zeros), stored as the byte e + 127.  A code is
+ * the round-to-nearest-even 8-bit float of x * 2^-e; NaN stays NaN, infinity
+ * becomes NaN in e4m3 and stays infinity in e5m2.  Rows of codes start on
+ * 16-byte boundaries (pitch a multiple of 16).  Nothing here allocates or
+ * synchronizes, except f64e_fp8_status. */
+enum { F64E_F32 = 0, F64E_F16 = 1, F64E_BF16 = 2 }; /* element types */
+enum { F64E_E4M3 = 0, F64E_E5M2 = 1 };              /* codes */
+/* Which values of a [rows, cols] matrix share a scale, and the scales' shape. */
+enum {
+  F64E_BLOCKS_ROW = 0, /* 128 neighbours of a row:      [rows, ceil(cols / 128)] */
+  F64E_BLOCKS_COL = 1, /* 128 neighbours of a column:   [ceil(rows / 128), cols] */
+  F64E_BLOCKS_TILE = 2 /* a 128 x 128 square:           [ceil(rows / 128), ceil(cols / 128)] */
+};
+
+/* Codes q [rows][ldq] and scales (contiguous, the shape above) of
+ * x [rows][ldx].  Codes between cols and the next multiple of 16 are written
+ * as zeros, nothing beyond. */
+F64E_API int f64e_fp8_quantize(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
+                               int32_t blocks, int32_t code, void* q, int64_t ldq, void* scale, void* stream);
+
+/* Row blocks and column blocks of x in one pass over it. */
+F64E_API int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
+                                    int32_t code, void* q_row, void* scale_row, void* q_col, void* scale_col,
+                                    int64_t ldq, void* stream);
+
+/* out [rows][cols] (contiguous, out_type) = code * scale, rounded once.
+ * scale_row / scale_col: strides of the scales in bytes; any ldq >= cols. */
+F64E_API int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int64_t cols, int64_t ldq,
+                                 int32_t blocks, const void* scale, int64_t scale_row, int64_t scale_col,
+                                 void* out, int32_t out_type, void* stream);
+
+/* Layouts of the products: out [M, N] = A @ B with */
+enum {
+  F64E_FP8_NT = 0, /* A [M, K], B [N, K]: scales along the rows of both */
+  F64E_FP8_NN = 1, /* A [M, K], B [K, N]: along A's rows and B's columns */
+  F64E_FP8_TN = 2  /* A [K, M], B [K, N]: along the columns of both */
+};
+typedef struct f64e_fp8_operand {
+  int64_t ld;          /* row pitch of the codes, a multiple of 16 */
+  int32_t code;        /* F64E_E4M3 or F64E_E5M2 */
+  int32_t tile;        /* 1: one scale per 128 x 128 square, 0: per 128 contracted values */
+  int64_t scale_row;   /* bytes from one scale to the next across M or N (or across squares) */
+  int64_t scale_block; /* bytes from one scale to the next along K */
+} f64e_fp8_operand;
+typedef struct f64e_fp8_problem {
+  int64_t M, N, K;
+  int32_t layout;   /* F64E_FP8_* */
+  int32_t out_type; /* F64E_F32, F64E_F16, F64E_BF16 */
+  int64_t ldo;      /* row pitch of out, in elements */
+  f64e_fp8_operand a, b;
+} f64e_fp8_problem;
+
+/* The product of the values codes and scales stand for; sums are held in 32
+ * bits and rounded once. */
+F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B,
+                           const void* b_scale, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

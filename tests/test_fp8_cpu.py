@@ -1,0 +1,190 @@
+"""CPU checks of the 8-bit floating-point operators: refusals of the Python
+surface, the torch ops and the C ABI (all before any device call), result
+shapes of the fake kernels, and the reference definition against torch's own
+8-bit types."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+import fp64_emu
+import fp8_ref as R
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+E4, E5, E8 = torch.float8_e4m3fn, torch.float8_e5m2, torch.float8_e8m0fnu
+
+
+def codes(r, c, dtype=E4):
+    return torch.zeros(r, c, dtype=torch.uint8).view(dtype)
+
+
+def scales(r, c):
+    return torch.full((r, c), 127, dtype=torch.uint8).view(E8)
+
+
+# ------------------------------------------------------------- definition --
+@pytest.mark.parametrize("code", [E4, E5])
+def test_reference_rounding_is_the_types_own(code):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(256, 256, generator=g) * torch.exp2(torch.randint(-20, 8, (256, 256), generator=g).float())
+    v, e = R.quantize(x, "tile", code)
+    t = torch.ldexp(x, -e.repeat_interleave(128, 0).repeat_interleave(128, 1).int())
+    assert torch.equal(v.float(), t.to(code).float())
+    fmax = R.FORMAT[code][0]
+    assert (v.abs().view(2, 128, 2, 128).amax((1, 3)) <= fmax).all()
+    assert (v.abs().view(2, 128, 2, 128).amax((1, 3)) > fmax / 2 * (1 - 2.0 ** -3)).all()
+
+
+@pytest.mark.parametrize("amax,e", [(448.0, 0), (448.0 * (1 + 2.0 ** -23), 1), (224.0, -1), (1.0, -8), (1.75, -8),
+                                    (1.7500001, -7), (2.0 ** -149, -127), (3.4e38, 120), (0.0, 0)])
+def test_reference_exponent_at_borders(amax, e):
+    x = torch.zeros(1, 5)
+    x[0, 3] = -amax
+    assert int(R.exponents(x, "row", E4)) == e
+
+
+# --------------------------------------------------------------- refusals --
+@pytest.mark.parametrize("call,msg", [
+    (lambda f: f.quantize_fp8(torch.zeros(2, 3, 4)), "must be a matrix"),
+    (lambda f: f.quantize_fp8(torch.zeros(3, 4, dtype=torch.float64)), "float32, float16 or bfloat16"),
+    (lambda f: f.quantize_fp8(torch.zeros(3, 4, dtype=torch.int32)), "float32, float16 or bfloat16"),
+    (lambda f: f.quantize_fp8(torch.zeros(3, 4), "row", torch.bfloat16), "the code must be"),
+    (lambda f: f.quantize_fp8(torch.zeros(3, 4)), "must be a CUDA tensor"),
+    (lambda f: f.quantize_fp8_both(torch.zeros(3)), "must be a matrix"),
+    (lambda f: f.quantize_fp8_both(torch.zeros(3, 4)), "must be a CUDA tensor"),
+    (lambda f: f.dequantize_fp8(torch.zeros(3, 4), scales(3, 1)), "codes must be"),
+    (lambda f: f.dequantize_fp8(codes(3, 4), torch.ones(3, 1)), "scales must be float8_e8m0fnu"),
+    (lambda f: f.dequantize_fp8(codes(3, 4), scales(1, 1)), "one entry per block"),
+    (lambda f: f.dequantize_fp8(codes(3, 4), scales(3, 1), "col"), "one entry per block"),
+    (lambda f: f.dequantize_fp8(codes(3, 4), scales(3, 1), dtype=torch.float64), "the result must be"),
+    (lambda f: f.dequantize_fp8(codes(3, 4), scales(3, 1)), "must be a CUDA tensor"),
+    (lambda f: f.mm_fp8(codes(3, 4), codes(5, 6), scales(3, 1), scales(5, 1)), "inner dimensions differ"),
+    (lambda f: f.mm_fp8(codes(3, 4), codes(5, 4), scales(3, 2), scales(5, 1)), "do not fit codes"),
+    (lambda f: f.mm_fp8(codes(300, 4), codes(5, 4), scales(2, 1), scales(5, 1)), "do not fit codes"),
+    (lambda f: f.mm_fp8(codes(3, 4), codes(5, 4), scales(3, 1), torch.ones(5, 1)), "float8_e8m0fnu"),
+    (lambda f: f.mm_fp8(codes(3, 4).view(torch.uint8), codes(5, 4), scales(3, 1), scales(5, 1)), "codes must be"),
+    (lambda f: f.mm_fp8(codes(3, 4)[0], codes(5, 4), scales(3, 1), scales(5, 1)), "must be matrices"),
+    (lambda f: f.mm_fp8(codes(3, 0), codes(5, 0), scales(3, 0), scales(5, 0)), "at least 1"),
+    (lambda f: f.mm_fp8(codes(3, 4), codes(5, 4), scales(3, 1), scales(5, 1), torch.float64), "the result must be"),
+    (lambda f: f.mm_fp8(codes(3, 4), codes(5, 4), scales(3, 1), scales(5, 1)), "must be a CUDA tensor"),
+    (lambda f: f.mm_nt_fp8(codes(3, 4), codes(5, 4), scales(3, 1), scales(1, 4)), "inner dimensions differ"),
+    (lambda f: f.mm_nt_fp8(codes(3, 4), codes(4, 5), scales(3, 1), scales(4, 1)), "do not fit codes"),
+    (lambda f: f.mm_tn_fp8(codes(4, 3), codes(4, 5), scales(4, 1), scales(1, 5)), "do not fit codes"),
+    (lambda f: f.mm_tn_fp8(codes(4, 3), codes(4, 5), scales(1, 3), scales(1, 5)), "must be a CUDA tensor"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(3, 5)), "last dimension"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(4)), "w two"),
+    (lambda f: f.linear_fp8(torch.zeros(()), torch.zeros(3, 5)), "at least one dimension"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4, dtype=torch.float64), torch.zeros(3, 4)), "float32, float16"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(3, 4, dtype=torch.float64)), "float32, float16"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(0, 4)), "must not be empty"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(3, 4), scales(1, 1)), "codes must be"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), codes(3, 4)), "w must be float32"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), codes(300, 4), scales(300, 1)), "128 x 128 square"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4), torch.zeros(3, 4)), "must be a CUDA tensor"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4, requires_grad=True), torch.zeros(3, 5)), "last dimension"),
+    (lambda f: f.linear_fp8(torch.zeros(2, 4, requires_grad=True), torch.zeros(3, 4)), "must be a CUDA tensor"),
+])
+def test_refusals(call, msg):
+    with pytest.raises(RuntimeError, match=msg.replace("(", r"\(")):
+        call(fp64_emu)
+
+
+def test_unknown_blocks_are_refused():
+    with pytest.raises(AssertionError, match="blocks must be"):
+        fp64_emu.quantize_fp8(torch.zeros(3, 4), "square")
+    with pytest.raises(AssertionError, match="blocks must be"):
+        fp64_emu.dequantize_fp8(codes(3, 4), scales(3, 1), "square")
+
+
+# ------------------------------------------------------------------- ABI --
+class Operand(ctypes.Structure):
+    _fields_ = [("ld", ctypes.c_int64), ("code", ctypes.c_int32), ("tile", ctypes.c_int32),
+                ("scale_row", ctypes.c_int64), ("scale_block", ctypes.c_int64)]
+
+
+class Problem(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("layout", ctypes.c_int32),
+                ("out_type", ctypes.c_int32), ("ldo", ctypes.c_int64), ("a", Operand), ("b", Operand)]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    L = ctypes.CDLL(os.path.join(ROOT, "fp64-emu_b200", "fp64_emu", "libf64e.so"))
+    vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    L.f64e_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp]
+    L.f64e_fp8_quantize_both.argtypes = [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp]
+    L.f64e_fp8_dequantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i64, i64, vp, i32, vp]
+    L.f64e_fp8_gemm.argtypes = [ctypes.POINTER(Problem), vp, vp, vp, vp, vp, vp]
+    L.f64e_last_error.restype = ctypes.c_char_p
+    return L
+
+
+P = 1 << 20   # a pointer value that no refused call may follow
+
+
+@pytest.mark.parametrize("args,msg", [
+    ((P, 7, 4, 16, 16, 0, 0, P, 16, P, None), "element type"),
+    ((P, 0, 4, 16, 16, 0, 2, P, 16, P, None), "code must be"),
+    ((P, 0, 4, 16, 16, 3, 0, P, 16, P, None), "blocks must be"),
+    ((P, 0, -1, 16, 16, 0, 0, P, 16, P, None), "negative"),
+    ((P, 0, 4, 1 << 31, 1 << 31, 0, 0, P, 1 << 31, P, None), "too large"),
+    ((None, 0, 4, 16, 16, 0, 0, P, 16, P, None), "null"),
+    ((P, 0, 4, 16, 15, 0, 0, P, 16, P, None), "pitch of x"),
+    ((P, 0, 4, 17, 17, 0, 0, P, 16, P, None), "below their columns"),
+    ((P, 0, 4, 17, 17, 0, 0, P, 24, P, None), "16-byte"),
+    ((P, 0, 4, 16, 16, 0, 0, P + 8, 16, P, None), "16-byte"),
+])
+def test_quantize_abi_refusals(lib, args, msg):
+    assert lib.f64e_fp8_quantize(*args) == 1
+    assert msg in lib.f64e_last_error().decode()
+
+
+def test_quantize_abi_empty_is_done_without_a_device(lib):
+    assert lib.f64e_fp8_quantize(None, 0, 0, 16, 16, 0, 0, None, 16, None, None) == 0
+    assert lib.f64e_fp8_quantize_both(None, 0, 5, 0, 0, 0, None, None, None, None, 0, None) == 0
+    assert lib.f64e_fp8_dequantize(None, 0, 0, 16, 16, 0, None, 1, 1, None, 0, None) == 0
+
+
+def good():
+    return Problem(64, 32, 256, 0, 0, 32, Operand(256, 0, 0, 2, 1), Operand(256, 0, 1, 2, 1))
+
+
+@pytest.mark.parametrize("change,msg", [
+    (dict(out_type=3), "element type"), (dict(layout=3), "layout"), (dict(M=-1), "negative"),
+    (dict(N=(1 << 30) + 1), "too large"), (dict(K=0), "at least 1"), (dict(ldo=31), "pitch of the output"),
+    (dict(a=Operand(255, 0, 0, 2, 1)), "below their columns"), (dict(a=Operand(264, 0, 0, 2, 1)), "16-byte"),
+    (dict(b=Operand(256, 2, 0, 2, 1)), "code must be"), (dict(b=Operand(256, 0, 2, 2, 1)), "tile must be"),
+])
+def test_gemm_abi_refusals(lib, change, msg):
+    p = good()
+    for k, v in change.items():
+        setattr(p, k, v)
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, P, P, P, P, None) == 1
+    assert msg in lib.f64e_last_error().decode()
+
+
+def test_gemm_abi_null_and_empty(lib):
+    p = good()
+    assert lib.f64e_fp8_gemm(None, P, P, P, P, P, None) == 1
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, None, P, P, P, None) == 1
+    p.M = 0
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), None, None, None, None, None, None) == 0
+
+
+# ------------------------------------------------------------------ fakes --
+def test_fake_kernels_give_shapes_and_types():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(200, 300, dtype=torch.bfloat16, device="cuda")
+        q, s = fp64_emu.quantize_fp8(x)
+        assert q.shape == (200, 300) and q.stride() == (304, 1) and q.dtype == E4
+        assert s.shape == (200, 3) and s.dtype == E8
+        assert fp64_emu.quantize_fp8(x, "col", E5)[1].shape == (2, 300)
+        assert fp64_emu.quantize_fp8(x, "tile")[1].shape == (2, 3)
+        q, s, qc, sc = fp64_emu.quantize_fp8_both(x)
+        assert s.shape == (200, 3) and sc.shape == (2, 300)
+        assert fp64_emu.dequantize_fp8(q, s, dtype=torch.float16).dtype == torch.float16
+        assert fp64_emu.mm_fp8(q, q, s, s).shape == (200, 200)
+        assert fp64_emu.mm_tn_fp8(qc, qc, sc, sc, torch.float32).shape == (300, 300)
+        assert fp64_emu.linear_fp8(torch.empty(2, 7, 300, device="cuda"), x.float()).shape == (2, 7, 200)
