@@ -16,6 +16,7 @@
 #include <cstdint>
 
 #include "f64e.h"
+#include "f64e_device.cuh"
 
 namespace f64e {
 
@@ -154,6 +155,112 @@ __device__ __forceinline__ uint2 codes8(const uint32_t* w, float r, bool special
     }
   }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+
+// ------------------------------------------------ block-scaled tcgen05 --
+// Everything below serves products of 8-bit codes whose 128-value blocks carry
+// power-of-two scales: the tensor cores take a scale per 32 values of k, read
+// from TMEM, so the four K = 32 instructions of a 128-value block read the
+// same one and the sums stay in one FP32 accumulator over all of K.
+
+// Bounded wait like mbar_wait, polling without sleeps (nothing else runs
+// beside these kernels' CTAs) and acquiring at cluster scope, for barriers
+// that the other CTA of a pair arrives on.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, "
+      "0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, uint64_t limit_ns, int* status,
+                                               int site) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; i++)
+      if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (globaltimer_ns() - t0 > limit_ns) {
+      record_status(status, site);
+      return false;
+    }
+  }
+}
+
+// 128 x 128-byte box of a 2-D map at (x, y): x along the contiguous direction.
+__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+// The same, counted on an mbarrier of either CTA of the pair (no multicast).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, int x, int y,
+                                                 uint32_t bar_cluster_addr) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+      "%3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster_addr)
+      : "memory");
+}
+
+// Generic-proxy writes to shared memory made visible to the tensor cores.
+__device__ __forceinline__ void fence_async_shared() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Instruction descriptor of kind::mxf8f6f4 with ue8m0 scales (bit 23): types
+// at bits 7-9 / 10-12 (0 e4m3, 1 e5m2), transposes (operand stored with M or N
+// contiguous) at bits 15 / 16, N >> 3 at bits 17-22, M >> 7 at bits 27-28.
+// The byte of the scale word each operand uses is added per instruction: B's
+// at bits 4-5, A's at bits 29-30.
+__host__ __device__ constexpr uint32_t idesc_mx(int M, int N, int a_code, int b_code, int a_mn, int b_mn) {
+  return ((uint32_t)a_code << 7) | ((uint32_t)b_code << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27);
+}
+__device__ __forceinline__ uint32_t idesc_scale_byte(uint32_t i) { return (i << 4) | (i << 29); }
+
+// Shared-memory descriptor of a scale atom: 32 rows of 16 bytes, 8-row core
+// matrices 128 bytes apart, no swizzle.  Row r holds the words of tile rows
+// r, r + 32, r + 64, r + 96, a word the scales of four neighbouring blocks.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(128 >> 4) << 32 |
+         (uint64_t)1 << 46;
+}
+
+// A scale atom to four TMEM columns, in every 32-lane quarter.
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// D[tmem] (+)= (A * scale)[smem] * (B * scale)[smem]^T, K = 32.
+__device__ __forceinline__ void mma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// A scale atom to four TMEM columns, in every 32-lane quarter of both CTAs, each from its own shared memory.
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// D[tmem] (+)= (A * scale)[smem] * (B * scale)[smem]^T, K = 32.
+__device__ __forceinline__ void mma_mx_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
 }
 
 }  // namespace f64e

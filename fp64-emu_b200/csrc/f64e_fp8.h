@@ -61,5 +61,7 @@ struct Fp8GemmArgs {
   int sms;
 };
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, cudaStream_t s);
+// The device's status word of these products, cleared by the read; synchronizes.
+cudaError_t read_fp8_status(int* status, cudaStream_t s);
 
 }  // namespace f64e

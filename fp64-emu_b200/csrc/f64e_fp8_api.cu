@@ -144,7 +144,7 @@ int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale,
     return bad("fp8: layout must be NT, NN or TN");
   if (p->M < 0 || p->N < 0 || p->K < 0) return bad("fp8: negative dimension");
   if (p->M > kMaxDim || p->N > kMaxDim || p->K > kMaxDim) return bad("fp8: dimension too large");
-  if ((p->M + 63) / 64 * ((p->N + 63) / 64) > 0x7FFFFFFF) return bad("fp8: product too large");
+  if ((p->M + 127) / 128 * ((p->N + 127) / 128) > 0x7FFFFFFF / 2) return bad("fp8: product too large");
   if (p->M == 0 || p->N == 0) return F64E_OK;
   if (p->K == 0) return bad("fp8: K must be at least 1");
   if (!A || !a_scale || !B || !b_scale || !out) return bad("fp8: null pointer");
@@ -176,6 +176,15 @@ int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale,
   g.wait_limit_ns = wait_limit_ns();
   if (const int rc = device_sms(&g.sms)) return rc;
   const cudaError_t e = launch_fp8_gemm(g, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+int f64e_fp8_status(void* stream, int32_t* status) {
+  begin_call();
+  if (!status) return bad("fp8: null argument");
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  const cudaError_t e = read_fp8_status(status, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? F64E_OK : cuda_error(e);
 }
 

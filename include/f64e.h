@@ -289,6 +289,12 @@ typedef struct f64e_fp8_problem {
 F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B,
                            const void* b_scale, void* out, void* stream);
 
+/* Status of the 8-bit products on the current device: 0, or the site code of
+ * the first bounded wait that ran out since the last read (the product's
+ * output is then not valid).  The codes of f64e_status, plus 6 and 7 (waits
+ * on scales).  Reading clears it.  Synchronizes the stream. */
+F64E_API int f64e_fp8_status(void* stream, int32_t* status);
+
 #ifdef __cplusplus
 }
 #endif
