@@ -60,7 +60,9 @@ struct Fp8GemmArgs {
   uint64_t wait_limit_ns;
   int sms;
 };
-cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, cudaStream_t s);
+// Scratch bytes the product needs (0: none).
+int64_t fp8_gemm_workspace(const Fp8GemmArgs& g);
+cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s);
 // The device's status word of these products, cleared by the read; synchronizes.
 cudaError_t read_fp8_status(int* status, cudaStream_t s);
 

@@ -43,6 +43,38 @@ const char* check_codes(const void* q, int64_t ldq, int64_t cols) {
   return nullptr;
 }
 
+// Sizes, types and pitches of a product; fills everything but the pointers.
+int check_problem(const f64e_fp8_problem* p, Fp8GemmArgs* g) {
+  if (!p) return bad("fp8: null problem");
+  if (const char* m = check_types(p->out_type, p->a.code)) return bad(m);
+  if (const char* m = check_types(p->out_type, p->b.code)) return bad(m);
+  if (p->M < 0 || p->N < 0 || p->K < 0) return bad("fp8: negative dimension");
+  if (p->M > kMaxDim || p->N > kMaxDim || p->K > kMaxDim) return bad("fp8: dimension too large");
+  if (blocks_of(p->M) * blocks_of(p->N) > 0x7FFFFFFF / 2 || blocks_of(p->K) * blocks_of(std::min(p->M, p->N)) > 0x7FFFFFFF)
+    return bad("fp8: product too large");
+  if (p->ldo < p->N) return bad("fp8: row pitch of the output is below its columns");
+  const f64e_fp8_operand* in[2] = {&p->a, &p->b};
+  Fp8Operand* o[2] = {&g->a, &g->b};
+  const int64_t rows[2] = {p->M, p->N};
+  for (int i = 0; i < 2; i++) {
+    if (in[i]->tile != 0 && in[i]->tile != 1) return bad("fp8: tile must be 0 or 1");
+    if (in[i]->k_major != 0 && in[i]->k_major != 1) return bad("fp8: k_major must be 0 or 1");
+    if (const char* m = check_codes(nullptr, in[i]->ld, in[i]->k_major ? p->K : rows[i])) return bad(m);
+    o[i]->kmajor = in[i]->k_major;
+    o[i]->ld = in[i]->ld;
+    o[i]->s_row = in[i]->scale_row;
+    o[i]->s_kb = in[i]->scale_block;
+    o[i]->s_shift = in[i]->tile ? 7 : 0;
+    o[i]->code = in[i]->code;
+  }
+  g->M = p->M;
+  g->N = p->N;
+  g->K = p->K;
+  g->ldo = p->ldo;
+  g->out_type = p->out_type;
+  return F64E_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -134,48 +166,34 @@ int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int64_t cols,
   return e == cudaSuccess ? F64E_OK : cuda_error(e);
 }
 
-int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B, const void* b_scale,
-                  void* out, void* stream) {
+size_t f64e_fp8_workspace_size(const f64e_fp8_problem* p) {
   begin_call();
-  if (!p) return bad("fp8: null problem");
-  if (const char* m = check_types(p->out_type, p->a.code)) return bad(m);
-  if (const char* m = check_types(p->out_type, p->b.code)) return bad(m);
-  if (p->layout != F64E_FP8_NT && p->layout != F64E_FP8_NN && p->layout != F64E_FP8_TN)
-    return bad("fp8: layout must be NT, NN or TN");
-  if (p->M < 0 || p->N < 0 || p->K < 0) return bad("fp8: negative dimension");
-  if (p->M > kMaxDim || p->N > kMaxDim || p->K > kMaxDim) return bad("fp8: dimension too large");
-  if ((p->M + 127) / 128 * ((p->N + 127) / 128) > 0x7FFFFFFF / 2) return bad("fp8: product too large");
+  Fp8GemmArgs g{};
+  if (check_problem(p, &g)) return 0;
+  return (size_t)fp8_gemm_workspace(g);
+}
+
+int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B, const void* b_scale,
+                  void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  begin_call();
+  Fp8GemmArgs g{};
+  if (const int rc = check_problem(p, &g)) return rc;
   if (p->M == 0 || p->N == 0) return F64E_OK;
   if (p->K == 0) return bad("fp8: K must be at least 1");
   if (!A || !a_scale || !B || !b_scale || !out) return bad("fp8: null pointer");
-  if (p->ldo < p->N) return bad("fp8: row pitch of the output is below its columns");
-  Fp8GemmArgs g{};
-  g.M = p->M;
-  g.N = p->N;
-  g.K = p->K;
-  const f64e_fp8_operand* in[2] = {&p->a, &p->b};
-  const void* q[2] = {A, B};
-  const void* sc[2] = {a_scale, b_scale};
-  Fp8Operand* o[2] = {&g.a, &g.b};
-  const int64_t rows[2] = {p->M, p->N};
-  for (int i = 0; i < 2; i++) {
-    o[i]->kmajor = i == 0 ? p->layout != F64E_FP8_TN : p->layout == F64E_FP8_NT;
-    if (const char* m = check_codes(q[i], in[i]->ld, o[i]->kmajor ? p->K : rows[i])) return bad(m);
-    if (in[i]->tile != 0 && in[i]->tile != 1) return bad("fp8: tile must be 0 or 1");
-    o[i]->q = static_cast<const uint8_t*>(q[i]);
-    o[i]->ld = in[i]->ld;
-    o[i]->s = static_cast<const uint8_t*>(sc[i]);
-    o[i]->s_row = in[i]->scale_row;
-    o[i]->s_kb = in[i]->scale_block;
-    o[i]->s_shift = in[i]->tile ? 7 : 0;
-    o[i]->code = in[i]->code;
-  }
+  if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15))
+    return bad("fp8: codes need 16-byte aligned rows");
+  g.a.q = static_cast<const uint8_t*>(A);
+  g.a.s = static_cast<const uint8_t*>(a_scale);
+  g.b.q = static_cast<const uint8_t*>(B);
+  g.b.s = static_cast<const uint8_t*>(b_scale);
   g.out = out;
-  g.ldo = p->ldo;
-  g.out_type = p->out_type;
+  const int64_t need = fp8_gemm_workspace(g);
+  if (need > 0 && (!workspace || workspace_bytes < (size_t)need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
+    return report_error(F64E_ERR_WORKSPACE, "fp8: workspace missing, too small or not 256-byte aligned");
   g.wait_limit_ns = wait_limit_ns();
   if (const int rc = device_sms(&g.sms)) return rc;
-  const cudaError_t e = launch_fp8_gemm(g, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_fp8_gemm(g, workspace, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? F64E_OK : cuda_error(e);
 }
 

@@ -22,46 +22,45 @@ __device__ int g_fp8_status;
 namespace {
 
 // ------------------------------------------------------------- epilogue --
-// A warp's 32 rows x 128 bytes of output, staged in shared memory so that
-// eight neighbouring lanes write one row's 128 bytes (16-byte chunks XORed
-// with the row: both sides free of bank conflicts).
-template <int OUT>
-struct OutOf;
-template <>
-struct OutOf<F64E_F32> {
-  static constexpr int kCols = 32;   // columns of a 128-byte row
-};
-template <>
-struct OutOf<F64E_F16> {
-  static constexpr int kCols = 64;
-};
-template <>
-struct OutOf<F64E_BF16> {
-  static constexpr int kCols = 64;
-};
+// A warp stages 2 KB of output rows in shared memory, 64 bytes of 32 rows (or
+// 128 bytes of 16), so that neighbouring lanes write neighbouring 16-byte
+// pieces of a row.  The pieces are XORed with the row number: both sides are
+// free of bank conflicts.
+constexpr uint32_t kStage = 2048;
 
 template <int OUT>
-__device__ __forceinline__ uint32_t pack2(uint32_t lo, uint32_t hi) {
+struct OutOf {
+  static constexpr int kBytes = OUT == F64E_F32 ? 4 : 2;
+};
+
+template <int RB>   // bytes of a staged row: 64 or 128
+__device__ __forceinline__ uint32_t staged_at(int row, int piece) {
+  return (uint32_t)(row * RB + ((RB == 64 ? piece ^ ((row >> 1) & 3) : piece ^ (row & 7)) << 4));
+}
+
+template <int OUT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if (OUT == F64E_F16) {
-    const __half2 h = __floats2half2_rn(__uint_as_float(lo), __uint_as_float(hi));
+    const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(lo), __uint_as_float(hi));
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Rows [0, rows) x columns [0, cols) of the staged block to out (row pitch
-// ldo elements); vec: 16-byte stores are aligned.
-template <int OUT>
+// The staged rows to out (row pitch ldo elements), of which `rows` rows and
+// `cols` columns exist; vec: 16-byte stores are aligned.
+template <int OUT, int RB>
 __device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, char* out, int64_t ldo, int rows,
                                              int cols, bool vec) {
-  constexpr int ES = OUT == F64E_F32 ? 4 : 2, COLS = OutOf<OUT>::kCols, PER = 16 / ES;
+  constexpr int ES = OutOf<OUT>::kBytes, PER = 16 / ES, LANES = RB / 16, AT_ONCE = 32 / LANES;
+  constexpr int ROWS = (int)kStage / RB;
   if (vec) {
-    const int ch = lane & 7;
+    const int ch = lane % LANES;
 #pragma unroll
-    for (int t = 0; t < 8; t++) {
-      const int r = t * 4 + (lane >> 3);
-      const uint8_t* s = stage + r * 128 + ((ch ^ (r & 7)) << 4);
+    for (int t = 0; t < ROWS / AT_ONCE; t++) {
+      const int r = t * AT_ONCE + lane / LANES;
+      const uint8_t* s = stage + staged_at<RB>(r, ch);
       const uint4 v = *reinterpret_cast<const uint4*>(s);
       char* o = out + (int64_t)r * ldo * ES + ch * 16;
       if (r < rows) {
@@ -80,67 +79,91 @@ __device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, cha
       }
     }
   } else {
+    constexpr int COLS = RB / ES, AT = 32 / COLS < 1 ? 1 : 32 / COLS;   // rows written at once
+    const int c = lane % COLS, ch = c / PER;
 #pragma unroll 4
-    for (int r = 0; r < 32; r++) {
-      if (r >= rows) break;
-#pragma unroll
-      for (int h = 0; h < COLS / 32; h++) {
-        const int c = h * 32 + lane, ch = c / PER;
-        const uint8_t* s = stage + r * 128 + ((ch ^ (r & 7)) << 4) + (c % PER) * ES;
-        char* o = out + ((int64_t)r * ldo + c) * ES;
-        if (c < cols) {
-          if (ES == 4)
-            *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(s);
-          else
-            *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(s);
-        }
+    for (int t = 0; t < ROWS; t += AT) {
+      const int r = t + lane / COLS;
+      const uint8_t* s = stage + staged_at<RB>(r, ch) + (c % PER) * ES;
+      char* o = out + ((int64_t)r * ldo + c) * ES;
+      if (r < rows && c < cols) {
+        if (ES == 4)
+          *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(s);
+        else
+          *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(s);
       }
     }
   }
 }
 
-// 32 FP32 accumulators of this lane's row into its staged row, from column
-// `half` * 32 on (half = 0 only, in 32 bits).
+// 64 / kBytes accumulators of this lane's row into its staged row.
 template <int OUT>
-__device__ __forceinline__ void stage32(uint8_t* stage, int lane, int half, const uint32_t (&v)[32]) {
-  uint8_t* row = stage + lane * 128;
-  if (OUT == F64E_F32) {
+__device__ __forceinline__ void stage_row(uint8_t* stage, int lane, const float* v) {
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      *reinterpret_cast<uint4*>(row + ((i ^ (lane & 7)) << 4)) =
-          make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      *reinterpret_cast<uint4*>(row + (((half * 4 + i) ^ (lane & 7)) << 4)) =
+  for (int i = 0; i < 4; i++)
+    if (OUT == F64E_F32)
+      *reinterpret_cast<float4*>(stage + staged_at<64>(lane, i)) =
+          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    else
+      *reinterpret_cast<uint4*>(stage + staged_at<64>(lane, i)) =
           make_uint4(pack2<OUT>(v[8 * i], v[8 * i + 1]), pack2<OUT>(v[8 * i + 2], v[8 * i + 3]),
                      pack2<OUT>(v[8 * i + 4], v[8 * i + 5]), pack2<OUT>(v[8 * i + 6], v[8 * i + 7]));
+}
+// The same of a transposed tile: this lane's accumulators are one column of
+// the staged rows (32 columns).
+template <int OUT>
+__device__ __forceinline__ void stage_column(uint8_t* stage, int lane, const float* v) {
+  constexpr int ES = OutOf<OUT>::kBytes, RB = 32 * ES, N = (int)kStage / RB;
+  const int ch = lane * ES / 16, at = lane * ES % 16;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    if (OUT == F64E_F32) {
+      *reinterpret_cast<float*>(stage + staged_at<RB>(i, ch) + at) = v[i];
+      *reinterpret_cast<float*>(stage + staged_at<RB>(i + 1, ch) + at) = v[i + 1];
+    } else {
+      const uint32_t p = pack2<OUT>(v[i], v[i + 1]);
+      *reinterpret_cast<uint16_t*>(stage + staged_at<RB>(i, ch) + at) = (uint16_t)p;
+      *reinterpret_cast<uint16_t*>(stage + staged_at<RB>(i + 1, ch) + at) = (uint16_t)(p >> 16);
+    }
   }
 }
 
 // --------------------------------------------------------------- scales --
-// The scale word of row r: bytes of blocks 4 j .. 4 j + 3, 0 outside the
-// operand (its codes read as zeros there, and 0 is a finite scale).
-__device__ __forceinline__ uint32_t scale_word(const Fp8Operand& o, int64_t rows, int nkb, int64_t r, int j,
-                                               bool words) {
-  if (r >= rows) return 0;
-  const uint8_t* p = o.s + (r >> o.s_shift) * o.s_row + (int64_t)(4 * j) * o.s_kb;
-  const int n = nkb - 4 * j;
-  if (words && n >= 4) return __ldg(reinterpret_cast<const uint32_t*>(p));
-  uint32_t w = 0;
+// Scale words of `N` atoms (rows r0 + 128 n + lane, + 32, + 64, + 96), a word
+// the bytes of blocks 4 j .. 4 j + 3.  Rows and blocks outside the operand read
+// their nearest neighbour's scale: their codes are zeros, and no store uses
+// them.  So no load depends on a branch, and all of them are in flight at once:
+// taken one word after the other they, not the MMAs, set the kernel's pace
+// where scales are strided bytes (4096 x 4096 x 8192 with column scales on
+// both sides: 231 us instead of 125).
+template <int N>
+__device__ __forceinline__ void scale_atoms(const Fp8Operand& o, int rows, int nkb, int r0, int j, int lane,
+                                            bool words, uint4* atoms) {
+  const uint8_t* p[4 * N];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (i < n) w |= (uint32_t)__ldg(p + i * o.s_kb) << (8 * i);
-  return w;
-}
-// The atom of rows r0 .. r0 + 127 (a warp; lane = row of the atom).
-__device__ __forceinline__ uint4 scale_atom(const Fp8Operand& o, int64_t rows, int nkb, int64_t r0, int j, int lane,
-                                            bool words) {
-  return make_uint4(scale_word(o, rows, nkb, r0 + lane, j, words), scale_word(o, rows, nkb, r0 + lane + 32, j, words),
-                    scale_word(o, rows, nkb, r0 + lane + 64, j, words),
-                    scale_word(o, rows, nkb, r0 + lane + 96, j, words));
+  for (int w = 0; w < 4 * N; w++)
+    p[w] = o.s + (int64_t)(min(r0 + w * 32 + lane, rows - 1) >> o.s_shift) * o.s_row;
+  uint32_t v[4 * N];
+  if (words && 4 * j + 4 <= nkb) {
+#pragma unroll
+    for (int w = 0; w < 4 * N; w++) v[w] = __ldg(reinterpret_cast<const uint32_t*>(p[w] + 4 * j));
+  } else {
+    uint32_t b[4 * N][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
+#pragma unroll
+      for (int w = 0; w < 4 * N; w++) b[w][i] = __ldg(p[w] + at);
+    }
+#pragma unroll
+    for (int w = 0; w < 4 * N; w++) v[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);
+  }
+#pragma unroll
+  for (int n = 0; n < N; n++) atoms[n] = make_uint4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
 }
 
+// The kernel's view of a product: a tile has rows of operand a and columns of
+// operand b.  out element (row, col) is at row * ldo + col, or transposed.
 struct GemmK {
   Fp8Operand a, b;
   int M, N, nkb;
@@ -155,23 +178,37 @@ struct GemmK {
 // --------------------------------------------------------------- CTA pair --
 // A cluster of two CTAs on two SMs computes a 256 x 256 tile: CTA r holds rows
 // [128 r, +128) of A's and of B's half tiles, and the leader's tcgen05.mma
-// works on both.  Per SM and K = 32 step the tensor core then reads 8 KB of
-// shared memory for 2^20 products; a lone CTA's 128 x 256 tile reads 12.
-//   warp 0      TMA: 128 x 128 boxes of A and B, 128-byte swizzle, 5 stages
-//   warp 1      TMEM owner; the leader's elected thread issues scale copies
-//               and MMAs and commits stages and tiles to both CTAs
-//   warps 2, 3  scales: gathered into atoms for 4 blocks of k at a time
-//   warps 4..7  epilogue: 128 TMEM lanes, 32 columns at a time
+// works on both, so an SM stages 32 KB for 128 values of k where a lone CTA's
+// 128 x 256 tile would stage 48.
+//   warp 0       TMA: 128 x 128 boxes of A and B, 6 stages
+//   warp 1       TMEM owner; the leader's elected thread issues scale copies
+//                and MMAs and commits stages and sums to both CTAs
+//   warps 2, 3   scales: gathered into atoms for 4 blocks of k at a time
+//   warps 4..11  epilogue: two warps for each 32 TMEM lanes, half the columns
+//                each
+// TMEM holds two accumulators, so MMAs run on while a tile is drained.  They
+// and the scales exceed its 512 columns: the accumulators overlap by 32
+// columns, which the epilogue drains first.
+// Operand storage: the tensor cores read an MN-major A as fast as a K-major
+// one, but take 1.75 times as long over an MN-major B (measured on resident
+// tiles, 4096^3).  Such products are therefore computed transposed, with the
+// operands' roles exchanged (TRANS), or after a transposition of one operand
+// (launch_fp8_gemm).
+// Sums: the tensor core truncates what an addition shifts out, an error that
+// grows with the number of additions (measured at K = 16384: 3e-6 of the
+// result's norm).  For 32-bit outputs the accumulator therefore restarts after
+// kChunk blocks of k and the parts are added in registers; 16-bit outputs keep
+// one accumulator, since their own rounding is 100 times that.
 // Every wait is bounded; one that runs out records its site and unwinds the
 // CTA: copies and MMAs in flight are waited for before TMEM is freed (see the
 // end of the kernel).
-constexpr int BK = kFp8Block, BN = 256, PBM = 256, PHALF = 128, STAGES = 5, SF_STAGES = 4, PGROUP_M = 8;
-constexpr int PTHREADS = 256;
-constexpr uint32_t TILE_BYTES = PHALF * BK, STAGE_BYTES = 2 * TILE_BYTES;
+constexpr int BK = kFp8Block, BN = 256, PBM = 256, PHALF = 128, STAGES = 6, SF_STAGES = 4, PGROUP_M = 8;
+constexpr int EPI_WARPS = 8, PTHREADS = 32 * (4 + EPI_WARPS);
+constexpr int kChunk = 16;   // 2048 values of k
 constexpr uint32_t ATOM = 512, SF_BYTES = 3 * ATOM;   // A's rows, B's rows 0-127, 128-255
-constexpr uint32_t STAGING = 4 * 32 * 128;
-constexpr size_t PSMEM = 1024 + (size_t)STAGES * STAGE_BYTES + STAGING + SF_STAGES * SF_BYTES + 256;
-constexpr uint32_t TMEM_COLS = 512, SF_COL = 256, SF_COLS = 12;   // scales: two buffers of 4 + 8 columns
+constexpr uint32_t TILE_BYTES = PHALF * BK, STAGE_BYTES = 2 * TILE_BYTES;
+constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 224, SF_COL = 480, SF_COLS = 12;   // scales: two buffers of 4 + 8
+constexpr size_t PSMEM = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * kStage + SF_STAGES * SF_BYTES + 256;
 
 enum : int { kWaitScales = 6, kWaitScalesFree = 7 };
 
@@ -183,7 +220,7 @@ __device__ __forceinline__ void tile_origin(int tile, int ntm, int ntn, int& m0,
   n0 = (o / mh) * BN;
 }
 
-template <int OUT>
+template <int OUT, bool TRANS>
 __global__ void __launch_bounds__(PTHREADS, 1)
     fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB,
                          const __grid_constant__ GemmK g) {
@@ -193,7 +230,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * TILE_BYTES;
   uint8_t* staging = smem + STAGES * STAGE_BYTES;
-  uint8_t* sSF = staging + STAGING;
+  uint8_t* sSF = staging + EPI_WARPS * kStage;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSF + SF_STAGES * SF_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sf_full = empty_bar + STAGES;
@@ -210,6 +247,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   const bool leader = rank == 0;
   const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   const int ntm = (g.M + PBM - 1) / PBM, ntn = (g.N + BN - 1) / BN, ntiles = ntm * ntn;
+  const int chunk = OUT == F64E_F32 ? kChunk : g.nkb;   // blocks of k per accumulator
   int* status = &g_fp8_status;
 
   if (threadIdx.x == 0) {
@@ -222,7 +260,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       mbar_init(&sf_empty[s], 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 2 * 4);   // the epilogue warps of both CTAs
+    mbar_init(acc_empty, 2 * EPI_WARPS);   // the epilogue warps of both CTAs
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     *peer_issued = 0;
@@ -277,16 +315,22 @@ __global__ void __launch_bounds__(PTHREADS, 1)
     if (leader && elect_one()) {
       uint32_t j = 0, it = 0, gr = 0;
       uint32_t last[2] = {0, 0};   // one past the last stage that used each scale buffer
-      const uint32_t a_step = g.a.kmajor ? 32 : 32 * BK, b_step = g.b.kmajor ? 32 : 32 * BK;
+      // K = 32 further on: 32 bytes along a K-major row, 32 rows of an MN-major box
+      const uint32_t a_step = g.a.kmajor ? 32 : 32 * PHALF, b_step = g.b.kmajor ? 32 : 32 * PHALF;
       bool ok = true;
-      for (int tile = cluster; tile < ntiles && ok; tile += nclusters, it++) {
-        if (!mbar_wait_poll(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) || *abort_flag) {
-          *abort_flag = 1;
-          break;
-        }
-        tc_fence_after();
-        uint32_t sf = 0;
-        for (int kb = 0; kb < g.nkb; kb++, j++) {
+      for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
+        uint32_t sf = 0, d_tmem = 0;
+        for (int kb = 0, left = 0; kb < g.nkb; kb++, j++, left--) {
+          if (left == 0) {   // a new accumulator
+            if (!mbar_wait_poll(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) || *abort_flag) {
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            d_tmem = tmem + (it & 1) * ACC_COLS;
+            it++;
+            left = min(chunk, g.nkb - kb);
+          }
           if ((kb & 3) == 0) {
             const uint32_t ss = gr % SF_STAGES, buf = gr & 1;
             bool got = mbar_wait_poll(&sf_full[ss], (gr / SF_STAGES) & 1, lim, status, kWaitScales);
@@ -321,19 +365,20 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           last[(gr - 1) & 1] = j + 1;
           const uint32_t a_addr = smem_u32(sA + s * TILE_BYTES), b_addr = smem_u32(sB + s * TILE_BYTES);
           const uint32_t id = g.idesc | idesc_scale_byte(kb & 3);
+          const bool first = kb % chunk == 0;
 #pragma unroll
           for (int kk = 0; kk < BK / 32; kk++)
-            mma_mx_pair(tmem, smem_desc_sw128(a_addr + kk * a_step), smem_desc_sw128(b_addr + kk * b_step), id, sf,
-                        sf + 4, (kb | kk) != 0);
+            mma_mx_pair(d_tmem, smem_desc_sw128(a_addr + kk * a_step), smem_desc_sw128(b_addr + kk * b_step), id, sf,
+                        sf + 4, !first || kk != 0);
           tc_commit_pair(&empty_bar[s], 0x3);
+          if (left == 1) tc_commit_pair(acc_full, 0x3);
         }
-        if (ok) tc_commit_pair(acc_full, 0x3);
       }
       tc_commit_pair(drain_bar, 0x1);
       mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain);
     }
   } else if (warp < 4) {
-    // Scales: warp 2 gathers A's atom (this CTA's rows), warp 3 both of B's.
+    // Scales: warp 2 gathers A's atom (this CTA's rows), warp 3 those of B.
     uint32_t gr = 0;
     bool ok = true;
     for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
@@ -342,23 +387,21 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       for (int kb = 0; kb < g.nkb; kb += 4, gr++) {
         const uint32_t ss = gr % SF_STAGES;
         uint8_t* dst = sSF + ss * SF_BYTES + lane * 16;
-        uint4 u, v;
-        if (warp == 2) {
-          u = scale_atom(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, g.a_words);
-        } else {
-          u = scale_atom(g.b, g.N, g.nkb, n0, kb >> 2, lane, g.b_words);
-          v = scale_atom(g.b, g.N, g.nkb, n0 + 128, kb >> 2, lane, g.b_words);
-        }
+        uint4 u[2];
+        if (warp == 2)
+          scale_atoms<1>(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, g.a_words, u);
+        else
+          scale_atoms<2>(g.b, g.N, g.nkb, n0, kb >> 2, lane, g.b_words, u);
         if (!mbar_wait_poll(&sf_empty[ss], ((gr / SF_STAGES) & 1) ^ 1, lim, status, kWaitScalesFree) || *abort_flag) {
           *abort_flag = 1;
           ok = false;
           break;
         }
         if (warp == 2) {
-          *reinterpret_cast<uint4*>(dst) = u;
+          *reinterpret_cast<uint4*>(dst) = u[0];
         } else {
-          *reinterpret_cast<uint4*>(dst + ATOM) = u;
-          *reinterpret_cast<uint4*>(dst + 2 * ATOM) = v;
+          *reinterpret_cast<uint4*>(dst + ATOM) = u[0];
+          *reinterpret_cast<uint4*>(dst + 2 * ATOM) = u[1];
         }
         fence_async_shared();
         __syncwarp();
@@ -366,38 +409,72 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       }
     }
   } else {
-    const int q = warp & 3;
-    constexpr int ES = OUT == F64E_F32 ? 4 : 2, COLS = OutOf<OUT>::kCols;
-    uint8_t* stage = staging + q * (32 * 128);
+    // Epilogue: warp q of 4 by lanes, half h of the columns.  A warp arrives on
+    // acc_empty once per accumulator, after its first 32 columns of it: by then
+    // it has left the other accumulator, and the columns both share (the last
+    // of the first accumulator, the first of the second) are in registers,
+    // since the half that holds them starts there.
+    const int q = warp & 3, h = (warp - 4) >> 2;
+    constexpr int ES = OutOf<OUT>::kBytes, COLS = 64 / ES, NP = BN / 2 / COLS;   // columns and number of a warp's passes
+    uint8_t* stage = staging + (warp - 4) * kStage;
     uint32_t it = 0;
-    for (int tile = cluster; tile < ntiles; tile += nclusters, it++) {
+    bool ok = true;
+    for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
       int m0, n0;
       tile_origin(tile, ntm, ntn, m0, n0);
-      if (!mbar_wait_poll(acc_full, it & 1, lim, status, kWaitAccFull) || *abort_flag) {
-        *abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
       const int row0 = m0 + PHALF * (int)rank + q * 32;
-      const int rows = min(32, g.M - row0);
-      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-#pragma unroll 1
-      for (int c = 0; c < BN; c += COLS) {
-#pragma unroll
-        for (int h = 0; h < COLS / 32; h++) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(taddr + c + h * 32, v);
-          tmem_wait_ld();
-          stage32<OUT>(stage, lane, h, v);
-        }
-        if (c + COLS >= BN) {   // the tile has left TMEM
-          tc_fence_before();
+      auto column = [&](int p) { return h * (BN / 2) + (h ? NP - 1 - p : p) * COLS; };
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(accempty0);
+      };
+      auto put = [&](int p, const float* v) {
+        const int col0 = n0 + column(p);
+        if (TRANS) {
+          stage_column<OUT>(stage, lane, v);
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(accempty0);
+          store_staged<OUT, 32 * ES>(stage, lane, g.out + ((int64_t)col0 * g.ldo + row0) * ES, g.ldo, g.N - col0,
+                                     g.M - row0, g.vec);
+        } else {
+          stage_row<OUT>(stage, lane, v);
+          __syncwarp();
+          store_staged<OUT, 64>(stage, lane, g.out + ((int64_t)row0 * g.ldo + col0) * ES, g.ldo, g.M - row0,
+                                g.N - col0, g.vec);
         }
         __syncwarp();
-        store_staged<OUT>(stage, lane, g.out + ((int64_t)row0 * g.ldo + n0 + c) * ES, g.ldo, rows, g.N - n0 - c, g.vec);
-        __syncwarp();
+      };
+      float sum[OUT == F64E_F32 ? NP : 1][COLS];
+      for (int kb = 0; kb < g.nkb; kb += chunk, it++) {
+        if (!mbar_wait_poll(acc_full, it & 1, lim, status, kWaitAccFull) || *abort_flag) {
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (it & 1) * ACC_COLS;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          if (OUT == F64E_F32) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(taddr + column(p), v);
+            tmem_wait_ld();
+            if (p == 1) release();   // 32 columns
+#pragma unroll
+            for (int k = 0; k < 16; k++)
+              sum[p][k] = kb == 0 ? __uint_as_float(v[k]) : sum[p][k] + __uint_as_float(v[k]);
+          } else {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(taddr + column(p), v);
+            tmem_wait_ld();
+            if (p == 0) release();
+            put(p, reinterpret_cast<const float*>(v));
+          }
+        }
+      }
+      if (OUT == F64E_F32 && ok) {
+#pragma unroll
+        for (int p = 0; p < NP; p++) put(p, sum[p]);
       }
     }
   }
@@ -426,9 +503,9 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   }
 }
 
-// Codes as TMA sees them: 128 x 128-byte boxes of a [outer][inner] byte matrix
-// with row pitch ld (a multiple of 16), zeros outside.
-bool encode_codes(CUtensorMap* map, const void* base, int64_t outer, int64_t inner, int64_t ld) {
+// An operand as TMA sees it: 128 x 128 boxes of a byte matrix with pitch ld (a
+// multiple of 16), 128-byte swizzle, zeros outside.
+bool encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K) {
   using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -441,11 +518,11 @@ bool encode_codes(CUtensorMap* map, const void* base, int64_t outer, int64_t inn
     return reinterpret_cast<EncodeFn>(f);
   }();
   if (!fn) return false;
-  const cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-  const cuuint64_t gstride[1] = {(cuuint64_t)ld};
+  const cuuint64_t gdim[2] = {(cuuint64_t)(o.kmajor ? K : rows), (cuuint64_t)(o.kmajor ? rows : K)};
+  const cuuint64_t gstride[1] = {(cuuint64_t)o.ld};
   const cuuint32_t box[2] = {128, 128};
   const cuuint32_t estride[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), gdim, gstride, box, estride,
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(o.q), gdim, gstride, box, estride,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -454,9 +531,10 @@ bool scale_words(const Fp8Operand& o) {
   return o.s_kb == 1 && o.s_row % 4 == 0 && (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
 }
 
-template <int OUT>
-cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const GemmK& k, int sms, cudaStream_t s) {
-  const int64_t tiles = (int64_t)((k.M + PBM - 1) / PBM) * ((k.N + BN - 1) / BN);
+template <int OUT, bool TRANS>
+cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
+  CUtensorMap ta, tb;
+  if (!encode_codes(&ta, k.a, k.M, K) || !encode_codes(&tb, k.b, k.N, K)) return cudaErrorInvalidValue;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -478,42 +556,124 @@ cudaError_t launch_pair(const CUtensorMap& ta, const CUtensorMap& tb, const Gemm
   std::unique_lock<std::mutex> lk(mtx);
   int& max_clusters = clusters_of.emplace(dev, -1).first->second;
   if (max_clusters < 0) {
-    e = cudaFuncSetAttribute(fp8_gemm_pair_kernel<OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PSMEM);
+    e = cudaFuncSetAttribute(fp8_gemm_pair_kernel<OUT, TRANS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PSMEM);
     if (e != cudaSuccess) return e;
     int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel<OUT>, &cfg);
+    e = cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel<OUT, TRANS>, &cfg);
     if (e != cudaSuccess) return e;
     max_clusters = std::max(n, 1);
   }
+  const int64_t tiles = (int64_t)((k.M + PBM - 1) / PBM) * ((k.N + BN - 1) / BN);
   cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_clusters), 1, 1);
   lk.unlock();
-  return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<OUT>, ta, tb, k);
+  return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<OUT, TRANS>, ta, tb, k);
+}
+
+template <int OUT>
+cudaError_t launch_out(const GemmK& k, bool trans, int64_t K, int sms, cudaStream_t s) {
+  return trans ? launch_pair<OUT, true>(k, K, sms, s) : launch_pair<OUT, false>(k, K, sms, s);
+}
+
+// ------------------------------------------------------ transposed copies --
+// [K][rows] codes to [rows][ldt], zeros up to ldt (K rounded up to 16): squares
+// of 128 x 128 through shared memory, 4 x 4 bytes transposed in registers.
+__global__ void __launch_bounds__(256) fp8_transpose_kernel(const uint8_t* q, int64_t ld, int64_t rows, int64_t K,
+                                                            uint8_t* t, int64_t ldt, int64_t nrb) {
+  __shared__ uint32_t sm[128][33];   // [row][k / 4], one word of padding
+  const int64_t r0 = (blockIdx.x % nrb) * 128, k0 = (blockIdx.x / nrb) * 128;
+  const int rg = threadIdx.x & 31, kg0 = threadIdx.x >> 5;   // 4 rows by 4 k each
+  uint32_t w[4][4];
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t k = k0 + (u * 8 + kg0) * 4 + i, r = r0 + rg * 4;
+      const uint8_t* p = q + k * ld + r;
+      uint32_t v = 0;
+      if (k < K) {
+        if (r + 4 <= rows) {
+          v = __ldg(reinterpret_cast<const uint32_t*>(p));
+        } else {
+#pragma unroll
+          for (int b = 0; b < 4; b++)
+            if (r + b < rows) v |= (uint32_t)__ldg(p + b) << (8 * b);
+        }
+      }
+      w[u][i] = v;
+    }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const uint32_t a = __byte_perm(w[u][0], w[u][1], 0x5140), b = __byte_perm(w[u][2], w[u][3], 0x5140);
+    const uint32_t c = __byte_perm(w[u][0], w[u][1], 0x7362), d = __byte_perm(w[u][2], w[u][3], 0x7362);
+    const int kg = u * 8 + kg0;
+    sm[rg * 4][kg] = __byte_perm(a, b, 0x5410);
+    sm[rg * 4 + 1][kg] = __byte_perm(a, b, 0x7632);
+    sm[rg * 4 + 2][kg] = __byte_perm(c, d, 0x5410);
+    sm[rg * 4 + 3][kg] = __byte_perm(c, d, 0x7632);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int row = u * 32 + (threadIdx.x >> 3), ch = threadIdx.x & 7;
+    const int64_t r = r0 + row, k = k0 + ch * 16;
+    if (r < rows && k < ldt)
+      *reinterpret_cast<uint4*>(t + r * ldt + k) =
+          make_uint4(sm[row][ch * 4], sm[row][ch * 4 + 1], sm[row][ch * 4 + 2], sm[row][ch * 4 + 3]);
+  }
+}
+
+int64_t round16(int64_t v) { return (v + 15) & ~(int64_t)15; }
+
+// Whether one of two MN-major operands is transposed first: where the time won
+// on the tensor cores (waves of tiles times blocks of k) exceeds a launch and
+// a pass over the smaller operand.
+bool transpose_first(int64_t M, int64_t N, int64_t K, int sms) {
+  const int64_t tiles = ((M + PBM - 1) / PBM) * ((N + BN - 1) / BN);
+  const int64_t waves = (tiles + sms / 2 - 1) / (sms / 2);
+  return waves * ((K + BK - 1) / BK) >= 32;
 }
 
 }  // namespace
 
-cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, cudaStream_t s) {
-  CUtensorMap ta, tb;
-  const bool ok = encode_codes(&ta, g.a.q, g.a.kmajor ? g.M : g.K, g.a.kmajor ? g.K : g.M, g.a.ld) &&
-                  encode_codes(&tb, g.b.q, g.b.kmajor ? g.N : g.K, g.b.kmajor ? g.K : g.N, g.b.ld);
-  if (!ok) return cudaErrorInvalidValue;
+int64_t fp8_gemm_workspace(const Fp8GemmArgs& g) {
+  if (g.a.kmajor || g.b.kmajor || !transpose_first(g.M, g.N, g.K, 148)) return 0;
+  return std::min(g.M, g.N) * round16(g.K);
+}
+
+cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s) {
   GemmK k;
   k.a = g.a;
   k.b = g.b;
-  k.M = (int)g.M;
-  k.N = (int)g.N;
+  const int64_t need = fp8_gemm_workspace(g);
+  if (need > 0) {
+    const bool a_side = g.M < g.N;
+    Fp8Operand& o = a_side ? k.a : k.b;
+    const int64_t rows = a_side ? g.M : g.N, nrb = (rows + 127) / 128;
+    uint8_t* t = static_cast<uint8_t*>(workspace);
+    fp8_transpose_kernel<<<(unsigned)(nrb * ((g.K + 127) / 128)), 256, 0, s>>>(o.q, o.ld, rows, g.K, t, round16(g.K),
+                                                                               nrb);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    o.q = t;
+    o.ld = round16(g.K);
+    o.kmajor = 1;
+  }
+  const bool trans = !k.b.kmajor && k.a.kmajor;   // the MN-major operand takes A's place
+  if (trans) std::swap(k.a, k.b);
+  k.M = (int)(trans ? g.N : g.M);
+  k.N = (int)(trans ? g.M : g.N);
   k.nkb = (int)((g.K + BK - 1) / BK);
   k.ldo = g.ldo;
   k.out = static_cast<char*>(g.out);
   k.wait_limit_ns = g.wait_limit_ns;
-  k.idesc = idesc_mx(PBM, BN, g.a.code, g.b.code, !g.a.kmajor, !g.b.kmajor);
-  k.a_words = scale_words(g.a);
-  k.b_words = scale_words(g.b);
+  k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
+  k.a_words = scale_words(k.a);
+  k.b_words = scale_words(k.b);
   k.vec = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
   switch (g.out_type) {
-    case F64E_F32: return launch_pair<F64E_F32>(ta, tb, k, g.sms, s);
-    case F64E_F16: return launch_pair<F64E_F16>(ta, tb, k, g.sms, s);
-    default: return launch_pair<F64E_BF16>(ta, tb, k, g.sms, s);
+    case F64E_F32: return launch_out<F64E_F32>(k, trans, g.K, g.sms, s);
+    case F64E_F16: return launch_out<F64E_F16>(k, trans, g.K, g.sms, s);
+    default: return launch_out<F64E_BF16>(k, trans, g.K, g.sms, s);
   }
 }
 

@@ -374,6 +374,8 @@ int fp8_type(at::ScalarType t) {
 int fp8_code(at::ScalarType t) {
   return t == at::kFloat8_e4m3fn ? F64E_E4M3 : t == at::kFloat8_e5m2 ? F64E_E5M2 : -1;
 }
+// Shapes of a product's operands: A [M, K] B [N, K], A [M, K] B [K, N], A [K, M] B [K, N].
+enum { kFp8NT = 0, kFp8NN = 1, kFp8TN = 2 };
 int64_t fp8_blocks(int64_t n) { return (n + 127) / 128; }
 
 void fp8_check_float(const at::Tensor& x, const char* what) {
@@ -464,19 +466,29 @@ void fp8_check_operand(const at::Tensor& q, const at::Tensor& s, int kdim, const
   TORCH_CHECK(sk == fp8_blocks(k) && (sr == r || sr == fp8_blocks(r)), name, ": scales of shape ", s.sizes(),
               " do not fit codes of shape ", q.sizes(), " with blocks of 128 along the contracted dimension");
 }
+// Whether the rows of the stored codes start on 16-byte boundaries, with
+// `fast` the contiguous dimension.
+bool fp8_aligned(const at::Tensor& q, int fast) {
+  const int64_t n = q.size(fast), m = q.size(1 - fast);
+  return (n <= 1 || q.stride(fast) == 1) && (m <= 1 || (q.stride(1 - fast) % 16 == 0 && q.stride(1 - fast) >= n)) &&
+         (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15) == 0;
+}
 Fp8Held fp8_hold(const at::Tensor& q, const at::Tensor& s, int kdim) {
   Fp8Held h;
-  const int64_t r = q.size(1 - kdim), C = q.size(1);
+  int fast = 1;
   h.q = q;
-  int64_t ld = q.size(0) <= 1 ? fp8_code_pitch(C) : q.stride(0);
-  if ((C > 1 && q.stride(1) != 1) || ld % 16 != 0 || ld < C || (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15)) {
-    h.q = fp8_new_codes(q, q.size(0), C, q.scalar_type());
-    h.q.copy_(q);
-    ld = fp8_code_pitch(C);
+  if (!fp8_aligned(q, 1)) {
+    if (fp8_aligned(q, 0)) {
+      fast = 0;
+    } else {
+      h.q = fp8_new_codes(q, q.size(0), q.size(1), q.scalar_type());
+      h.q.copy_(q);
+    }
   }
-  h.o.ld = ld;
+  h.o.ld = h.q.size(1 - fast) <= 1 ? fp8_code_pitch(h.q.size(fast)) : h.q.stride(1 - fast);
+  h.o.k_major = fast == kdim;
   h.o.code = fp8_code(q.scalar_type());
-  h.o.tile = s.size(1 - kdim) == r ? 0 : 1;
+  h.o.tile = s.size(1 - kdim) == q.size(1 - kdim) ? 0 : 1;
   h.o.scale_row = s.stride(1 - kdim);
   h.o.scale_block = s.stride(kdim);
   return h;
@@ -484,8 +496,8 @@ Fp8Held fp8_hold(const at::Tensor& q, const at::Tensor& s, int kdim) {
 
 at::Tensor fp8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa, const at::Tensor& sb, int64_t layout,
                   at::ScalarType dtype) {
-  TORCH_CHECK(layout >= F64E_FP8_NT && layout <= F64E_FP8_TN, "layout must be 0 (NT), 1 (NN) or 2 (TN)");
-  const int ka = layout == F64E_FP8_TN ? 0 : 1, kb = layout == F64E_FP8_NT ? 1 : 0;
+  TORCH_CHECK(layout >= kFp8NT && layout <= kFp8TN, "layout must be 0 (NT), 1 (NN) or 2 (TN)");
+  const int ka = layout == kFp8TN ? 0 : 1, kb = layout == kFp8NT ? 1 : 0;
   fp8_check_operand(a, sa, ka, "A");
   fp8_check_operand(b, sb, kb, "B");
   TORCH_CHECK(a.size(ka) == b.size(kb), "inner dimensions differ");
@@ -500,13 +512,15 @@ at::Tensor fp8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa
   p.M = a.size(1 - ka);
   p.N = b.size(1 - kb);
   p.K = a.size(ka);
-  p.layout = (int32_t)layout;
   p.out_type = fp8_type(dtype);
   p.ldo = p.N;
   p.a = ha.o;
   p.b = hb.o;
   at::Tensor out = at::empty({p.M, p.N}, a.options().dtype(dtype));
-  check(f64e_fp8_gemm(&p, ha.q.data_ptr(), sa.data_ptr(), hb.q.data_ptr(), sb.data_ptr(), out.data_ptr(), stream_of()));
+  const size_t nb = f64e_fp8_workspace_size(&p);
+  const at::Tensor ws = nb ? at::empty({(int64_t)nb}, a.options().dtype(at::kByte)) : at::Tensor();
+  check(f64e_fp8_gemm(&p, ha.q.data_ptr(), sa.data_ptr(), hb.q.data_ptr(), sb.data_ptr(), out.data_ptr(),
+                      nb ? ws.data_ptr() : nullptr, nb, stream_of()));
   return out;
 }
 
@@ -541,7 +555,7 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optio
     wsc = *ws;
   else
     std::tie(wq, wsc) = fp8_quantize(w, F64E_BLOCKS_TILE, at::kFloat8_e4m3fn);
-  at::Tensor y = fp8_mm(q, wq, s, wsc, F64E_FP8_NT, x.scalar_type());
+  at::Tensor y = fp8_mm(q, wq, s, wsc, kFp8NT, x.scalar_type());
   return x.dim() == 2 ? y : y.view(fp8_out_sizes(x, w.size(0)));
 }
 
@@ -593,7 +607,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       wsc = *ws;
     else
       std::tie(wq, wsc) = call_quantize(w, F64E_BLOCKS_TILE);
-    at::Tensor y = call_mm(q, wq, s, wsc, F64E_FP8_NT, x.scalar_type());
+    at::Tensor y = call_mm(q, wq, s, wsc, kFp8NT, x.scalar_type());
     const bool want_x = x.requires_grad();
     ctx->save_for_backward({want_x ? wq : at::Tensor(), want_x ? wsc : at::Tensor(), qc, sc});
     ctx->saved_data["x_sizes"] = x.sizes().vec();
@@ -620,13 +634,13 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       else
         std::tie(gc, gsc) = call_quantize(g, F64E_BLOCKS_COL);
       if (want_x) {
-        dx = call_mm(q, wq, s, wsc, F64E_FP8_NN, (at::ScalarType)ctx->saved_data["x_type"].toInt());
+        dx = call_mm(q, wq, s, wsc, kFp8NN, (at::ScalarType)ctx->saved_data["x_type"].toInt());
         const auto sizes = ctx->saved_data["x_sizes"].toIntVector();
         if (sizes.size() != 2) dx = dx.view(sizes);
       }
       if (want_w) {
         const auto wt = (at::ScalarType)ctx->saved_data["w_type"].toInt();
-        dw = g.size(0) > 0 ? call_mm(gc, qc, gsc, sc, F64E_FP8_TN, wt)
+        dw = g.size(0) > 0 ? call_mm(gc, qc, gsc, sc, kFp8TN, wt)
                            : at::zeros({g.size(1), qc.size(1)}, g.options().dtype(wt));
       }
     }

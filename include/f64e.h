@@ -263,31 +263,35 @@ F64E_API int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int6
                                  int32_t blocks, const void* scale, int64_t scale_row, int64_t scale_col,
                                  void* out, int32_t out_type, void* stream);
 
-/* Layouts of the products: out [M, N] = A @ B with */
-enum {
-  F64E_FP8_NT = 0, /* A [M, K], B [N, K]: scales along the rows of both */
-  F64E_FP8_NN = 1, /* A [M, K], B [K, N]: along A's rows and B's columns */
-  F64E_FP8_TN = 2  /* A [K, M], B [K, N]: along the columns of both */
-};
+/* out [M, N] = sum over k of a[m, k] * b[n, k].  An operand's codes are stored
+ * with k contiguous (k_major = 1: [M, K] or [N, K]) or with m / n contiguous
+ * ([K, M] or [K, N]); its scales are per 128 neighbours along k, or per
+ * 128 x 128 square. */
 typedef struct f64e_fp8_operand {
   int64_t ld;          /* row pitch of the codes, a multiple of 16 */
   int32_t code;        /* F64E_E4M3 or F64E_E5M2 */
   int32_t tile;        /* 1: one scale per 128 x 128 square, 0: per 128 contracted values */
+  int32_t k_major;
   int64_t scale_row;   /* bytes from one scale to the next across M or N (or across squares) */
   int64_t scale_block; /* bytes from one scale to the next along K */
 } f64e_fp8_operand;
 typedef struct f64e_fp8_problem {
   int64_t M, N, K;
-  int32_t layout;   /* F64E_FP8_* */
   int32_t out_type; /* F64E_F32, F64E_F16, F64E_BF16 */
   int64_t ldo;      /* row pitch of out, in elements */
   f64e_fp8_operand a, b;
 } f64e_fp8_problem;
 
+/* Scratch bytes of the product; 0 when it needs none (or its arguments are
+ * refused: f64e_last_error() then says why).  Only products of two operands
+ * that both have m / n contiguous need scratch. */
+F64E_API size_t f64e_fp8_workspace_size(const f64e_fp8_problem* p);
+
 /* The product of the values codes and scales stand for; sums are held in 32
- * bits and rounded once. */
+ * bits and rounded once.  workspace: at least f64e_fp8_workspace_size() bytes
+ * of device memory, 256-byte aligned, or NULL where that is 0. */
 F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B,
-                           const void* b_scale, void* out, void* stream);
+                           const void* b_scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Status of the 8-bit products on the current device: 0, or the site code of
  * the first bounded wait that ran out since the last read (the product's

@@ -100,12 +100,11 @@ def test_unknown_blocks_are_refused():
 # ------------------------------------------------------------------- ABI --
 class Operand(ctypes.Structure):
     _fields_ = [("ld", ctypes.c_int64), ("code", ctypes.c_int32), ("tile", ctypes.c_int32),
-                ("scale_row", ctypes.c_int64), ("scale_block", ctypes.c_int64)]
+                ("k_major", ctypes.c_int32), ("scale_row", ctypes.c_int64), ("scale_block", ctypes.c_int64)]
 
 
 class Problem(ctypes.Structure):
-    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("layout", ctypes.c_int32),
-                ("out_type", ctypes.c_int32), ("ldo", ctypes.c_int64), ("a", Operand), ("b", Operand)]
+    _fields_ = [("M", ctypes.c_int64), ("N", ctypes.c_int64), ("K", ctypes.c_int64), ("out_type", ctypes.c_int32), ("ldo", ctypes.c_int64), ("a", Operand), ("b", Operand)]
 
 
 @pytest.fixture(scope="module")
@@ -115,7 +114,9 @@ def lib():
     L.f64e_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp]
     L.f64e_fp8_quantize_both.argtypes = [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp]
     L.f64e_fp8_dequantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i64, i64, vp, i32, vp]
-    L.f64e_fp8_gemm.argtypes = [ctypes.POINTER(Problem), vp, vp, vp, vp, vp, vp]
+    L.f64e_fp8_gemm.argtypes = [ctypes.POINTER(Problem), vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    L.f64e_fp8_workspace_size.argtypes = [ctypes.POINTER(Problem)]
+    L.f64e_fp8_workspace_size.restype = ctypes.c_size_t
     L.f64e_last_error.restype = ctypes.c_char_p
     return L
 
@@ -147,29 +148,45 @@ def test_quantize_abi_empty_is_done_without_a_device(lib):
 
 
 def good():
-    return Problem(64, 32, 256, 0, 0, 32, Operand(256, 0, 0, 2, 1), Operand(256, 0, 1, 2, 1))
+    return Problem(64, 32, 256, 0, 32, Operand(256, 0, 0, 1, 2, 1), Operand(256, 0, 1, 1, 2, 1))
 
 
 @pytest.mark.parametrize("change,msg", [
-    (dict(out_type=3), "element type"), (dict(layout=3), "layout"), (dict(M=-1), "negative"),
+    (dict(out_type=3), "element type"), (dict(M=-1), "negative"),
     (dict(N=(1 << 30) + 1), "too large"), (dict(K=0), "at least 1"), (dict(ldo=31), "pitch of the output"),
-    (dict(a=Operand(255, 0, 0, 2, 1)), "below their columns"), (dict(a=Operand(264, 0, 0, 2, 1)), "16-byte"),
-    (dict(b=Operand(256, 2, 0, 2, 1)), "code must be"), (dict(b=Operand(256, 0, 2, 2, 1)), "tile must be"),
+    (dict(a=Operand(255, 0, 0, 1, 2, 1)), "below their columns"), (dict(a=Operand(264, 0, 0, 1, 2, 1)), "16-byte"),
+    (dict(b=Operand(256, 2, 0, 1, 2, 1)), "code must be"), (dict(b=Operand(256, 0, 2, 1, 2, 1)), "tile must be"),
+    (dict(b=Operand(256, 0, 0, 2, 2, 1)), "k_major must be"), (dict(b=Operand(16, 0, 0, 0, 2, 1)), "below their columns"),
 ])
 def test_gemm_abi_refusals(lib, change, msg):
     p = good()
     for k, v in change.items():
         setattr(p, k, v)
-    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, P, P, P, P, None) == 1
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, P, P, P, P, None, 0, None) == 1
     assert msg in lib.f64e_last_error().decode()
 
 
 def test_gemm_abi_null_and_empty(lib):
     p = good()
-    assert lib.f64e_fp8_gemm(None, P, P, P, P, P, None) == 1
-    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, None, P, P, P, None) == 1
+    assert lib.f64e_fp8_gemm(None, P, P, P, P, P, None, 0, None) == 1
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), P, None, P, P, P, None, 0, None) == 1
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), P + 4, P, P, P, P, None, 0, None) == 1
+    assert "16-byte" in lib.f64e_last_error().decode()
     p.M = 0
-    assert lib.f64e_fp8_gemm(ctypes.byref(p), None, None, None, None, None, None) == 0
+    assert lib.f64e_fp8_gemm(ctypes.byref(p), None, None, None, None, None, None, 0, None) == 0
+
+
+def test_gemm_abi_workspace(lib):
+    p = good()
+    assert lib.f64e_fp8_workspace_size(ctypes.byref(p)) == 0
+    p = Problem(2048, 4096, 16380, 0, 4096, Operand(2048, 0, 0, 0, 1, 2048), Operand(4096, 0, 0, 0, 1, 4096))
+    need = lib.f64e_fp8_workspace_size(ctypes.byref(p))
+    assert need == 2048 * 16384
+    for ws, nb in ((None, need), (P, need - 1), (P + 16, need)):
+        assert lib.f64e_fp8_gemm(ctypes.byref(p), P, P, P, P, P, ws, nb, None) == 2
+        assert "workspace" in lib.f64e_last_error().decode()
+    p.b.k_major, p.b.ld = 1, 16384
+    assert lib.f64e_fp8_workspace_size(ctypes.byref(p)) == 0
 
 
 # ------------------------------------------------------------------ fakes --
