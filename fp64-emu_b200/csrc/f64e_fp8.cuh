@@ -164,9 +164,12 @@ __device__ __forceinline__ uint2 codes8(const uint32_t* w, float r, bool special
 // same one and the sums stay in one FP32 accumulator over all of K.
 
 // Bounded wait like mbar_wait, polling without sleeps (nothing else runs
-// beside these kernels' CTAs) and acquiring at cluster scope, for barriers
-// that the other CTA of a pair arrives on.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+// beside these kernels' CTAs).  CLUSTER: acquires at cluster scope, for a
+// barrier that orders the other CTA's shared-memory writes; the acquire costs
+// some 270 cycles, so the waits on copies and MMAs, every block of k, go without.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  if (!CLUSTER) return mbar_try_wait(bar, parity);
   uint32_t ok;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, "
@@ -176,14 +179,15 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, uint64_t limit_ns, int* status,
                                                int site) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
+  if (mbar_test<CLUSTER>(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
   while (true) {
 #pragma unroll 1
     for (int i = 0; i < 64; i++)
-      if (mbar_try_wait_cluster(bar, parity)) return true;
+      if (mbar_test<CLUSTER>(bar, parity)) return true;
     if (globaltimer_ns() - t0 > limit_ns) {
       record_status(status, site);
       return false;
@@ -208,6 +212,33 @@ __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* m
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster_addr)
       : "memory");
 }
+
+// Box of shared memory to a 2-D map at (x, y), clipped at its extents; done
+// (shared memory read) when the thread's bulk groups say so.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, const void* src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(smem_u32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int LEFT>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// Arrival on an mbarrier of either CTA that orders no memory (what it signals
+// is a tcgen05.ld that has completed): a release at cluster scope would wait
+// 550 cycles for the warp's stores.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The two halves of a cluster barrier; a warp's lanes may reach them apart.
+// The relaxed arrival orders nothing but barriers set up before fence_barrier_init().
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Generic-proxy writes to shared memory made visible to the tensor cores.
 __device__ __forceinline__ void fence_async_shared() {

@@ -23,9 +23,10 @@ namespace {
 
 // ------------------------------------------------------------- epilogue --
 // A warp stages 2 KB of output rows in shared memory, 64 bytes of 32 rows (or
-// 128 bytes of 16), so that neighbouring lanes write neighbouring 16-byte
-// pieces of a row.  The pieces are XORed with the row number: both sides are
-// free of bank conflicts.
+// 128 bytes of 16), 16-byte pieces XORed with the row number as in TMA's
+// swizzle, which keeps the writes free of bank conflicts.  From there a TMA
+// store takes them, or, where the output's rows are not on 16-byte boundaries,
+// the warp itself, neighbouring lanes writing neighbouring elements.
 constexpr uint32_t kStage = 2048;
 
 template <int OUT>
@@ -49,49 +50,23 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // The staged rows to out (row pitch ldo elements), of which `rows` rows and
-// `cols` columns exist; vec: 16-byte stores are aligned.
+// `cols` columns exist.
 template <int OUT, int RB>
 __device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, char* out, int64_t ldo, int rows,
-                                             int cols, bool vec) {
-  constexpr int ES = OutOf<OUT>::kBytes, PER = 16 / ES, LANES = RB / 16, AT_ONCE = 32 / LANES;
-  constexpr int ROWS = (int)kStage / RB;
-  if (vec) {
-    const int ch = lane % LANES;
-#pragma unroll
-    for (int t = 0; t < ROWS / AT_ONCE; t++) {
-      const int r = t * AT_ONCE + lane / LANES;
-      const uint8_t* s = stage + staged_at<RB>(r, ch);
-      const uint4 v = *reinterpret_cast<const uint4*>(s);
-      char* o = out + (int64_t)r * ldo * ES + ch * 16;
-      if (r < rows) {
-        if (ch * PER + PER <= cols) {
-          *reinterpret_cast<uint4*>(o) = v;
-        } else {
-#pragma unroll
-          for (int i = 0; i < PER; i++)
-            if (ch * PER + i < cols) {
-              if (ES == 4)
-                reinterpret_cast<uint32_t*>(o)[i] = reinterpret_cast<const uint32_t*>(s)[i];
-              else
-                reinterpret_cast<uint16_t*>(o)[i] = reinterpret_cast<const uint16_t*>(s)[i];
-            }
-        }
-      }
-    }
-  } else {
-    constexpr int COLS = RB / ES, AT = 32 / COLS < 1 ? 1 : 32 / COLS;   // rows written at once
-    const int c = lane % COLS, ch = c / PER;
+                                             int cols) {
+  constexpr int ES = OutOf<OUT>::kBytes, PER = 16 / ES, COLS = RB / ES;
+  constexpr int ROWS = (int)kStage / RB, AT = 32 / COLS;   // staged rows, rows written at once
+  const int c = lane % COLS, ch = c / PER;
 #pragma unroll 4
-    for (int t = 0; t < ROWS; t += AT) {
-      const int r = t + lane / COLS;
-      const uint8_t* s = stage + staged_at<RB>(r, ch) + (c % PER) * ES;
-      char* o = out + ((int64_t)r * ldo + c) * ES;
-      if (r < rows && c < cols) {
-        if (ES == 4)
-          *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(s);
-        else
-          *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(s);
-      }
+  for (int t = 0; t < ROWS; t += AT) {
+    const int r = t + lane / COLS;
+    const uint8_t* s = stage + staged_at<RB>(r, ch) + (c % PER) * ES;
+    char* o = out + ((int64_t)r * ldo + c) * ES;
+    if (r < rows && c < cols) {
+      if (ES == 4)
+        *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(s);
+      else
+        *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(s);
     }
   }
 }
@@ -172,7 +147,7 @@ struct GemmK {
   uint64_t wait_limit_ns;
   uint32_t idesc;
   int a_words, b_words;   // scales may be read four at a time
-  int vec;                // 16-byte stores of the output are aligned
+  int tma_out;            // the output's rows start on 16-byte boundaries
 };
 
 // --------------------------------------------------------------- CTA pair --
@@ -180,7 +155,7 @@ struct GemmK {
 // [128 r, +128) of A's and of B's half tiles, and the leader's tcgen05.mma
 // works on both, so an SM stages 32 KB for 128 values of k where a lone CTA's
 // 128 x 256 tile would stage 48.
-//   warp 0       TMA: 128 x 128 boxes of A and B, 6 stages
+//   warp 0       TMA: 128 x 128 boxes of A and B, 5 stages
 //   warp 1       TMEM owner; the leader's elected thread issues scale copies
 //                and MMAs and commits stages and sums to both CTAs
 //   warps 2, 3   scales: gathered into atoms for 4 blocks of k at a time
@@ -202,13 +177,13 @@ struct GemmK {
 // Every wait is bounded; one that runs out records its site and unwinds the
 // CTA: copies and MMAs in flight are waited for before TMEM is freed (see the
 // end of the kernel).
-constexpr int BK = kFp8Block, BN = 256, PBM = 256, PHALF = 128, STAGES = 6, SF_STAGES = 4, PGROUP_M = 8;
+constexpr int BK = kFp8Block, BN = 256, PBM = 256, PHALF = 128, STAGES = 5, SF_STAGES = 4, PGROUP_M = 8;
 constexpr int EPI_WARPS = 8, PTHREADS = 32 * (4 + EPI_WARPS);
 constexpr int kChunk = 16;   // 2048 values of k
 constexpr uint32_t ATOM = 512, SF_BYTES = 3 * ATOM;   // A's rows, B's rows 0-127, 128-255
 constexpr uint32_t TILE_BYTES = PHALF * BK, STAGE_BYTES = 2 * TILE_BYTES;
 constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 224, SF_COL = 480, SF_COLS = 12;   // scales: two buffers of 4 + 8
-constexpr size_t PSMEM = 1024 + (size_t)STAGES * STAGE_BYTES + EPI_WARPS * kStage + SF_STAGES * SF_BYTES + 256;
+constexpr size_t PSMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 2 * EPI_WARPS * kStage + SF_STAGES * SF_BYTES + 256;
 
 enum : int { kWaitScales = 6, kWaitScalesFree = 7 };
 
@@ -223,14 +198,14 @@ __device__ __forceinline__ void tile_origin(int tile, int ntm, int ntn, int& m0,
 template <int OUT, bool TRANS>
 __global__ void __launch_bounds__(PTHREADS, 1)
     fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB,
-                         const __grid_constant__ GemmK g) {
+                         const __grid_constant__ CUtensorMap tmapO, const __grid_constant__ GemmK g) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_s = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * TILE_BYTES;
   uint8_t* staging = smem + STAGES * STAGE_BYTES;
-  uint8_t* sSF = staging + EPI_WARPS * kStage;
+  uint8_t* sSF = staging + 2 * EPI_WARPS * kStage;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSF + SF_STAGES * SF_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sf_full = empty_bar + STAGES;
@@ -241,6 +216,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile uint32_t* peer_issued = reinterpret_cast<volatile uint32_t*>(tmem_slot + 2);
+  volatile uint32_t* all_done = reinterpret_cast<volatile uint32_t*>(tmem_slot + 3);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -264,48 +240,84 @@ __global__ void __launch_bounds__(PTHREADS, 1)
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     *peer_issued = 0;
+    *all_done = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tmapA);
     tma_prefetch_desc(&tmapB);
   }
-  __syncwarp();
-  // TMEM: allocated by both CTAs once both run, the permit given up once both
-  // have it (see residue_gemm_pair_kernel).
-  cluster_sync();
-  if (warp == 1) tmem_alloc_pair(tmem_slot, TMEM_COLS);
-  tc_fence_before();
-  __syncwarp();
-  cluster_sync();
-  tc_fence_after();
-  if (warp == 1) tmem_relinquish_pair();
-  const uint32_t tmem = *tmem_slot;
+  // What can start early does: the first scales are gathered (two dependent
+  // loads) while the CTAs of the pair meet and are handed over by the barrier
+  // of the TMEM allocation; copies begin when both CTAs' barriers are known to
+  // be set up.  One after the other, the first MMA came 3.5 us into the kernel.
   const uint64_t lim = g.wait_limit_ns;
+  int m0, n0;
+  tile_origin(cluster, ntm, ntn, m0, n0);
+  uint4 atoms[2];
+  auto gather = [&](int kb) {
+    if (warp == 2)
+      scale_atoms<1>(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, g.a_words, atoms);
+    else
+      scale_atoms<2>(g.b, g.N, g.nkb, n0, kb >> 2, lane, g.b_words, atoms);
+  };
+  __syncwarp();
+  cluster_arrive_relaxed();
+  if (warp == 2 || warp == 3) gather(0);
+  cluster_wait();
   const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
   const uint32_t sffull0 = mapa_shared(smem_u32(sf_full), 0);
   const uint32_t accempty0 = mapa_shared(smem_u32(acc_empty), 0);
+  auto stage_scales = [&](uint32_t ss) {
+    uint8_t* dst = sSF + ss * SF_BYTES + lane * 16;
+    if (warp == 2) {
+      *reinterpret_cast<uint4*>(dst) = atoms[0];
+    } else {
+      *reinterpret_cast<uint4*>(dst + ATOM) = atoms[0];
+      *reinterpret_cast<uint4*>(dst + 2 * ATOM) = atoms[1];
+    }
+    fence_async_shared();
+    __syncwarp();
+  };
+  auto load = [&](uint32_t s, int kb) {
+    const int k = kb * BK, ra = m0 + PHALF * (int)rank, rb = n0 + PHALF * (int)rank;
+    if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * STAGE_BYTES);
+    tma_load_2d_pair(sA + s * TILE_BYTES, &tmapA, g.a.kmajor ? k : ra, g.a.kmajor ? ra : k, full0 + 8 * s);
+    tma_load_2d_pair(sB + s * TILE_BYTES, &tmapB, g.b.kmajor ? k : rb, g.b.kmajor ? rb : k, full0 + 8 * s);
+  };
+  // TMEM: allocated by both CTAs once both run, the permit given up at the end
+  // (see residue_gemm_pair_kernel).
+  const bool uses_tmem = warp == 1 || warp >= 4;
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, TMEM_COLS);
+    tc_fence_before();
+    __syncwarp();
+  }
+  if (warp == 2 || warp == 3) stage_scales(0);
+  cluster_arrive();
+  const bool producer = warp == 0 && elect_one();
+  const int head = min(STAGES, g.nkb);   // blocks loaded ahead
+  if (producer)
+    for (int kb = 0; kb < head; kb++) load(kb, kb);
+  if (uses_tmem) {
+    cluster_wait();
+    tc_fence_after();
+  }
+  const uint32_t tmem = uses_tmem ? *tmem_slot : 0;
 
   uint32_t issued = 0;
-  bool producer = false;
   if (warp == 0) {
-    producer = elect_one();
     if (producer) {
-      uint32_t j = 0;
+      uint32_t j = head;
       bool ok = true;
       for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
-        int m0, n0;
         tile_origin(tile, ntm, ntn, m0, n0);
-        const int ra = m0 + PHALF * (int)rank, rb = n0 + PHALF * (int)rank;
-        for (int kb = 0; kb < g.nkb; kb++, j++) {
+        for (int kb = tile == cluster ? head : 0; kb < g.nkb; kb++, j++) {
           const uint32_t s = j % STAGES, ph = (j / STAGES) & 1;
           if (!mbar_wait_poll(&empty_bar[s], ph ^ 1, lim, status, kWaitEmpty) || *abort_flag) {
             *abort_flag = 1;
             ok = false;
             break;
           }
-          const int k = kb * BK;
-          if (leader) mbar_arrive_expect_tx(&full_bar[s], 2 * STAGE_BYTES);
-          tma_load_2d_pair(sA + s * TILE_BYTES, &tmapA, g.a.kmajor ? k : ra, g.a.kmajor ? ra : k, full0 + 8 * s);
-          tma_load_2d_pair(sB + s * TILE_BYTES, &tmapB, g.b.kmajor ? k : rb, g.b.kmajor ? rb : k, full0 + 8 * s);
+          load(s, kb);
         }
       }
       issued = j;
@@ -333,7 +345,9 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           }
           if ((kb & 3) == 0) {
             const uint32_t ss = gr % SF_STAGES, buf = gr & 1;
-            bool got = mbar_wait_poll(&sf_full[ss], (gr / SF_STAGES) & 1, lim, status, kWaitScales);
+            // (group 0 came with the allocation's barrier)
+            bool got = gr == 0 || mbar_wait_poll<true>(&sf_full[ss], ((gr / SF_STAGES) & 1) ^ (ss == 0), lim, status,
+                                                       kWaitScales);
             // The buffer's earlier MMAs have completed: by the ring (a stage
             // is filled again only after them), else by their own commit.
             if (got && last[buf] + STAGES > j + 1 && last[buf] > 0) {
@@ -374,37 +388,27 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           if (left == 1) tc_commit_pair(acc_full, 0x3);
         }
       }
+      // Every copy was waited for above and every MMA is waited for here: both
+      // CTAs may then leave at the next barrier.
       tc_commit_pair(drain_bar, 0x1);
-      mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain);
+      if (mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain) && ok)
+        for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa_shared(smem_u32((const void*)all_done), r), 1);
     }
   } else if (warp < 4) {
     // Scales: warp 2 gathers A's atom (this CTA's rows), warp 3 those of B.
-    uint32_t gr = 0;
+    uint32_t gr = 1;
     bool ok = true;
     for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
-      int m0, n0;
       tile_origin(tile, ntm, ntn, m0, n0);
-      for (int kb = 0; kb < g.nkb; kb += 4, gr++) {
+      for (int kb = tile == cluster ? 4 : 0; kb < g.nkb; kb += 4, gr++) {
         const uint32_t ss = gr % SF_STAGES;
-        uint8_t* dst = sSF + ss * SF_BYTES + lane * 16;
-        uint4 u[2];
-        if (warp == 2)
-          scale_atoms<1>(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, g.a_words, u);
-        else
-          scale_atoms<2>(g.b, g.N, g.nkb, n0, kb >> 2, lane, g.b_words, u);
+        gather(kb);
         if (!mbar_wait_poll(&sf_empty[ss], ((gr / SF_STAGES) & 1) ^ 1, lim, status, kWaitScalesFree) || *abort_flag) {
           *abort_flag = 1;
           ok = false;
           break;
         }
-        if (warp == 2) {
-          *reinterpret_cast<uint4*>(dst) = u[0];
-        } else {
-          *reinterpret_cast<uint4*>(dst + ATOM) = u[0];
-          *reinterpret_cast<uint4*>(dst + 2 * ATOM) = u[1];
-        }
-        fence_async_shared();
-        __syncwarp();
+        stage_scales(ss);
         if (lane == 0) mbar_arrive_cluster(sffull0 + 8 * ss);
       }
     }
@@ -416,33 +420,43 @@ __global__ void __launch_bounds__(PTHREADS, 1)
     // since the half that holds them starts there.
     const int q = warp & 3, h = (warp - 4) >> 2;
     constexpr int ES = OutOf<OUT>::kBytes, COLS = 64 / ES, NP = BN / 2 / COLS;   // columns and number of a warp's passes
-    uint8_t* stage = staging + (warp - 4) * kStage;
-    uint32_t it = 0;
+    uint32_t it = 0, puts = 0;
     bool ok = true;
     for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
-      int m0, n0;
       tile_origin(tile, ntm, ntn, m0, n0);
       const int row0 = m0 + PHALF * (int)rank + q * 32;
       auto column = [&](int p) { return h * (BN / 2) + (h ? NP - 1 - p : p) * COLS; };
       auto release = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(accempty0);
+        if (lane == 0) mbar_arrive_cluster_relaxed(accempty0);
       };
       auto put = [&](int p, const float* v) {
+        constexpr int RB = TRANS ? 32 * ES : 64;
         const int col0 = n0 + column(p);
-        if (TRANS) {
-          stage_column<OUT>(stage, lane, v);
+        uint8_t* stage = staging + (2 * (warp - 4) + (puts++ & 1)) * kStage;
+        if (g.tma_out) {   // the store before the last has been read
+          if (lane == 0) tma_store_wait_read<1>();
           __syncwarp();
-          store_staged<OUT, 32 * ES>(stage, lane, g.out + ((int64_t)col0 * g.ldo + row0) * ES, g.ldo, g.N - col0,
-                                     g.M - row0, g.vec);
-        } else {
-          stage_row<OUT>(stage, lane, v);
-          __syncwarp();
-          store_staged<OUT, 64>(stage, lane, g.out + ((int64_t)row0 * g.ldo + col0) * ES, g.ldo, g.M - row0,
-                                g.N - col0, g.vec);
         }
-        __syncwarp();
+        if (TRANS)
+          stage_column<OUT>(stage, lane, v);
+        else
+          stage_row<OUT>(stage, lane, v);
+        if (g.tma_out) {
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0 && row0 < g.M && col0 < g.N) tma_store_2d(&tmapO, TRANS ? row0 : col0, TRANS ? col0 : row0, stage);
+        } else {
+          __syncwarp();
+          if (TRANS)
+            store_staged<OUT, RB>(stage, lane, g.out + ((int64_t)col0 * g.ldo + row0) * ES, g.ldo, g.N - col0,
+                                  g.M - row0);
+          else
+            store_staged<OUT, RB>(stage, lane, g.out + ((int64_t)row0 * g.ldo + col0) * ES, g.ldo, g.M - row0,
+                                  g.N - col0);
+          __syncwarp();
+        }
       };
       float sum[OUT == F64E_F32 ? NP : 1][COLS];
       for (int kb = 0; kb < g.nkb; kb += chunk, it++) {
@@ -477,38 +491,41 @@ __global__ void __launch_bounds__(PTHREADS, 1)
         for (int p = 0; p < NP; p++) put(p, sum[p]);
       }
     }
+    if (lane == 0) tma_store_wait();   // shared memory outlives the stores
   }
 
+  __syncwarp();
+  if (!uses_tmem) cluster_wait();   // the allocation's barrier
   tc_fence_before();
-  __syncwarp();
-  cluster_sync();   // the peer's stage count is visible; the leader's MMAs have drained
-  if (producer && leader) {
-    // Every copy of the pair lands before either CTA releases its shared
-    // memory: the accounting of residue_gemm_pair_kernel.
-    const uint32_t jp = *peer_issued;
-    const uint32_t jmax = issued > jp ? issued : jp;
-    const uint32_t lo = jmax > (uint32_t)STAGES ? jmax - STAGES : 0;
-    for (uint32_t jj = lo; jj < jmax; jj++) {
-      const uint32_t s = jj % STAGES;
-      if (jj >= issued) mbar_arrive_expect_tx(&full_bar[s], STAGE_BYTES);
-      else if (jj >= jp) mbar_complete_tx(&full_bar[s], STAGE_BYTES);
-      mbar_wait_poll(&full_bar[s], (jj / STAGES) & 1, drain_limit(lim), status, kWaitDrain);
+  cluster_sync();   // the leader's MMAs have drained; the peer's stage count is visible
+  if (!*all_done) {
+    // A wait ran out.  Every copy of the pair lands before either CTA releases
+    // its shared memory: the accounting of residue_gemm_pair_kernel.
+    if (producer && leader) {
+      const uint32_t jp = *peer_issued;
+      const uint32_t jmax = issued > jp ? issued : jp;
+      const uint32_t lo = jmax > (uint32_t)STAGES ? jmax - STAGES : 0;
+      for (uint32_t jj = lo; jj < jmax; jj++) {
+        const uint32_t s = jj % STAGES;
+        if (jj >= issued) mbar_arrive_expect_tx(&full_bar[s], STAGE_BYTES);
+        else if (jj >= jp) mbar_complete_tx(&full_bar[s], STAGE_BYTES);
+        mbar_wait_poll(&full_bar[s], (jj / STAGES) & 1, drain_limit(lim), status, kWaitDrain);
+      }
     }
+    __syncwarp();
+    cluster_sync();
   }
-  __syncwarp();
-  cluster_sync();
   if (warp == 1) {
     tc_fence_after();
+    tmem_relinquish_pair();
     tmem_dealloc_pair(tmem, TMEM_COLS);
   }
 }
 
-// An operand as TMA sees it: 128 x 128 boxes of a byte matrix with pitch ld (a
-// multiple of 16), 128-byte swizzle, zeros outside.
-bool encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K) {
-  using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
   static EncodeFn fn = [] {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult qr;
@@ -517,14 +534,32 @@ bool encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K
       f = nullptr;
     return reinterpret_cast<EncodeFn>(f);
   }();
+  return fn;
+}
+bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
+               int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle) {
+  const EncodeFn fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t gdim[2] = {(cuuint64_t)(o.kmajor ? K : rows), (cuuint64_t)(o.kmajor ? rows : K)};
-  const cuuint64_t gstride[1] = {(cuuint64_t)o.ld};
-  const cuuint32_t box[2] = {128, 128};
+  const cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t gstride[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
   const cuuint32_t estride[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(o.q), gdim, gstride, box, estride,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return fn(map, type, 2, base, gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// An operand as TMA sees it: 128 x 128 boxes of a byte matrix with pitch ld (a
+// multiple of 16), 128-byte swizzle, zeros outside.
+bool encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K) {
+  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(o.q), o.kmajor ? K : rows,
+                   o.kmajor ? rows : K, o.ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// The output in boxes of one staged block.
+template <int OUT, bool TRANS>
+bool encode_out(CUtensorMap* map, const GemmK& k) {
+  constexpr int ES = OutOf<OUT>::kBytes, RB = TRANS ? 32 * ES : 64;
+  return encode_2d(map, ES == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, k.out,
+                   TRANS ? k.M : k.N, TRANS ? k.N : k.M, k.ldo * ES, RB / ES, (int)kStage / RB,
+                   RB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool scale_words(const Fp8Operand& o) {
@@ -534,7 +569,10 @@ bool scale_words(const Fp8Operand& o) {
 template <int OUT, bool TRANS>
 cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   CUtensorMap ta, tb;
-  if (!encode_codes(&ta, k.a, k.M, K) || !encode_codes(&tb, k.b, k.N, K)) return cudaErrorInvalidValue;
+  CUtensorMap to = {};
+  if (!encode_codes(&ta, k.a, k.M, K) || !encode_codes(&tb, k.b, k.N, K) ||
+      (k.tma_out && !encode_out<OUT, TRANS>(&to, k)))
+    return cudaErrorInvalidValue;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -566,7 +604,7 @@ cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   const int64_t tiles = (int64_t)((k.M + PBM - 1) / PBM) * ((k.N + BN - 1) / BN);
   cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_clusters), 1, 1);
   lk.unlock();
-  return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<OUT, TRANS>, ta, tb, k);
+  return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<OUT, TRANS>, ta, tb, to, k);
 }
 
 template <int OUT>
@@ -669,7 +707,7 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
   k.a_words = scale_words(k.a);
   k.b_words = scale_words(k.b);
-  k.vec = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
+  k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
   switch (g.out_type) {
     case F64E_F32: return launch_out<F64E_F32>(k, trans, g.K, g.sms, s);
     case F64E_F16: return launch_out<F64E_F16>(k, trans, g.K, g.sms, s);
