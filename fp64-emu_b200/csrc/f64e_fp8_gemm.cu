@@ -324,75 +324,91 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       if (!leader) st_cluster_u32(mapa_shared(smem_u32((const void*)peer_issued), 0), j);
     }
   } else if (warp == 1) {
-    if (leader && elect_one()) {
-      uint32_t j = 0, it = 0, gr = 0;
-      uint32_t last[2] = {0, 0};   // one past the last stage that used each scale buffer
-      // K = 32 further on: 32 bytes along a K-major row, 32 rows of an MN-major box
-      const uint32_t a_step = g.a.kmajor ? 32 : 32 * PHALF, b_step = g.b.kmajor ? 32 : 32 * PHALF;
+    if (leader) {
+      // The whole warp runs the loop, so its counters and descriptors are
+      // uniform; one thread issues.  A block of k has 512 cycles before the
+      // tensor cores run dry, which the loop must not exceed: stage counters
+      // instead of divisions, descriptors by addition, and no check of the
+      // abort flag where a wait would notice.
+      const bool issuer = elect_one();
+      // K = 32 further on: 32 bytes along a K-major row, 32 rows of an MN-major box (in 16-byte units)
+      const uint32_t a_step = (g.a.kmajor ? 32 : 32 * PHALF) >> 4, b_step = (g.b.kmajor ? 32 : 32 * PHALF) >> 4;
+      const uint64_t desc_a = smem_desc_sw128(smem_u32(sA)), desc_b = smem_desc_sw128(smem_u32(sB));
+      const uint64_t desc_sf = smem_desc_scales(smem_u32(sSF));
+      uint32_t s = 0, ph = 0;        // stage and its parity
+      uint32_t ss = 0, sph = 0;      // scale stage and its parity
+      uint32_t j = 0, prev = 0;      // stages so far; where the previous group of 4 began
+      uint32_t it = 0, gr = 0;
       bool ok = true;
       for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
-        uint32_t sf = 0, d_tmem = 0;
-        for (int kb = 0, left = 0; kb < g.nkb; kb++, j++, left--) {
-          if (left == 0) {   // a new accumulator
-            if (!mbar_wait_poll(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) || *abort_flag) {
-              *abort_flag = 1;
-              ok = false;
-              break;
-            }
-            d_tmem = tmem + (it & 1) * ACC_COLS;
-            it++;
-            left = min(chunk, g.nkb - kb);
-          }
-          if ((kb & 3) == 0) {
-            const uint32_t ss = gr % SF_STAGES, buf = gr & 1;
-            // (group 0 came with the allocation's barrier)
-            bool got = gr == 0 || mbar_wait_poll<true>(&sf_full[ss], ((gr / SF_STAGES) & 1) ^ (ss == 0), lim, status,
-                                                       kWaitScales);
-            // The buffer's earlier MMAs have completed: by the ring (a stage
-            // is filled again only after them), else by their own commit.
-            if (got && last[buf] + STAGES > j + 1 && last[buf] > 0) {
-              const uint32_t p = last[buf] - 1;
-              got = mbar_wait_poll(&empty_bar[p % STAGES], (p / STAGES) & 1, lim, status, kWaitScales);
-            }
-            if (!got || *abort_flag) {
-              *abort_flag = 1;
-              ok = false;
-              break;
-            }
-          }
-          const uint32_t s = j % STAGES, ph = (j / STAGES) & 1;
-          if (!mbar_wait_poll(&full_bar[s], ph, lim, status, kWaitFull) || *abort_flag) {
-            *abort_flag = 1;
+        for (int kb = 0; kb < g.nkb && ok; it++) {   // an accumulator
+          if (!mbar_wait_poll(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) || *abort_flag) {
             ok = false;
             break;
           }
           tc_fence_after();
-          if ((kb & 3) == 0) {
-            const uint32_t ss = gr % SF_STAGES, buf = gr & 1, sa = smem_u32(sSF + ss * SF_BYTES);
-            sf = tmem + SF_COL + buf * SF_COLS;
-            copy_scales_pair(sf, smem_desc_scales(sa));
-            copy_scales_pair(sf + 4, smem_desc_scales(sa + ATOM));
-            copy_scales_pair(sf + 8, smem_desc_scales(sa + 2 * ATOM));
-            tc_commit_pair(&sf_empty[ss], 0x3);
-            gr++;
-          }
-          last[(gr - 1) & 1] = j + 1;
-          const uint32_t a_addr = smem_u32(sA + s * TILE_BYTES), b_addr = smem_u32(sB + s * TILE_BYTES);
-          const uint32_t id = g.idesc | idesc_scale_byte(kb & 3);
-          const bool first = kb % chunk == 0;
+          const uint32_t d_tmem = tmem + (it & 1) * ACC_COLS;
+          const int end = min(kb + chunk, g.nkb);
+          uint32_t accumulate = 0;
+          while (kb < end && ok) {   // a group of 4 blocks
+            // Its scales (group 0's came with the allocation's barrier).
+            if (gr > 0 && !mbar_wait_poll<true>(&sf_full[ss], sph ^ (ss == 0), lim, status, kWaitScales)) ok = false;
+            // Two buffers in TMEM: the MMAs of the group before the last have
+            // completed, by the ring (a stage is filled again only after
+            // them) or, after short groups, by their own commit.
+            if (ok && prev + STAGES > j + 1 && prev > 0) {
+              const uint32_t p = prev - 1;
+              ok = mbar_wait_poll(&empty_bar[p % STAGES], (p / STAGES) & 1, lim, status, kWaitScales);
+            }
+            prev = j;
+            const uint32_t sf = tmem + SF_COL + (gr & 1) * SF_COLS;
+            const int last = min(kb + 4, end);
+            for (uint32_t i = 0; kb < last && ok; kb++, i++, j++) {
+              if (!mbar_wait_poll(&full_bar[s], ph, lim, status, kWaitFull)) {
+                ok = false;
+                break;
+              }
+              if (issuer) {
+                if (i == 0) {
+                  const uint64_t d = desc_sf + ss * (SF_BYTES >> 4);
+                  tc_fence_after();
+                  copy_scales_pair(sf, d);
+                  copy_scales_pair(sf + 4, d + (ATOM >> 4));
+                  copy_scales_pair(sf + 8, d + (2 * ATOM >> 4));
+                  tc_commit_pair(&sf_empty[ss], 0x3);
+                }
+                const uint64_t da = desc_a + s * (TILE_BYTES >> 4), db = desc_b + s * (TILE_BYTES >> 4);
+                const uint32_t id = g.idesc | idesc_scale_byte(i);
+                mma_mx_pair(d_tmem, da, db, id, sf, sf + 4, accumulate);
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; kk++)
-            mma_mx_pair(d_tmem, smem_desc_sw128(a_addr + kk * a_step), smem_desc_sw128(b_addr + kk * b_step), id, sf,
-                        sf + 4, !first || kk != 0);
-          tc_commit_pair(&empty_bar[s], 0x3);
-          if (left == 1) tc_commit_pair(acc_full, 0x3);
+                for (int kk = 1; kk < BK / 32; kk++)
+                  mma_mx_pair(d_tmem, da + kk * a_step, db + kk * b_step, id, sf, sf + 4, 1);
+                tc_commit_pair(&empty_bar[s], 0x3);
+              }
+              __syncwarp();
+              accumulate = 1;
+              if (++s == STAGES) {
+                s = 0;
+                ph ^= 1;
+              }
+            }
+            gr++;
+            if (++ss == SF_STAGES) {
+              ss = 0;
+              sph ^= 1;
+            }
+          }
+          if (ok && issuer) tc_commit_pair(acc_full, 0x3);
         }
       }
+      if (!ok) *abort_flag = 1;
       // Every copy was waited for above and every MMA is waited for here: both
       // CTAs may then leave at the next barrier.
-      tc_commit_pair(drain_bar, 0x1);
-      if (mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain) && ok)
-        for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa_shared(smem_u32((const void*)all_done), r), 1);
+      if (issuer) {
+        tc_commit_pair(drain_bar, 0x1);
+        if (mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain) && ok)
+          for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa_shared(smem_u32((const void*)all_done), r), 1);
+      }
     }
   } else if (warp < 4) {
     // Scales: warp 2 gathers A's atom (this CTA's rows), warp 3 those of B.
