@@ -25,7 +25,8 @@ namespace f64e {
 // m * 2^p with m in [1, 1.75], one more above.  Subnormal magnitudes give
 // exponents below -127 whatever their leading bit, so the field serves as p.
 template <int CODE>
-__device__ __forceinline__ int scale_exponent(uint32_t amax_bits) {
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t amax_bits = __float_as_uint(amax);
   constexpr int emax = CODE == F64E_E4M3 ? 8 : 15;
   if (amax_bits == 0) return 0;
   const int p = (int)(amax_bits >> 23) - 127;
@@ -68,93 +69,146 @@ __device__ __forceinline__ float2 values2(uint32_t codes) {
 }
 
 // --------------------------------------------------------------- elements --
-// Eight neighbouring elements of a row as 32-bit words.
+// Sixteen elements of a thread as 32-bit words (two 16-bit elements a word),
+// their largest magnitude, and their values.  NaN never counts as a largest
+// magnitude; an infinity does, and is looked for by the callers.
 template <int T>
 struct Elem;
 template <>
 struct Elem<F64E_F32> {
   using type = float;
-  static constexpr int kWords = 8;
+  static constexpr int kWords = 16;
+  using mag = float;   // magnitudes of one word
+  __device__ static mag zero() { return 0.f; }
+  __device__ static mag max_mag(mag m, uint32_t w) { return fmaxf(m, fabsf(__uint_as_float(w))); }
+  __device__ static mag max_of(mag a, mag b) { return fmaxf(a, b); }
+  __device__ static mag shfl(mag a, int o) { return __shfl_xor_sync(0xFFFFFFFFu, a, o); }
   __device__ static float get(const uint32_t* w, int i) { return __uint_as_float(w[i]); }
   __device__ static uint32_t bits(float v) { return __float_as_uint(v); }
 };
+template <typename H2>
+struct Elem16 {
+  static constexpr int kWords = 8;
+  using mag = H2;
+  __device__ static mag max_mag(mag m, uint32_t w) {
+    w &= 0x7FFF7FFFu;
+    return __hmax2(m, *reinterpret_cast<const H2*>(&w));
+  }
+  __device__ static mag max_of(mag a, mag b) { return __hmax2(a, b); }
+  __device__ static mag shfl(mag a, int o) {
+    const uint32_t w = __shfl_xor_sync(0xFFFFFFFFu, *reinterpret_cast<const uint32_t*>(&a), o);
+    return *reinterpret_cast<const H2*>(&w);
+  }
+  __device__ static mag zero() {
+    const uint32_t w = 0;
+    return *reinterpret_cast<const H2*>(&w);
+  }
+};
 template <>
-struct Elem<F64E_F16> {
+struct Elem<F64E_F16> : Elem16<__half2> {
   using type = __half;
-  static constexpr int kWords = 4;
   __device__ static float get(const uint32_t* w, int i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i >> 1]));
     return (i & 1) ? f.y : f.x;
   }
+  __device__ static float lo(__half2 m) { return __low2float(m); }
+  __device__ static float hi(__half2 m) { return __high2float(m); }
   __device__ static uint32_t bits(float v) { return (uint32_t)__half_as_ushort(__float2half_rn(v)); }
 };
 template <>
-struct Elem<F64E_BF16> {
+struct Elem<F64E_BF16> : Elem16<__nv_bfloat162> {
   using type = __nv_bfloat16;
-  static constexpr int kWords = 4;
   __device__ static float get(const uint32_t* w, int i) {
     return __uint_as_float((i & 1) ? (w[i >> 1] & 0xFFFF0000u) : (w[i >> 1] << 16));
   }
+  __device__ static float lo(__nv_bfloat162 m) { return __low2float(m); }
+  __device__ static float hi(__nv_bfloat162 m) { return __high2float(m); }
   __device__ static uint32_t bits(float v) { return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 };
 
-// Loads eight elements at p, of which the first n exist (n <= 0: none); the
-// others read as zero.  vec: p is 16-byte aligned.
+// Sixteen contiguous elements at p, all there: 32-byte loads where `wide`
+// (p 32-byte aligned), else 16-byte loads.
 template <int T>
-__device__ __forceinline__ void load8(const typename Elem<T>::type* p, int64_t n, bool vec, uint32_t* w) {
-  if (vec && n >= 8) {
+__device__ __forceinline__ void load16(const typename Elem<T>::type* p, bool wide, uint32_t* w) {
+  if (wide) {
 #pragma unroll
-    for (int i = 0; i < Elem<T>::kWords / 4; i++) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      w[4 * i] = v.x;
-      w[4 * i + 1] = v.y;
-      w[4 * i + 2] = v.z;
-      w[4 * i + 3] = v.w;
+    for (int i = 0; i < Elem<T>::kWords; i += 8)
+      asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+          : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]),
+            "=r"(w[i + 7])
+          : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < Elem<T>::kWords; i += 4) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+      w[i] = v.x;
+      w[i + 1] = v.y;
+      w[i + 2] = v.z;
+      w[i + 3] = v.w;
     }
-    return;
   }
+}
+// Elements p[0], p[step], .. p[15 step], of which those with index below n
+// exist; the others read as zero.
+template <int T>
+__device__ __forceinline__ void load16_some(const typename Elem<T>::type* p, int step, int64_t n, uint32_t* w) {
+  if (Elem<T>::kWords == 16) {
 #pragma unroll
-  for (int i = 0; i < Elem<T>::kWords; i++) w[i] = 0;
-  if (Elem<T>::kWords == 8) {
-    const uint32_t* u = reinterpret_cast<const uint32_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < n) w[i] = __ldg(u + i);
+    for (int i = 0; i < 16; i++) w[i % Elem<T>::kWords] = i * step < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i * step) : 0;
   } else {
     const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      if (i < n) w[i >> 1] |= (uint32_t)__ldg(u + i) << (16 * (i & 1));
+    for (int i = 0; i < 16; i += 2) {
+      const uint32_t lo = i * step < n ? __ldg(u + i * step) : 0;
+      const uint32_t hi = (i + 1) * step < n ? __ldg(u + (i + 1) * step) : 0;
+      w[i / 2] = lo | (hi << 16);
+    }
   }
 }
 
-// ----------------------------------------------------------- magnitudes --
-// Largest magnitude as 32-bit float bits; infinity and NaN order above every
-// finite value, so "non-finite present" is amax >= kInfBits.
-constexpr uint32_t kInfBits = 0x7F800000u;
-
+// Largest magnitude of sixteen elements, as a float.
+__device__ __forceinline__ float fold(float m) { return m; }
+__device__ __forceinline__ float fold(__half2 m) { return fmaxf(__low2float(m), __high2float(m)); }
+__device__ __forceinline__ float fold(__nv_bfloat162 m) { return fmaxf(__low2float(m), __high2float(m)); }
 template <int T>
-__device__ __forceinline__ uint32_t mag(const uint32_t* w, int i) {
-  return __float_as_uint(Elem<T>::get(w, i)) & 0x7FFFFFFFu;
+__device__ __forceinline__ float max16(const uint32_t* w) {
+  typename Elem<T>::mag m = Elem<T>::zero();
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kWords; i++) m = Elem<T>::max_mag(m, w[i]);
+  return fold(m);
 }
+// The same over finite values only.
+template <int T>
+__device__ __forceinline__ float max16_finite(const uint32_t* w) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; i++) {
+    const float v = fabsf(Elem<T>::get(w, i));
+    if (v < __uint_as_float(0x7F800000u)) m = fmaxf(m, v);
+  }
+  return m;
+}
+__device__ __forceinline__ bool is_inf(float m) { return __float_as_uint(m) == 0x7F800000u; }
 
-// Eight codes of eight elements, all with the inverse scale r.  special: the
-// block holds an infinity or a NaN.
-template <int T, int CODE>
-__device__ __forceinline__ uint2 codes8(const uint32_t* w, float r, bool special) {
-  uint32_t c[4];
+// Codes of sixteen elements, two a word: element i scaled by r(i).  infs: some
+// block here holds an infinity, which the conversion would saturate.
+template <int T, int CODE, typename R>
+__device__ __forceinline__ void codes16(const uint32_t* w, R r, bool infs, uint32_t* c) {
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    c[i] = code2<CODE>(Elem<T>::get(w, 2 * i) * r, Elem<T>::get(w, 2 * i + 1) * r);
-  if (special) {
+  for (int i = 0; i < 8; i++)
+    c[i] = code2<CODE>(Elem<T>::get(w, 2 * i) * r(2 * i), Elem<T>::get(w, 2 * i + 1) * r(2 * i + 1));
+  if (infs) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < 16; i++) {
       const float v = Elem<T>::get(w, i);
-      if ((__float_as_uint(v) & 0x7FFFFFFFu) == kInfBits)
+      if (is_inf(fabsf(v)))
         c[i >> 1] = (c[i >> 1] & ~(0xFFu << (8 * (i & 1)))) | (code_of_inf<CODE>(v < 0.f) << (8 * (i & 1)));
     }
   }
-  return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+// The words of sixteen neighbouring codes.
+__device__ __forceinline__ uint4 row_of_codes(const uint32_t* c) {
+  return make_uint4(c[0] | (c[1] << 16), c[2] | (c[3] << 16), c[4] | (c[5] << 16), c[6] | (c[7] << 16));
 }
 
 // ------------------------------------------------ block-scaled tcgen05 --

@@ -21,11 +21,13 @@ struct Fp8QuantArgs {
   uint8_t* qc;          // codes [rows][ldq]: blocks along the column
   uint8_t* sc;          // scales [ceil(rows / 128)][cols]
   int64_t ldq;          // row pitch of q and qc: a multiple of 16, at least cols
+  int64_t ldt;          // not 0: qc holds the column codes transposed, [cols][ldt]
 };
 // x_type F64E_F32 / F16 / BF16, code F64E_E4M3 / E5M2.
 cudaError_t launch_fp8_quant_rows(const Fp8QuantArgs& a, int x_type, int code, cudaStream_t s);
 // 128 x 128 squares held in registers: tile != 0 writes q / s with one scale
-// per square; otherwise qc / sc, and q / s too when q is not null.
+// per square; otherwise qc / sc, and q / s too when q is not null (only then
+// may qc be transposed).
 cudaError_t launch_fp8_quant_squares(const Fp8QuantArgs& a, int x_type, int code, int tile, cudaStream_t s);
 
 struct Fp8DequantArgs {

@@ -30,9 +30,8 @@ const char* check_types(int x_type, int code) {
 const char* check_matrix(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 0) return "fp8: negative dimension";
   if (rows > kMaxDim || cols > kMaxDim) return "fp8: dimension too large";
-  // every launch covers the matrix with at most one CTA for 16 x 512, 128 x 128 or 4096 values
-  if (blocks_of(rows) * blocks_of(cols) > 0x7FFFFFFF || (rows + 15) / 16 * ((cols + 511) / 512) > 0x7FFFFFFF ||
-      rows * ((cols + 15) / 16) / 256 >= 0x7FFFFFFF)
+  // a CTA for 32 x 512 or 128 x 128 values
+  if (blocks_of(rows) * blocks_of(cols) > 0x7FFFFFFF || (rows + 31) / 32 * ((cols + 511) / 512) > 0x7FFFFFFF)
     return "fp8: matrix too large";
   return nullptr;
 }
@@ -114,7 +113,8 @@ int f64e_fp8_quantize(const void* x, int32_t x_type, int64_t rows, int64_t cols,
 }
 
 int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx, int32_t code,
-                           void* q_row, void* scale_row, void* q_col, void* scale_col, int64_t ldq, void* stream) {
+                           void* q_row, void* scale_row, int64_t ldq, void* q_col, void* scale_col, int32_t transposed,
+                           int64_t ld_col, void* stream) {
   begin_call();
   if (const char* m = check_types(x_type, code)) return bad(m);
   if (const char* m = check_matrix(rows, cols)) return bad(m);
@@ -122,7 +122,9 @@ int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t 
   if (!x || !q_row || !scale_row || !q_col || !scale_col) return bad("fp8: null pointer");
   if (ldx < cols) return bad("fp8: row pitch of x is below its columns");
   if (const char* m = check_codes(q_row, ldq, cols)) return bad(m);
-  if (const char* m = check_codes(q_col, ldq, cols)) return bad(m);
+  if (transposed != 0 && transposed != 1) return bad("fp8: transposed must be 0 or 1");
+  if (const char* m = check_codes(q_col, ld_col, transposed ? rows : cols)) return bad(m);
+  if (!transposed && ld_col != ldq) return bad("fp8: row and column codes need the same pitch");
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
   Fp8QuantArgs a{};
@@ -131,6 +133,7 @@ int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t 
   a.cols = cols;
   a.ldx = ldx;
   a.ldq = ldq;
+  a.ldt = transposed ? ld_col : 0;
   a.q = static_cast<uint8_t*>(q_row);
   a.s = static_cast<uint8_t*>(scale_row);
   a.qc = static_cast<uint8_t*>(q_col);

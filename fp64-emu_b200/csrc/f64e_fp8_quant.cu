@@ -1,8 +1,14 @@
 // Block quantisation to 8-bit floating point and back.
 //
-// Both kernels are bound by memory: rows reads e bytes a value (e = 2 or 4)
-// and writes 1 + 1/128; the squares kernel does the same and, asked for row
-// and column blocks at once, writes 2 (1 + 1/128) for one read.
+// All three kernels are bound by memory: quantising reads e bytes a value (e =
+// 2 or 4) and writes 1 + 1/128, or twice that for row and column blocks from
+// one read; restoring is the reverse.  An SM must then handle about 6 values a
+// cycle, some 16 instructions a value at most, so a thread works on sixteen
+// neighbouring values at a time: one or two loads, packed magnitudes, and the
+// scale's arithmetic shared by all of them.
+// Where rows do not start on 16-byte boundaries (VEC = false) the same thread
+// takes every eighth value instead, so that neighbouring lanes still touch
+// neighbouring elements, and codes are put in order in shared memory.
 #include "f64e_fp8.cuh"
 #include "f64e_fp8.h"
 
@@ -12,295 +18,415 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Largest finite magnitude of a block is wanted; the first pass takes the
-// largest of all, and only a block that holds a non-finite value pays for a
-// second look.
-template <int T>
-__device__ __forceinline__ uint32_t max8(const uint32_t* w) {
-  uint32_t m = 0;
+// Lanes l = 0..7 hold one 128-value row block: the maximum over them.
+__device__ __forceinline__ float max_over_block(float m) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) m = max(m, mag<T>(w, i));
+  for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   return m;
 }
-template <int T>
-__device__ __forceinline__ uint32_t max8_finite(const uint32_t* w) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const uint32_t v = mag<T>(w, i);
-    if (v < kInfBits) m = max(m, v);
+// Exponent of the row block these lanes hold.
+template <int T, int CODE>
+__device__ __forceinline__ int row_exponent(const uint32_t* w, bool* infs) {
+  float m = max_over_block(max16<T>(w));
+  *infs = is_inf(m);
+  if (__any_sync(0xFFFFFFFFu, *infs)) {
+    const float f = max_over_block(max16_finite<T>(w));
+    if (*infs) m = f;
   }
-  return m;
+  return scale_exponent<CODE>(m);
 }
 
-// Maximum over the 16 lanes that hold one 128-value row block.
-__device__ __forceinline__ uint32_t max_half_warp(uint32_t m) {
-#pragma unroll
-  for (int o = 8; o; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  return m;
+// Column of a thread's i-th value within its 128, from lane l of eight.
+template <bool VEC>
+__device__ __forceinline__ int col_of(int l, int i) {
+  return VEC ? l * 16 + i : i * 8 + l;
+}
+template <int T, bool VEC>
+__device__ __forceinline__ void load_row(const typename Elem<T>::type* row, int l, int64_t n, bool wide, uint32_t* w) {
+  if (VEC && n >= (l + 1) * 16)
+    load16<T>(row + l * 16, wide, w);
+  else
+    load16_some<T>(row + (VEC ? l * 16 : l), VEC ? 1 : 8, n - (VEC ? l * 16 : l), w);
 }
 
 // --------------------------------------------------------------- rows ----
-// Half a warp holds a block: eight values a lane, one 16-byte load each (two
-// in 32 bits).  A CTA covers 16 rows by four blocks, all its loads in flight
-// before the first reduction.
-constexpr int kRowBlocks = 4, kRowPasses = 4, kRowsPerPass = kThreads / (16 * kRowBlocks);
+// A warp covers four neighbouring blocks (512 columns) of four rows.
+constexpr int kRowPasses = 4;
 
-template <int T, int CODE>
-__global__ void __launch_bounds__(kThreads) fp8_quant_rows_kernel(const Fp8QuantArgs a, int64_t nkb, int64_t ngroups,
-                                                                  bool vec) {
-  const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t kb = (blockIdx.x % ngroups) * kRowBlocks + (half & (kRowBlocks - 1));
-  const int64_t row0 = (blockIdx.x / ngroups) * (kRowsPerPass * kRowPasses) + half / kRowBlocks;
-  const int64_t col = kb * kFp8Block + l * 8;
-  const int64_t padded = (a.cols + 15) & ~(int64_t)15;
-  const typename Elem<T>::type* x = static_cast<const typename Elem<T>::type*>(a.x);
+template <int T, int CODE, bool VEC>
+__global__ void __launch_bounds__(kThreads) fp8_quant_rows_kernel(const Fp8QuantArgs a, int nkb, int ngroups,
+                                                                  bool wide) {
+  __shared__ __align__(16) uint8_t s_codes[VEC ? 1 : kThreads / 32][VEC ? 16 : 512];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7;
+  const int kb = (int)(blockIdx.x % ngroups) * 4 + (lane >> 3);
+  const int64_t row0 = ((int64_t)(blockIdx.x / ngroups) * (kThreads / 32) + warp) * kRowPasses;
+  const int64_t col = (int64_t)kb * kFp8Block, padded = (a.cols + 15) & ~(int64_t)15;
+  const typename Elem<T>::type* x = static_cast<const typename Elem<T>::type*>(a.x) + row0 * a.ldx + col;
+  uint8_t* q = a.q + row0 * a.ldq + col + l * 16;
+  uint8_t* s = a.s + row0 * nkb + kb;
   uint32_t w[kRowPasses][Elem<T>::kWords];
 #pragma unroll
-  for (int u = 0; u < kRowPasses; u++) {
-    const int64_t r = row0 + u * kRowsPerPass;
-    load8<T>(x + r * a.ldx + col, r < a.rows ? a.cols - col : 0, vec, w[u]);
-  }
+  for (int u = 0; u < kRowPasses; u++)
+    load_row<T, VEC>(x + u * a.ldx, l, row0 + u < a.rows ? a.cols - col : 0, wide, w[u]);
 #pragma unroll
   for (int u = 0; u < kRowPasses; u++) {
-    const int64_t r = row0 + u * kRowsPerPass;
-    uint32_t m = max_half_warp(max8<T>(w[u]));
-    const bool special = m >= kInfBits;
-    if (__any_sync(0xFFFFFFFFu, special)) {
-      const uint32_t f = max_half_warp(max8_finite<T>(w[u]));
-      if (special) m = f;
+    bool infs;
+    const int e = row_exponent<T, CODE>(w[u], &infs);
+    const float r = inverse_scale(e);
+    uint32_t c[8];
+    codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c);
+    uint4 v;
+    if (VEC) {
+      v = row_of_codes(c);
+    } else {
+      uint8_t* st = s_codes[warp % (VEC ? 1 : kThreads / 32)] + (lane >> 3) * (VEC ? 0 : 128);
+#pragma unroll
+      for (int i = 0; i < 16; i++) st[(VEC ? 0 : i * 8) + l] = (uint8_t)(c[i >> 1] >> (8 * (i & 1)));
+      __syncwarp();
+      v = *reinterpret_cast<const uint4*>(st + l * (VEC ? 0 : 16));
+      __syncwarp();
     }
-    const int e = scale_exponent<CODE>(m);
-    const uint2 c = codes8<T, CODE>(w[u], inverse_scale(e), special);
-    if (r < a.rows) {
-      if (col < padded) *reinterpret_cast<uint2*>(a.q + r * a.ldq + col) = c;
-      if (l == 0 && kb < nkb) a.s[r * nkb + kb] = (uint8_t)(e + 127);
+    if (row0 + u < a.rows && kb < nkb) {
+      if (col + l * 16 < padded) *reinterpret_cast<uint4*>(q + u * a.ldq) = v;
+      if (l == 0) s[(int64_t)u * nkb] = (uint8_t)(e + 127);
     }
   }
 }
 
 // ------------------------------------------------------------ squares ----
-// A CTA keeps a 128 x 128 square in registers: thread (g, l), g = half-warp,
-// holds eight columns 8 l.. of the rows g, g + 16, ..; the value is read once
-// for both block directions.  Column maxima: over the thread's rows, the two
-// half-warps of a warp, then the eight warps through shared memory.
-constexpr int kSqRows = kFp8Block / (kThreads / 16);
+// A CTA keeps a 128 x 128 square in registers, a thread sixteen columns of the
+// four rows 4 g .. 4 g + 3, so one read serves both block directions.  Column
+// maxima: packed over the thread's rows and the four threads of a warp that
+// share its columns, then over the eight warps in shared memory, where one
+// thread a column turns them into the scale.
+// Transposed codes leave through shared memory: a thread's four rows of a
+// column are one 32-bit word there.
+enum { kCols = 0, kRowsCols = 1, kTile = 2, kRowsColsT = 3 };
 
-template <int T, int CODE, int MODE>  // MODE 0: column blocks, 1: column and row blocks, 2: square blocks
-__global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8QuantArgs a, int64_t nkb, bool vec) {
-  __shared__ uint32_t s_max[kThreads / 32][kFp8Block];
-  const int g = threadIdx.x >> 4, l = threadIdx.x & 15, warp = threadIdx.x >> 5;
-  const int64_t kb = blockIdx.x % nkb, rb = blockIdx.x / nkb;
-  const int64_t col = kb * kFp8Block + l * 8;
-  const int64_t padded = (a.cols + 15) & ~(int64_t)15;
-  const typename Elem<T>::type* x = static_cast<const typename Elem<T>::type*>(a.x);
-  uint32_t w[kSqRows][Elem<T>::kWords];
+struct SquareSmem {
+  float max[kThreads / 32][kFp8Block];
+  float inv[kFp8Block];
+  int infs;
+};
+
+// Row-major codes of the thread's four rows; VEC = false puts them in order in
+// `tile` (the whole CTA calls it).
+template <bool VEC>
+__device__ __forceinline__ void store_rows(uint8_t* q, int64_t ldq, int64_t rows, int64_t row0, int64_t col,
+                                           int64_t padded, int g, int l, uint8_t* tile, const uint32_t (&c)[4][8]) {
+  if (VEC) {
 #pragma unroll
-  for (int u = 0; u < kSqRows; u++) {
-    const int64_t r = rb * kFp8Block + u * (kThreads / 16) + g;
-    load8<T>(x + r * a.ldx + col, r < a.rows ? a.cols - col : 0, vec, w[u]);
+    for (int u = 0; u < 4; u++)
+      if (row0 + 4 * g + u < rows && col + l * 16 < padded)
+        *reinterpret_cast<uint4*>(q + (row0 + 4 * g + u) * ldq + col + l * 16) = row_of_codes(c[u]);
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) tile[(4 * g + u) * 128 + i * 8 + l] = (uint8_t)(c[u][i >> 1] >> (8 * (i & 1)));
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int r = u * 32 + (threadIdx.x >> 3);
+      if (row0 + r < rows && col + l * 16 < padded)
+        *reinterpret_cast<uint4*>(q + (row0 + r) * ldq + col + l * 16) =
+            *reinterpret_cast<const uint4*>(tile + r * 128 + l * 16);
+    }
   }
+}
+// The same codes with rows contiguous: qt[col][row], pitch ldt.
+template <bool VEC>
+__device__ __forceinline__ void store_columns(uint8_t* qt, int64_t ldt, int64_t cols, int64_t padded_rows, int64_t row0,
+                                              int64_t col, int g, int l, uint8_t* tile, const uint32_t (&c)[4][8]) {
+  uint32_t* words = reinterpret_cast<uint32_t*>(tile);   // [128 columns][32 words], words XORed by 4 x (column / 16)
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; k++) {
+    const uint32_t x = __byte_perm(c[0][k], c[1][k], 0x5140), y = __byte_perm(c[2][k], c[3][k], 0x5140);
+    const int c0 = col_of<VEC>(l, 2 * k), c1 = col_of<VEC>(l, 2 * k + 1);
+    words[c0 * 32 + (g ^ ((c0 >> 4) << 2))] = __byte_perm(x, y, 0x5410);
+    words[c1 * 32 + (g ^ ((c1 >> 4) << 2))] = __byte_perm(x, y, 0x7632);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int cc = u * 32 + (threadIdx.x >> 3), ch = threadIdx.x & 7;
+    if (col + cc < cols && row0 + ch * 16 < padded_rows)
+      *reinterpret_cast<uint4*>(qt + (col + cc) * ldt + row0 + ch * 16) =
+          *reinterpret_cast<const uint4*>(tile + cc * 128 + ((ch ^ (cc >> 4)) << 4));
+  }
+}
 
-  // Maxima of the eight columns over the square, every thread's copy.
-  auto column_maxima = [&](bool finite_only, uint32_t* cm) {
+template <int T, int CODE, int MODE, bool VEC>
+__global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8QuantArgs a, int nkb, bool wide) {
+  using E = Elem<T>;
+  __shared__ SquareSmem sm;
+  __shared__ __align__(16) uint8_t tile[!VEC || MODE == kRowsColsT ? 128 * 128 : 16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 7, g = threadIdx.x >> 3;
+  const int kb = (int)(blockIdx.x % nkb);
+  const int64_t rb = blockIdx.x / nkb, row0 = rb * kFp8Block, col = (int64_t)kb * kFp8Block;
+  const int64_t padded = (a.cols + 15) & ~(int64_t)15;
+  const typename E::type* x = static_cast<const typename E::type*>(a.x) + (row0 + 4 * g) * a.ldx + col;
+  uint32_t w[4][E::kWords], c[4][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) cm[i] = 0;
+  for (int u = 0; u < 4; u++)
+    load_row<T, VEC>(x + u * a.ldx, l, row0 + 4 * g + u < a.rows ? a.cols - col : 0, wide, w[u]);
+  if (threadIdx.x == 0) sm.infs = 0;
+
+  if (MODE == kTile) {
+    float m = 0.f;
 #pragma unroll
-    for (int u = 0; u < kSqRows; u++)
+    for (int u = 0; u < 4; u++) m = fmaxf(m, max16<T>(w[u]));
+    auto over_square = [&](float v) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const uint32_t v = mag<T>(w[u], i);
-        if (!finite_only || v < kInfBits) cm[i] = max(cm[i], v);
-      }
+      for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+      if (lane == 0) sm.inv[warp] = v;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; i++) cm[i] = max(cm[i], __shfl_xor_sync(0xFFFFFFFFu, cm[i], 16));
-    if ((threadIdx.x & 31) < 16) {
-      *reinterpret_cast<uint4*>(&s_max[warp][l * 8]) = make_uint4(cm[0], cm[1], cm[2], cm[3]);
-      *reinterpret_cast<uint4*>(&s_max[warp][l * 8 + 4]) = make_uint4(cm[4], cm[5], cm[6], cm[7]);
+      for (int i = 0; i < kThreads / 32; i++) v = fmaxf(v, sm.inv[i]);
+      __syncthreads();
+      return v;
+    };
+    m = over_square(m);
+    const bool infs = is_inf(m);
+    if (infs) {
+      m = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; u++) m = fmaxf(m, max16_finite<T>(w[u]));
+      m = over_square(m);
     }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < kThreads / 32; v++) {
-      const uint4 p = *reinterpret_cast<const uint4*>(&s_max[v][l * 8]);
-      const uint4 q = *reinterpret_cast<const uint4*>(&s_max[v][l * 8 + 4]);
-      cm[0] = max(cm[0], p.x);
-      cm[1] = max(cm[1], p.y);
-      cm[2] = max(cm[2], p.z);
-      cm[3] = max(cm[3], p.w);
-      cm[4] = max(cm[4], q.x);
-      cm[5] = max(cm[5], q.y);
-      cm[6] = max(cm[6], q.z);
-      cm[7] = max(cm[7], q.w);
-    }
-    __syncthreads();
-  };
-  auto all_of = [&](const uint32_t* cm) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) m = max(m, cm[i]);
-    return max_half_warp(m);
-  };
-
-  uint32_t cm[8];
-  column_maxima(false, cm);
-  const bool special = all_of(cm) >= kInfBits;   // the same in every thread
-  uint32_t fin[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) fin[i] = cm[i];
-  if (special) column_maxima(true, fin);
-
-  if (MODE == 2) {
-    const int e = scale_exponent<CODE>(all_of(fin));
+    const int e = scale_exponent<CODE>(m);
     const float r = inverse_scale(e);
 #pragma unroll
-    for (int u = 0; u < kSqRows; u++) {
-      const int64_t row = rb * kFp8Block + u * (kThreads / 16) + g;
-      const uint2 c = codes8<T, CODE>(w[u], r, special);
-      if (row < a.rows && col < padded) *reinterpret_cast<uint2*>(a.q + row * a.ldq + col) = c;
-    }
+    for (int u = 0; u < 4; u++) codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c[u]);
+    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
     if (threadIdx.x == 0) a.s[rb * nkb + kb] = (uint8_t)(e + 127);
     return;
   }
 
-  float r[8];
+  // Row blocks first: their registers are free again before the columns'.
+  if (MODE == kRowsCols || MODE == kRowsColsT) {
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int e = scale_exponent<CODE>(fin[i]);
-    r[i] = inverse_scale(e);
-    if (g == 0 && col + i < a.cols) a.sc[rb * a.cols + col + i] = (uint8_t)(e + 127);
-  }
-#pragma unroll
-  for (int u = 0; u < kSqRows; u++) {
-    const int64_t row = rb * kFp8Block + u * (kThreads / 16) + g;
-    uint32_t c[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      c[i] = code2<CODE>(Elem<T>::get(w[u], 2 * i) * r[2 * i], Elem<T>::get(w[u], 2 * i + 1) * r[2 * i + 1]);
-    if (special) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float v = Elem<T>::get(w[u], i);
-        if ((__float_as_uint(v) & 0x7FFFFFFFu) == kInfBits)
-          c[i >> 1] = (c[i >> 1] & ~(0xFFu << (8 * (i & 1)))) | (code_of_inf<CODE>(v < 0.f) << (8 * (i & 1)));
-      }
+    for (int u = 0; u < 4; u++) {
+      bool infs;
+      const int e = row_exponent<T, CODE>(w[u], &infs);
+      const float r = inverse_scale(e);
+      codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c[u]);
+      const int64_t row = row0 + 4 * g + u;
+      if (l == 0 && row < a.rows) a.s[row * nkb + kb] = (uint8_t)(e + 127);
     }
-    if (row < a.rows && col < padded)
-      *reinterpret_cast<uint2*>(a.qc + row * a.ldq + col) = make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
   }
-  if (MODE == 1) {
+
+  auto publish = [&](int i, float m) { sm.max[warp][col_of<VEC>(l, i)] = m; };
+  {
+    typename E::mag m[E::kWords];
 #pragma unroll
-    for (int u = 0; u < kSqRows; u++) {
-      const int64_t row = rb * kFp8Block + u * (kThreads / 16) + g;
-      uint32_t m = max_half_warp(max8<T>(w[u]));
-      const bool sp = m >= kInfBits;
-      if (__any_sync(0xFFFFFFFFu, sp)) {
-        const uint32_t f = max_half_warp(max8_finite<T>(w[u]));
-        if (sp) m = f;
-      }
-      const int e = scale_exponent<CODE>(m);
-      const uint2 c = codes8<T, CODE>(w[u], inverse_scale(e), sp);
-      if (row < a.rows) {
-        if (col < padded) *reinterpret_cast<uint2*>(a.q + row * a.ldq + col) = c;
-        if (l == 0) a.s[row * nkb + kb] = (uint8_t)(e + 127);
-      }
+    for (int k = 0; k < E::kWords; k++) {
+      m[k] = E::zero();
+#pragma unroll
+      for (int u = 0; u < 4; u++) m[k] = E::max_mag(m[k], w[u][k]);
+      m[k] = E::max_of(m[k], E::shfl(m[k], 8));
+      m[k] = E::max_of(m[k], E::shfl(m[k], 16));
     }
+#pragma unroll
+    for (int k = 0; k < E::kWords; k++)
+      if ((lane >> 3) == k * 4 / E::kWords) {   // each of the four writes a quarter
+        if constexpr (T == F64E_F32) {
+          publish(k, m[k]);
+        } else {
+          publish(2 * k, E::lo(m[k]));
+          publish(2 * k + 1, E::hi(m[k]));
+        }
+      }
   }
+  auto finish = [&]() {
+    __syncthreads();
+    if (threadIdx.x < kFp8Block) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; i++) m = fmaxf(m, sm.max[i][threadIdx.x]);
+      if (is_inf(m)) {
+        sm.infs = 1;
+      }
+      const int e = is_inf(m) ? 0 : scale_exponent<CODE>(m);
+      sm.inv[threadIdx.x] = inverse_scale(e);
+      if (col + threadIdx.x < a.cols) a.sc[rb * a.cols + col + threadIdx.x] = (uint8_t)(e + 127);
+    }
+    __syncthreads();
+  };
+  finish();
+  const bool infs = sm.infs != 0;
+  if (infs) {   // the columns once more, over finite values
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      float m = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const float v = fabsf(E::get(w[u], i));
+        if (v < __uint_as_float(0x7F800000u)) m = fmaxf(m, v);
+      }
+      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+      if (lane < 8) publish(i, m);
+    }
+    finish();
+  }
+  float r[16];
+  if (VEC) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float4 v = *reinterpret_cast<const float4*>(&sm.inv[l * 16 + 4 * i]);
+      r[4 * i] = v.x;
+      r[4 * i + 1] = v.y;
+      r[4 * i + 2] = v.z;
+      r[4 * i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i++) r[i] = sm.inv[i * 8 + l];
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) codes16<T, CODE>(w[u], [&](int i) { return r[i]; }, infs, c[u]);
+  if (MODE == kRowsColsT)
+    store_columns<VEC>(a.qc, a.ldt, a.cols, (a.rows + 15) & ~(int64_t)15, row0, col, g, l, tile, c);
+  else
+    store_rows<VEC>(a.qc, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
 }
 
 // --------------------------------------------------------- dequantise ----
-// Sixteen codes a thread; a row block or square gives them one scale.
-template <int CODE, int T>
-__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantArgs a, int64_t nvec, bool vec_in,
-                                                               bool vec_out) {
-  const int64_t id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t r = id / nvec, c = (id - r * nvec) * 16;
-  if (r >= a.rows) return;
-  const int64_t n = a.cols - c;
-  const uint8_t* q = a.q + r * a.ldq + c;
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (vec_in && n >= 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(q));
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-  } else {
+// Sixteen columns of up to four rows of one row block a thread (rows g, g +
+// 32, .. of the 128), so column scales are read once for the four.
+template <int CODE, int T, bool VEC>
+__global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantArgs a, int ncb, bool wide) {
+  const int l = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int64_t rb = blockIdx.x / ncb, col = (int64_t)(blockIdx.x % ncb) * kFp8Block;
+  const int64_t n = a.cols - col;
+  const uint8_t* q = a.q + (rb * kFp8Block + g) * a.ldq + col;
+  uint32_t w[4][4];
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (i < n) w[i >> 2] |= (uint32_t)__ldg(q + i) << (8 * (i & 3));
-  }
-  const uint8_t* s = a.s + (a.blocks == F64E_BLOCKS_ROW ? r : r / kFp8Block) * a.s_row;
-  const bool per_col = a.blocks == F64E_BLOCKS_COL;
-  const float one = per_col ? 1.0f : scale_of_byte(__ldg(s + c / kFp8Block * a.s_col));
-  float f[16];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float2 v = values2<CODE>((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
-#pragma unroll
-  for (int i = 0; i < 16; i++) f[i] *= per_col ? (i < n ? scale_of_byte(__ldg(s + (c + i) * a.s_col)) : 0.0f) : one;
-  typename Elem<T>::type* o = static_cast<typename Elem<T>::type*>(a.out) + r * a.cols + c;
-  if (vec_out && n >= 16) {
-    if (T == F64E_F32) {
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        reinterpret_cast<float4*>(o)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  for (int u = 0; u < 4; u++) {
+    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
+    if (rb * kFp8Block + g + 32 * u >= a.rows) continue;
+    const uint8_t* p = q + (int64_t)(32 * u) * a.ldq;
+    if (VEC && n >= (l + 1) * 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + l * 16));
+      w[u][0] = v.x;
+      w[u][1] = v.y;
+      w[u][2] = v.z;
+      w[u][3] = v.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        uint32_t p[4];
+      for (int i = 0; i < 16; i++)
+        if (col_of<VEC>(l, i) < n) w[u][i >> 2] |= (uint32_t)__ldg(p + col_of<VEC>(l, i)) << (8 * (i & 3));
+    }
+  }
+  const bool per_col = a.blocks == F64E_BLOCKS_COL;
+  const int64_t cb = blockIdx.x % ncb;
+  float sc[16];
+  if (per_col) {
+    const uint8_t* s = a.s + rb * a.s_row + col * a.s_col;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          p[j] = Elem<T>::bits(f[8 * i + 2 * j]) | (Elem<T>::bits(f[8 * i + 2 * j + 1]) << 16);
-        reinterpret_cast<uint4*>(o)[i] = make_uint4(p[0], p[1], p[2], p[3]);
+    for (int i = 0; i < 16; i++) {
+      const int c = col_of<VEC>(l, i);
+      sc[i] = c < n ? scale_of_byte(__ldg(s + c * a.s_col)) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    const int64_t row = rb * kFp8Block + g + 32 * u;
+    if (row >= a.rows) break;
+    if (!per_col) {
+      const float one = scale_of_byte(__ldg(a.s + (a.blocks == F64E_BLOCKS_ROW ? row : rb) * a.s_row + cb * a.s_col));
+#pragma unroll
+      for (int i = 0; i < 16; i++) sc[i] = one;
+    }
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float2 v = values2<CODE>((w[u][i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+      f[2 * i] = v.x * sc[2 * i];
+      f[2 * i + 1] = v.y * sc[2 * i + 1];
+    }
+    typename Elem<T>::type* o = static_cast<typename Elem<T>::type*>(a.out) + row * a.cols + col;
+    if (VEC && n >= (l + 1) * 16) {
+      uint32_t b[Elem<T>::kWords];
+#pragma unroll
+      for (int i = 0; i < Elem<T>::kWords; i++)
+        b[i] = T == F64E_F32 ? Elem<T>::bits(f[i]) : Elem<T>::bits(f[(2 * i) & 15]) | (Elem<T>::bits(f[(2 * i + 1) & 15]) << 16);
+      uint32_t* ow = reinterpret_cast<uint32_t*>(o + l * 16);
+      if (wide) {
+#pragma unroll
+        for (int i = 0; i < Elem<T>::kWords; i += 8)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(ow + i), "r"(b[i]), "r"(b[i + 1]),
+                       "r"(b[i + 2]), "r"(b[i + 3]), "r"(b[i + 4]), "r"(b[i + 5]), "r"(b[i + 6]), "r"(b[i + 7])
+                       : "memory");
+      } else {
+#pragma unroll
+        for (int i = 0; i < Elem<T>::kWords; i += 4)
+          *reinterpret_cast<uint4*>(ow + i) = make_uint4(b[i], b[i + 1], b[i + 2], b[i + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int c = col_of<VEC>(l, i);
+        if (c < n) {
+          if (T == F64E_F32)
+            reinterpret_cast<uint32_t*>(o)[c] = Elem<T>::bits(f[i]);
+          else
+            reinterpret_cast<uint16_t*>(o)[c] = (uint16_t)Elem<T>::bits(f[i]);
+        }
       }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (i < n) {
-        if (T == F64E_F32)
-          reinterpret_cast<uint32_t*>(o)[i] = Elem<T>::bits(f[i]);
-        else
-          reinterpret_cast<uint16_t*>(o)[i] = (uint16_t)Elem<T>::bits(f[i]);
-      }
   }
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-bool aligned16(const void* p, int64_t pitch_bytes) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && pitch_bytes % 16 == 0;
+bool aligned(const void* p, int64_t pitch_bytes, int64_t to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && pitch_bytes % to == 0;
 }
 
 template <int T, int CODE>
 cudaError_t rows_of(const Fp8QuantArgs& a, cudaStream_t s) {
-  const int64_t nkb = ceil_div(a.cols, kFp8Block), ng = ceil_div(nkb, kRowBlocks);
-  const int64_t grid = ng * ceil_div(a.rows, kRowsPerPass * kRowPasses);
-  const bool vec = aligned16(a.x, a.ldx * (int64_t)sizeof(typename Elem<T>::type));
-  fp8_quant_rows_kernel<T, CODE><<<(unsigned)grid, kThreads, 0, s>>>(a, nkb, ng, vec);
+  const int nkb = (int)ceil_div(a.cols, kFp8Block), ng = (nkb + 3) / 4;
+  const unsigned grid = (unsigned)(ng * ceil_div(a.rows, kThreads / 32 * kRowPasses));
+  const int64_t pitch = a.ldx * (int64_t)sizeof(typename Elem<T>::type);
+  const bool wide = aligned(a.x, pitch, 32);
+  if (aligned(a.x, pitch, 16))
+    fp8_quant_rows_kernel<T, CODE, true><<<grid, kThreads, 0, s>>>(a, nkb, ng, wide);
+  else
+    fp8_quant_rows_kernel<T, CODE, false><<<grid, kThreads, 0, s>>>(a, nkb, ng, wide);
+  return cudaGetLastError();
+}
+template <int T, int CODE, int MODE>
+cudaError_t squares_mode(const Fp8QuantArgs& a, cudaStream_t s) {
+  const int nkb = (int)ceil_div(a.cols, kFp8Block);
+  const unsigned grid = (unsigned)(nkb * ceil_div(a.rows, kFp8Block));
+  const int64_t pitch = a.ldx * (int64_t)sizeof(typename Elem<T>::type);
+  const bool wide = aligned(a.x, pitch, 32);
+  if (aligned(a.x, pitch, 16))
+    fp8_quant_squares_kernel<T, CODE, MODE, true><<<grid, kThreads, 0, s>>>(a, nkb, wide);
+  else
+    fp8_quant_squares_kernel<T, CODE, MODE, false><<<grid, kThreads, 0, s>>>(a, nkb, wide);
   return cudaGetLastError();
 }
 template <int T, int CODE>
 cudaError_t squares_of(const Fp8QuantArgs& a, int tile, cudaStream_t s) {
-  const int64_t nkb = ceil_div(a.cols, kFp8Block);
-  const unsigned grid = (unsigned)(nkb * ceil_div(a.rows, kFp8Block));
-  const bool vec = aligned16(a.x, a.ldx * (int64_t)sizeof(typename Elem<T>::type));
-  if (tile)
-    fp8_quant_squares_kernel<T, CODE, 2><<<grid, kThreads, 0, s>>>(a, nkb, vec);
-  else if (a.q)
-    fp8_quant_squares_kernel<T, CODE, 1><<<grid, kThreads, 0, s>>>(a, nkb, vec);
-  else
-    fp8_quant_squares_kernel<T, CODE, 0><<<grid, kThreads, 0, s>>>(a, nkb, vec);
-  return cudaGetLastError();
+  if (tile) return squares_mode<T, CODE, kTile>(a, s);
+  if (!a.q) return squares_mode<T, CODE, kCols>(a, s);
+  return a.ldt ? squares_mode<T, CODE, kRowsColsT>(a, s) : squares_mode<T, CODE, kRowsCols>(a, s);
 }
 template <int CODE, int T>
 cudaError_t dequant_of(const Fp8DequantArgs& a, cudaStream_t s) {
-  const int64_t nvec = ceil_div(a.cols, 16);
-  const unsigned grid = (unsigned)ceil_div(nvec * a.rows, kThreads);
-  const bool vin = aligned16(a.q, a.ldq), vout = aligned16(a.out, a.cols * (int64_t)sizeof(typename Elem<T>::type));
-  fp8_dequant_kernel<CODE, T><<<grid, kThreads, 0, s>>>(a, nvec, vin, vout);
+  const int ncb = (int)ceil_div(a.cols, kFp8Block);
+  const unsigned grid = (unsigned)(ncb * ceil_div(a.rows, kFp8Block));
+  const int64_t pitch = a.cols * (int64_t)sizeof(typename Elem<T>::type);
+  const bool wide = aligned(a.out, pitch, 32);
+  if (aligned(a.q, a.ldq, 16) && aligned(a.out, pitch, 16))
+    fp8_dequant_kernel<CODE, T, true><<<grid, kThreads, 0, s>>>(a, ncb, wide);
+  else
+    fp8_dequant_kernel<CODE, T, false><<<grid, kThreads, 0, s>>>(a, ncb, wide);
   return cudaGetLastError();
 }
 

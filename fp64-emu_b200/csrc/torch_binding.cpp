@@ -414,7 +414,8 @@ std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, int64_t blo
   return {q, s};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> fp8_quantize_both(const at::Tensor& x, at::ScalarType code) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> fp8_quantize_both(const at::Tensor& x, at::ScalarType code,
+                                                                             bool transposed) {
   TORCH_CHECK(x.dim() == 2, "x must be a matrix");
   fp8_check_float(x, "x");
   TORCH_CHECK(fp8_code(code) >= 0, "the code must be float8_e4m3fn or float8_e5m2");
@@ -422,12 +423,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> fp8_quantize_both(con
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t R = x.size(0), C = x.size(1);
   const at::Tensor xr = fp8_rows(x);
-  at::Tensor q = fp8_new_codes(x, R, C, code), qc = fp8_new_codes(x, R, C, code);
+  at::Tensor q = fp8_new_codes(x, R, C, code);
+  at::Tensor qc = transposed ? fp8_new_codes(x, C, R, code).t() : fp8_new_codes(x, R, C, code);
   const auto so = x.options().dtype(at::kFloat8_e8m0fnu);
   at::Tensor s = at::empty({R, fp8_blocks(C)}, so), sc = at::empty({fp8_blocks(R), C}, so);
   check(f64e_fp8_quantize_both(xr.data_ptr(), fp8_type(x.scalar_type()), R, C, fp8_pitch(xr), fp8_code(code),
-                               q.data_ptr(), s.data_ptr(), qc.data_ptr(), sc.data_ptr(), fp8_code_pitch(C),
-                               stream_of()));
+                               q.data_ptr(), s.data_ptr(), fp8_code_pitch(C), qc.data_ptr(), sc.data_ptr(), transposed,
+                               fp8_code_pitch(transposed ? R : C), stream_of()));
   return {q, s, qc, sc};
 }
 
@@ -561,7 +563,8 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optio
 
 // The same with gradients.  What the backward pass needs of x is kept in 8
 // bits with blocks along the rows of x (the tokens), the direction the weight
-// gradient contracts; the operators are called through the dispatcher, so a
+// gradient contracts, and those contiguous, so that product takes x's codes as
+// the K-major operand it needs; the operators are called through the dispatcher, so a
 // tracer sees them.
 using Two = std::tuple<at::Tensor, at::Tensor>;
 using Four = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
@@ -571,11 +574,11 @@ Two call_quantize(const at::Tensor& x, int64_t blocks) {
                        .typed<Two(const at::Tensor&, int64_t, at::ScalarType)>();
   return op.call(x, blocks, at::kFloat8_e4m3fn);
 }
-Four call_quantize_both(const at::Tensor& x) {
+Four call_quantize_both(const at::Tensor& x, bool transposed) {
   static auto op = c10::Dispatcher::singleton()
                        .findSchemaOrThrow("fp64_emu_b200::fp8_quantize_both", "")
-                       .typed<Four(const at::Tensor&, at::ScalarType)>();
-  return op.call(x, at::kFloat8_e4m3fn);
+                       .typed<Four(const at::Tensor&, at::ScalarType, bool)>();
+  return op.call(x, at::kFloat8_e4m3fn, transposed);
 }
 at::Tensor call_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa, const at::Tensor& sb,
                    int64_t layout, at::ScalarType dtype) {
@@ -600,7 +603,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     const bool want_w = w.requires_grad() && !ws.has_value();
     at::Tensor q, s, qc, sc, wq = w, wsc;
     if (want_w)
-      std::tie(q, s, qc, sc) = call_quantize_both(x2);
+      std::tie(q, s, qc, sc) = call_quantize_both(x2, true);
     else
       std::tie(q, s) = call_quantize(x2, F64E_BLOCKS_ROW);
     if (ws.has_value())
@@ -628,7 +631,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       const at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, grads[0].size(-1)});
       at::Tensor q, s, gc, gsc;
       if (want_x && want_w)
-        std::tie(q, s, gc, gsc) = call_quantize_both(g);
+        std::tie(q, s, gc, gsc) = call_quantize_both(g, false);
       else if (want_x)
         std::tie(q, s) = call_quantize(g, F64E_BLOCKS_ROW);
       else
@@ -702,7 +705,7 @@ TORCH_LIBRARY(fp64_emu_b200, ops) {
   ops.def("fp64_emu_set_wait_limit_ns(int ns) -> ()");
   ops.def("fp64_emu_wait_selftest(Tensor! ws, int limit_ns) -> int");
   ops.def("fp8_quantize(Tensor x, int blocks, ScalarType code) -> (Tensor, Tensor)");
-  ops.def("fp8_quantize_both(Tensor x, ScalarType code) -> (Tensor, Tensor, Tensor, Tensor)");
+  ops.def("fp8_quantize_both(Tensor x, ScalarType code, bool transposed) -> (Tensor, Tensor, Tensor, Tensor)");
   ops.def("fp8_dequantize(Tensor q, Tensor s, int blocks, ScalarType dtype) -> Tensor");
   ops.def("fp8_mm(Tensor a, Tensor b, Tensor sa, Tensor sb, int layout, ScalarType dtype) -> Tensor");
   ops.def("fp8_linear(Tensor x, Tensor w, Tensor? ws=None) -> Tensor");

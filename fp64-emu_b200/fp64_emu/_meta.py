@@ -43,9 +43,10 @@ def _fake_quantize(x, blocks, code):
 
 
 @torch.library.register_fake("fp64_emu_b200::fp8_quantize_both")
-def _fake_quantize_both(x, code):
+def _fake_quantize_both(x, code, transposed):
     rows, cols = x.shape
-    return _codes(x, code), _scales(x, rows, _nb(cols)), _codes(x, code), _scales(x, _nb(rows), cols)
+    qc = _codes(x.t(), code).t() if transposed else _codes(x, code)
+    return _codes(x, code), _scales(x, rows, _nb(cols)), qc, _scales(x, _nb(rows), cols)
 
 
 @torch.library.register_fake("fp64_emu_b200::fp8_dequantize")

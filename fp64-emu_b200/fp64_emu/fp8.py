@@ -35,10 +35,13 @@ def quantize_fp8(x: torch.Tensor, blocks: str = "row", code: torch.dtype = torch
     return _quantize(x, _BLOCKS[blocks], code)
 
 
-def quantize_fp8_both(x: torch.Tensor, code: torch.dtype = torch.float8_e4m3fn) -> tuple:
+def quantize_fp8_both(x: torch.Tensor, code: torch.dtype = torch.float8_e4m3fn, transposed: bool = False) -> tuple:
     """(row codes, row scales, col codes, col scales) in one pass over x: what
-    a layer's forward product and its weight gradient contract."""
-    return _quantize_both(x, code)
+    a layer's forward product and its weight gradient contract.  transposed:
+    the col codes, of the same shape, are stored with columns contiguous; a
+    product that contracts columns needs one of its operands so, and makes
+    that copy itself otherwise."""
+    return _quantize_both(x, code, transposed)
 
 
 def dequantize_fp8(codes: torch.Tensor, scales: torch.Tensor, blocks: str = "row",

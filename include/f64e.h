@@ -252,10 +252,13 @@ enum {
 F64E_API int f64e_fp8_quantize(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
                                int32_t blocks, int32_t code, void* q, int64_t ldq, void* scale, void* stream);
 
-/* Row blocks and column blocks of x in one pass over it. */
+/* Row blocks and column blocks of x in one pass over it.  transposed = 1
+ * stores the column codes as [cols][ld_col] (k_major for a product that
+ * contracts x's rows), up to the next multiple of 16 rows; 0 as [rows][ldq]
+ * (ld_col = ldq). */
 F64E_API int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t cols, int64_t ldx,
-                                    int32_t code, void* q_row, void* scale_row, void* q_col, void* scale_col,
-                                    int64_t ldq, void* stream);
+                                    int32_t code, void* q_row, void* scale_row, int64_t ldq, void* q_col,
+                                    void* scale_col, int32_t transposed, int64_t ld_col, void* stream);
 
 /* out [rows][cols] (contiguous, out_type) = code * scale, rounded once.
  * scale_row / scale_col: strides of the scales in bytes; any ldq >= cols. */

@@ -112,7 +112,7 @@ def lib():
     L = ctypes.CDLL(os.path.join(ROOT, "fp64-emu_b200", "fp64_emu", "libf64e.so"))
     vp, i64, i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
     L.f64e_fp8_quantize.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, i64, vp, vp]
-    L.f64e_fp8_quantize_both.argtypes = [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, i64, vp]
+    L.f64e_fp8_quantize_both.argtypes = [vp, i32, i64, i64, i64, i32, vp, vp, i64, vp, vp, i32, i64, vp]
     L.f64e_fp8_dequantize.argtypes = [vp, i32, i64, i64, i64, i32, vp, i64, i64, vp, i32, vp]
     L.f64e_fp8_gemm.argtypes = [ctypes.POINTER(Problem), vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     L.f64e_fp8_workspace_size.argtypes = [ctypes.POINTER(Problem)]
@@ -141,9 +141,21 @@ def test_quantize_abi_refusals(lib, args, msg):
     assert msg in lib.f64e_last_error().decode()
 
 
+@pytest.mark.parametrize("args,msg", [
+    ((P, 0, 40, 20, 20, 0, P, P, 32, P, P, 2, 32, None), "transposed must be"),
+    ((P, 0, 40, 20, 20, 0, P, P, 32, P, P, 0, 48, None), "same pitch"),
+    ((P, 0, 40, 20, 20, 0, P, P, 32, P, P, 1, 32, None), "below their columns"),
+    ((P, 0, 40, 20, 20, 0, P, P, 32, P + 1, P, 1, 48, None), "16-byte"),
+    ((P, 0, 40, 20, 20, 0, P, P, 32, P, None, 1, 48, None), "null"),
+])
+def test_quantize_both_abi_refusals(lib, args, msg):
+    assert lib.f64e_fp8_quantize_both(*args) == 1
+    assert msg in lib.f64e_last_error().decode()
+
+
 def test_quantize_abi_empty_is_done_without_a_device(lib):
     assert lib.f64e_fp8_quantize(None, 0, 0, 16, 16, 0, 0, None, 16, None, None) == 0
-    assert lib.f64e_fp8_quantize_both(None, 0, 5, 0, 0, 0, None, None, None, None, 0, None) == 0
+    assert lib.f64e_fp8_quantize_both(None, 0, 5, 0, 0, 0, None, None, 0, None, None, 0, 0, None) == 0
     assert lib.f64e_fp8_dequantize(None, 0, 0, 16, 16, 0, None, 1, 1, None, 0, None) == 0
 
 
@@ -201,6 +213,7 @@ def test_fake_kernels_give_shapes_and_types():
         assert fp64_emu.quantize_fp8(x, "tile")[1].shape == (2, 3)
         q, s, qc, sc = fp64_emu.quantize_fp8_both(x)
         assert s.shape == (200, 3) and sc.shape == (2, 300)
+        assert fp64_emu.quantize_fp8_both(x, transposed=True)[2].stride() == (1, 208)
         assert fp64_emu.dequantize_fp8(q, s, dtype=torch.float16).dtype == torch.float16
         assert fp64_emu.mm_fp8(q, q, s, s).shape == (200, 200)
         assert fp64_emu.mm_tn_fp8(qc, qc, sc, sc, torch.float32).shape == (300, 300)

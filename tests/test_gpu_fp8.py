@@ -67,6 +67,10 @@ def test_quantize_both(dtype, code):
         q, s, qc, sc = fp64_emu.quantize_fp8_both(x, code)
         check_codes(x, q, s, "row", code)
         check_codes(x, qc, sc, "col", code)
+        q2, s2, qt, st = fp64_emu.quantize_fp8_both(x, code, transposed=True)
+        assert qt.t().is_contiguous() or qt.stride(0) == 1
+        check_codes(x, qt, st, "col", code)
+        assert same(q2.float(), q.float()) and torch.equal(s2.view(torch.uint8), s.view(torch.uint8))
 
 
 @pytest.mark.parametrize("blocks", ["row", "col", "tile"])
@@ -76,6 +80,8 @@ def test_quantize_strided_inputs(blocks):
         check_codes(x, *fp64_emu.quantize_fp8(x, blocks), blocks, E4)
     q, s, qc, sc = fp64_emu.quantize_fp8_both(big[1:, 3:])
     check_codes(big[1:, 3:], q, s, "row", E4)
+    check_codes(big[1:, 3:], qc, sc, "col", E4)
+    _, _, qc, sc = fp64_emu.quantize_fp8_both(big[1:, 3:], transposed=True)
     check_codes(big[1:, 3:], qc, sc, "col", E4)
 
 
@@ -97,6 +103,10 @@ def test_quantize_special_values(blocks, dtype, code):
     q, s, qc, sc = fp64_emu.quantize_fp8_both(x, code)
     check_codes(x, q, s, "row", code)
     check_codes(x, qc, sc, "col", code)
+    check_codes(x, *fp64_emu.quantize_fp8_both(x, code, transposed=True)[2:], "col", code)
+    odd = x[:, 1:258]
+    check_codes(odd, *fp64_emu.quantize_fp8(odd, blocks, code), blocks, code)
+    check_codes(odd, *fp64_emu.quantize_fp8_both(odd, code, transposed=True)[2:], "col", code)
     q, s = fp64_emu.quantize_fp8(x, blocks, code)
     assert torch.signbit(q.float()[9, 200])
 
@@ -183,7 +193,14 @@ def operand(rows, cols, blocks, code, seed, spread=2):
     return q, s, R.values(q, s, blocks)
 
 
-def product(layout, M, N, K, out, a_blocks, b_blocks, ac=E4, bc=E4, seed=0):
+def columns_first(q):
+    """The same codes with columns contiguous."""
+    t = torch.empty(q.shape[1], q.shape[0] + (-q.shape[0] % 16), dtype=torch.uint8, device="cuda")[:, :q.shape[0]]
+    t.copy_(q.view(torch.uint8).t())
+    return t.view(q.dtype).t()
+
+
+def product(layout, M, N, K, out, a_blocks, b_blocks, ac=E4, bc=E4, seed=0, stored=False):
     if layout == "tn":
         a, sa, av = operand(K, M, a_blocks, ac, seed)
         av = av.t()
@@ -198,6 +215,9 @@ def product(layout, M, N, K, out, a_blocks, b_blocks, ac=E4, bc=E4, seed=0):
     got = f(a, b, sa, sb, out)
     assert got.shape == (M, N) and got.dtype == out and got.is_contiguous()
     R.check_product(got, av, bv)
+    if stored:   # either operand, and both, stored the other way
+        for qa, qb in ((columns_first(a), b), (a, columns_first(b)), (columns_first(a), columns_first(b))):
+            R.check_product(f(qa, qb, sa, sb, out), av, bv)
 
 
 MM_SHAPES = [(1, 1, 1), (1, 128, 128), (2, 3, 129), (17, 40, 512), (64, 256, 640), (128, 255, 1000), (130, 129, 127),
@@ -220,6 +240,15 @@ def test_products_of_codes(layout, ac, bc):
     a_vec = "col" if layout == "tn" else "row"
     product(layout, 200, 264, 700, SF, a_vec, "tile", ac, bc)
     product(layout, 5, 264, 700, BF, a_vec, "tile", ac, bc)
+
+
+@pytest.mark.parametrize("layout", ["nt", "nn", "tn"])
+@pytest.mark.parametrize("out", [BF, SF])
+def test_products_of_operands_stored_either_way(layout, out):
+    a_vec = "col" if layout == "tn" else "row"
+    b_vec = "row" if layout == "nt" else "col"
+    for M, N, K in ((1, 3, 5), (130, 264, 700), (300, 520, 4100), (17, 600, 1000)):
+        product(layout, M, N, K, out, a_vec, b_vec, seed=3, stored=True)
 
 
 @pytest.mark.parametrize("M", [1, 2, 8, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 96, 127, 128, 129, 192, 256])
