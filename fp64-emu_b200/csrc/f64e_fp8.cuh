@@ -42,7 +42,8 @@ __device__ __forceinline__ float scale_of_byte(uint32_t b) {
 
 // ------------------------------------------------------------------ codes --
 // Two codes from two scaled values, `lo` in the low byte.  Finite values are
-// within FMAX by the choice of the scale; a NaN becomes a NaN code.
+// within FMAX by the choice of the scale; a NaN becomes a NaN code (and an
+// infinity would become the largest finite one, see infs_to_nan).
 template <int CODE>
 __device__ __forceinline__ uint32_t code2(float lo, float hi) {
   uint16_t r;
@@ -51,12 +52,6 @@ __device__ __forceinline__ uint32_t code2(float lo, float hi) {
   else
     asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
-}
-// The code of an infinity (the conversion above would saturate it): infinity
-// where the type has one, NaN in e4m3.
-template <int CODE>
-__device__ __forceinline__ uint32_t code_of_inf(bool negative) {
-  return (CODE == F64E_E4M3 ? 0x7Fu : 0x7Cu) | (negative ? 0x80u : 0u);
 }
 template <int CODE>
 __device__ __forceinline__ float2 values2(uint32_t codes) {
@@ -71,7 +66,7 @@ __device__ __forceinline__ float2 values2(uint32_t codes) {
 // --------------------------------------------------------------- elements --
 // Sixteen elements of a thread as 32-bit words (two 16-bit elements a word),
 // their largest magnitude, and their values.  NaN never counts as a largest
-// magnitude; an infinity does, and is looked for by the callers.
+// magnitude.
 template <int T>
 struct Elem;
 template <>
@@ -85,6 +80,7 @@ struct Elem<F64E_F32> {
   __device__ static mag shfl(mag a, int o) { return __shfl_xor_sync(0xFFFFFFFFu, a, o); }
   __device__ static float get(const uint32_t* w, int i) { return __uint_as_float(w[i]); }
   __device__ static uint32_t bits(float v) { return __float_as_uint(v); }
+  __device__ static uint32_t pack(float, float) { return 0; }   // two elements never share a word
 };
 template <typename H2>
 struct Elem16 {
@@ -114,6 +110,10 @@ struct Elem<F64E_F16> : Elem16<__half2> {
   __device__ static float lo(__half2 m) { return __low2float(m); }
   __device__ static float hi(__half2 m) { return __high2float(m); }
   __device__ static uint32_t bits(float v) { return (uint32_t)__half_as_ushort(__float2half_rn(v)); }
+  __device__ static uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 template <>
 struct Elem<F64E_BF16> : Elem16<__nv_bfloat162> {
@@ -124,6 +124,10 @@ struct Elem<F64E_BF16> : Elem16<__nv_bfloat162> {
   __device__ static float lo(__nv_bfloat162 m) { return __low2float(m); }
   __device__ static float hi(__nv_bfloat162 m) { return __high2float(m); }
   __device__ static uint32_t bits(float v) { return (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+  __device__ static uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 
 // Sixteen contiguous elements at p, all there: 32-byte loads where `wide`
@@ -177,34 +181,30 @@ __device__ __forceinline__ float max16(const uint32_t* w) {
   for (int i = 0; i < Elem<T>::kWords; i++) m = Elem<T>::max_mag(m, w[i]);
   return fold(m);
 }
-// The same over finite values only.
-template <int T>
-__device__ __forceinline__ float max16_finite(const uint32_t* w) {
-  float m = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; i++) {
-    const float v = fabsf(Elem<T>::get(w, i));
-    if (v < __uint_as_float(0x7F800000u)) m = fmaxf(m, v);
-  }
-  return m;
-}
 __device__ __forceinline__ bool is_inf(float m) { return __float_as_uint(m) == 0x7F800000u; }
+// Infinities among sixteen elements become NaN: no scale could hold them, and
+// as NaN they neither count as magnitudes nor saturate.  Where a block's
+// largest magnitude is infinite it is taken again after this.
+template <int T>
+__device__ __forceinline__ void infs_to_nan(uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kWords; i++) {
+    if (T == F64E_F32) {
+      if ((w[i] & 0x7FFFFFFFu) == 0x7F800000u) w[i] = 0x7FFFFFFFu;
+    } else {
+      constexpr uint32_t inf = T == F64E_F16 ? 0x7C00u : 0x7F80u;
+      if ((w[i] & 0x7FFFu) == inf) w[i] |= 0x7FFFu;
+      if (((w[i] >> 16) & 0x7FFFu) == inf) w[i] |= 0x7FFF0000u;
+    }
+  }
+}
 
-// Codes of sixteen elements, two a word: element i scaled by r(i).  infs: some
-// block here holds an infinity, which the conversion would saturate.
+// Codes of sixteen elements, two a word: element i scaled by r(i).
 template <int T, int CODE, typename R>
-__device__ __forceinline__ void codes16(const uint32_t* w, R r, bool infs, uint32_t* c) {
+__device__ __forceinline__ void codes16(const uint32_t* w, R r, uint32_t* c) {
 #pragma unroll
   for (int i = 0; i < 8; i++)
     c[i] = code2<CODE>(Elem<T>::get(w, 2 * i) * r(2 * i), Elem<T>::get(w, 2 * i + 1) * r(2 * i + 1));
-  if (infs) {
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float v = Elem<T>::get(w, i);
-      if (is_inf(fabsf(v)))
-        c[i >> 1] = (c[i >> 1] & ~(0xFFu << (8 * (i & 1)))) | (code_of_inf<CODE>(v < 0.f) << (8 * (i & 1)));
-    }
-  }
 }
 // The words of sixteen neighbouring codes.
 __device__ __forceinline__ uint4 row_of_codes(const uint32_t* c) {

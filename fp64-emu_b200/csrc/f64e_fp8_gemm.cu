@@ -39,16 +39,6 @@ __device__ __forceinline__ uint32_t staged_at(int row, int piece) {
   return (uint32_t)(row * RB + ((RB == 64 ? piece ^ ((row >> 1) & 3) : piece ^ (row & 7)) << 4));
 }
 
-template <int OUT>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if (OUT == F64E_F16) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // The staged rows to out (row pitch ldo elements), of which `rows` rows and
 // `cols` columns exist.
 template <int OUT, int RB>
@@ -81,8 +71,8 @@ __device__ __forceinline__ void stage_row(uint8_t* stage, int lane, const float*
           make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     else
       *reinterpret_cast<uint4*>(stage + staged_at<64>(lane, i)) =
-          make_uint4(pack2<OUT>(v[8 * i], v[8 * i + 1]), pack2<OUT>(v[8 * i + 2], v[8 * i + 3]),
-                     pack2<OUT>(v[8 * i + 4], v[8 * i + 5]), pack2<OUT>(v[8 * i + 6], v[8 * i + 7]));
+          make_uint4(Elem<OUT>::pack(v[8 * i], v[8 * i + 1]), Elem<OUT>::pack(v[8 * i + 2], v[8 * i + 3]),
+                     Elem<OUT>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<OUT>::pack(v[8 * i + 6], v[8 * i + 7]));
 }
 // The same of a transposed tile: this lane's accumulators are one column of
 // the staged rows (32 columns).
@@ -96,7 +86,7 @@ __device__ __forceinline__ void stage_column(uint8_t* stage, int lane, const flo
       *reinterpret_cast<float*>(stage + staged_at<RB>(i, ch) + at) = v[i];
       *reinterpret_cast<float*>(stage + staged_at<RB>(i + 1, ch) + at) = v[i + 1];
     } else {
-      const uint32_t p = pack2<OUT>(v[i], v[i + 1]);
+      const uint32_t p = Elem<OUT>::pack(v[i], v[i + 1]);
       *reinterpret_cast<uint16_t*>(stage + staged_at<RB>(i, ch) + at) = (uint16_t)p;
       *reinterpret_cast<uint16_t*>(stage + staged_at<RB>(i + 1, ch) + at) = (uint16_t)(p >> 16);
     }

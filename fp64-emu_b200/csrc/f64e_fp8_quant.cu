@@ -24,14 +24,13 @@ __device__ __forceinline__ float max_over_block(float m) {
   for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   return m;
 }
-// Exponent of the row block these lanes hold.
+// Exponent of the row block these lanes hold; its infinities are NaN after.
 template <int T, int CODE>
-__device__ __forceinline__ int row_exponent(const uint32_t* w, bool* infs) {
+__device__ __forceinline__ int row_exponent(uint32_t* w) {
   float m = max_over_block(max16<T>(w));
-  *infs = is_inf(m);
-  if (__any_sync(0xFFFFFFFFu, *infs)) {
-    const float f = max_over_block(max16_finite<T>(w));
-    if (*infs) m = f;
+  if (__any_sync(0xFFFFFFFFu, is_inf(m))) {
+    infs_to_nan<T>(w);
+    m = max_over_block(max16<T>(w));
   }
   return scale_exponent<CODE>(m);
 }
@@ -70,11 +69,10 @@ __global__ void __launch_bounds__(kThreads) fp8_quant_rows_kernel(const Fp8Quant
     load_row<T, VEC>(x + u * a.ldx, l, row0 + u < a.rows ? a.cols - col : 0, wide, w[u]);
 #pragma unroll
   for (int u = 0; u < kRowPasses; u++) {
-    bool infs;
-    const int e = row_exponent<T, CODE>(w[u], &infs);
+    const int e = row_exponent<T, CODE>(w[u]);
     const float r = inverse_scale(e);
     uint32_t c[8];
-    codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c);
+    codes16<T, CODE>(w[u], [&](int) { return r; }, c);
     uint4 v;
     if (VEC) {
       v = row_of_codes(c);
@@ -106,25 +104,29 @@ enum { kCols = 0, kRowsCols = 1, kTile = 2, kRowsColsT = 3 };
 struct SquareSmem {
   float max[kThreads / 32][kFp8Block];
   float inv[kFp8Block];
-  int infs;
 };
 
-// Row-major codes of the thread's four rows; VEC = false puts them in order in
-// `tile` (the whole CTA calls it).
-template <bool VEC>
+// Row-major codes of the thread's four rows, codes(u, c) giving those of row u.
+// VEC = false puts them in order in `tile` (the whole CTA calls it).
+template <bool VEC, typename F>
 __device__ __forceinline__ void store_rows(uint8_t* q, int64_t ldq, int64_t rows, int64_t row0, int64_t col,
-                                           int64_t padded, int g, int l, uint8_t* tile, const uint32_t (&c)[4][8]) {
+                                           int64_t padded, int g, int l, uint8_t* tile, F codes) {
+  uint32_t c[8];
   if (VEC) {
+    uint8_t* p = q + (row0 + 4 * g) * ldq + col + l * 16;
 #pragma unroll
-    for (int u = 0; u < 4; u++)
-      if (row0 + 4 * g + u < rows && col + l * 16 < padded)
-        *reinterpret_cast<uint4*>(q + (row0 + 4 * g + u) * ldq + col + l * 16) = row_of_codes(c[u]);
+    for (int u = 0; u < 4; u++) {
+      codes(u, c);
+      if (row0 + 4 * g + u < rows && col + l * 16 < padded) *reinterpret_cast<uint4*>(p + u * ldq) = row_of_codes(c);
+    }
   } else {
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 4; u++)
+    for (int u = 0; u < 4; u++) {
+      codes(u, c);
 #pragma unroll
-      for (int i = 0; i < 16; i++) tile[(4 * g + u) * 128 + i * 8 + l] = (uint8_t)(c[u][i >> 1] >> (8 * (i & 1)));
+      for (int i = 0; i < 16; i++) tile[(4 * g + u) * 128 + i * 8 + l] = (uint8_t)(c[i >> 1] >> (8 * (i & 1)));
+    }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < 4; u++) {
@@ -159,7 +161,8 @@ __device__ __forceinline__ void store_columns(uint8_t* qt, int64_t ldt, int64_t 
 }
 
 template <int T, int CODE, int MODE, bool VEC>
-__global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8QuantArgs a, int nkb, bool wide) {
+__global__ void __launch_bounds__(kThreads, T == F64E_F32 || MODE == kRowsCols ? 2 : MODE == kRowsColsT ? 3 : 4)
+    fp8_quant_squares_kernel(const Fp8QuantArgs a, int nkb, bool wide) {
   using E = Elem<T>;
   __shared__ SquareSmem sm;
   __shared__ __align__(16) uint8_t tile[!VEC || MODE == kRowsColsT ? 128 * 128 : 16];
@@ -168,59 +171,57 @@ __global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8Qu
   const int64_t rb = blockIdx.x / nkb, row0 = rb * kFp8Block, col = (int64_t)kb * kFp8Block;
   const int64_t padded = (a.cols + 15) & ~(int64_t)15;
   const typename E::type* x = static_cast<const typename E::type*>(a.x) + (row0 + 4 * g) * a.ldx + col;
-  uint32_t w[4][E::kWords], c[4][8];
+  uint32_t w[4][E::kWords];
 #pragma unroll
   for (int u = 0; u < 4; u++)
     load_row<T, VEC>(x + u * a.ldx, l, row0 + 4 * g + u < a.rows ? a.cols - col : 0, wide, w[u]);
-  if (threadIdx.x == 0) sm.infs = 0;
+
+  // Rows are unpacked one after the other, each time anew: all 64 values kept
+  // as floats would leave an SM one CTA instead of three.
+  auto one_row = [](uint32_t (&r)[E::kWords]) {
+#pragma unroll
+    for (int k = 0; k < E::kWords; k++) asm volatile("" : "+r"(r[k])::"memory");
+  };
 
   if (MODE == kTile) {
-    float m = 0.f;
-#pragma unroll
-    for (int u = 0; u < 4; u++) m = fmaxf(m, max16<T>(w[u]));
-    auto over_square = [&](float v) {
-#pragma unroll
-      for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-      if (lane == 0) sm.inv[warp] = v;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; i++) v = fmaxf(v, sm.inv[i]);
-      __syncthreads();
-      return v;
-    };
-    m = over_square(m);
-    const bool infs = is_inf(m);
-    if (infs) {
+    float m;
+    while (true) {   // a second time after infinities
       m = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; u++) m = fmaxf(m, max16_finite<T>(w[u]));
-      m = over_square(m);
+      for (int u = 0; u < 4; u++) m = fmaxf(m, max16<T>(w[u]));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      if (lane == 0) sm.inv[warp] = m;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; i++) m = fmaxf(m, sm.inv[i]);
+      if (!is_inf(m)) break;
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 4; u++) infs_to_nan<T>(w[u]);
     }
     const int e = scale_exponent<CODE>(m);
     const float r = inverse_scale(e);
-#pragma unroll
-    for (int u = 0; u < 4; u++) codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c[u]);
-    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
+    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, [&](int u, uint32_t* c) {
+      one_row(w[u]);
+      codes16<T, CODE>(w[u], [&](int) { return r; }, c);
+    });
     if (threadIdx.x == 0) a.s[rb * nkb + kb] = (uint8_t)(e + 127);
     return;
   }
 
-  // Row blocks first: their registers are free again before the columns'.
   if (MODE == kRowsCols || MODE == kRowsColsT) {
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      bool infs;
-      const int e = row_exponent<T, CODE>(w[u], &infs);
+    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, [&](int u, uint32_t* c) {
+      one_row(w[u]);
+      const int e = row_exponent<T, CODE>(w[u]);
       const float r = inverse_scale(e);
-      codes16<T, CODE>(w[u], [&](int) { return r; }, infs, c[u]);
+      codes16<T, CODE>(w[u], [&](int) { return r; }, c);
       const int64_t row = row0 + 4 * g + u;
       if (l == 0 && row < a.rows) a.s[row * nkb + kb] = (uint8_t)(e + 127);
-    }
-    store_rows<VEC>(a.q, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
+    });
   }
 
-  auto publish = [&](int i, float m) { sm.max[warp][col_of<VEC>(l, i)] = m; };
-  {
+  while (true) {   // a second time after infinities (the rows above left none)
     typename E::mag m[E::kWords];
 #pragma unroll
     for (int k = 0; k < E::kWords; k++) {
@@ -234,44 +235,30 @@ __global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8Qu
     for (int k = 0; k < E::kWords; k++)
       if ((lane >> 3) == k * 4 / E::kWords) {   // each of the four writes a quarter
         if constexpr (T == F64E_F32) {
-          publish(k, m[k]);
+          sm.max[warp][col_of<VEC>(l, k)] = m[k];
         } else {
-          publish(2 * k, E::lo(m[k]));
-          publish(2 * k + 1, E::hi(m[k]));
+          sm.max[warp][col_of<VEC>(l, 2 * k)] = E::lo(m[k]);
+          sm.max[warp][col_of<VEC>(l, 2 * k + 1)] = E::hi(m[k]);
         }
       }
-  }
-  auto finish = [&]() {
     __syncthreads();
+    float top = 0.f;
     if (threadIdx.x < kFp8Block) {
-      float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; i++) m = fmaxf(m, sm.max[i][threadIdx.x]);
-      if (is_inf(m)) {
-        sm.infs = 1;
-      }
-      const int e = is_inf(m) ? 0 : scale_exponent<CODE>(m);
+      for (int i = 0; i < kThreads / 32; i++) top = fmaxf(top, sm.max[i][threadIdx.x]);
+    }
+    if (MODE == kCols && __syncthreads_or(is_inf(top))) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) infs_to_nan<T>(w[u]);
+      continue;
+    }
+    if (threadIdx.x < kFp8Block) {
+      const int e = scale_exponent<CODE>(top);
       sm.inv[threadIdx.x] = inverse_scale(e);
       if (col + threadIdx.x < a.cols) a.sc[rb * a.cols + col + threadIdx.x] = (uint8_t)(e + 127);
     }
     __syncthreads();
-  };
-  finish();
-  const bool infs = sm.infs != 0;
-  if (infs) {   // the columns once more, over finite values
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      float m = 0.f;
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        const float v = fabsf(E::get(w[u], i));
-        if (v < __uint_as_float(0x7F800000u)) m = fmaxf(m, v);
-      }
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
-      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-      if (lane < 8) publish(i, m);
-    }
-    finish();
+    break;
   }
   float r[16];
   if (VEC) {
@@ -287,12 +274,18 @@ __global__ void __launch_bounds__(kThreads) fp8_quant_squares_kernel(const Fp8Qu
 #pragma unroll
     for (int i = 0; i < 16; i++) r[i] = sm.inv[i * 8 + l];
   }
+  auto codes = [&](int u, uint32_t* c) {
+    one_row(w[u]);
+    codes16<T, CODE>(w[u], [&](int i) { return r[i]; }, c);
+  };
+  if (MODE == kRowsColsT) {
+    uint32_t c[4][8];
 #pragma unroll
-  for (int u = 0; u < 4; u++) codes16<T, CODE>(w[u], [&](int i) { return r[i]; }, infs, c[u]);
-  if (MODE == kRowsColsT)
+    for (int u = 0; u < 4; u++) codes(u, c[u]);
     store_columns<VEC>(a.qc, a.ldt, a.cols, (a.rows + 15) & ~(int64_t)15, row0, col, g, l, tile, c);
-  else
-    store_rows<VEC>(a.qc, a.ldq, a.rows, row0, col, padded, g, l, tile, c);
+  } else {
+    store_rows<VEC>(a.qc, a.ldq, a.rows, row0, col, padded, g, l, tile, codes);
+  }
 }
 
 // --------------------------------------------------------- dequantise ----
@@ -354,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
       uint32_t b[Elem<T>::kWords];
 #pragma unroll
       for (int i = 0; i < Elem<T>::kWords; i++)
-        b[i] = T == F64E_F32 ? Elem<T>::bits(f[i]) : Elem<T>::bits(f[(2 * i) & 15]) | (Elem<T>::bits(f[(2 * i + 1) & 15]) << 16);
+        b[i] = T == F64E_F32 ? Elem<T>::bits(f[i]) : Elem<T>::pack(f[(2 * i) & 15], f[(2 * i + 1) & 15]);
       uint32_t* ow = reinterpret_cast<uint32_t*>(o + l * 16);
       if (wide) {
 #pragma unroll

@@ -631,7 +631,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
       const at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, grads[0].size(-1)});
       at::Tensor q, s, gc, gsc;
       if (want_x && want_w)
-        std::tie(q, s, gc, gsc) = call_quantize_both(g, false);
+        std::tie(q, s, gc, gsc) = call_quantize_both(g, true);
       else if (want_x)
         std::tie(q, s) = call_quantize(g, F64E_BLOCKS_ROW);
       else

@@ -3,8 +3,8 @@
 A block of up to 128 values with largest finite magnitude amax is held as codes
 (float8_e4m3fn, or float8_e5m2 for values of wider range) and one scale 2^e
 (float8_e8m0fnu), e the smallest integer >= -127 with amax <= FMAX * 2^e; a code
-is the round-to-nearest-even 8-bit float of x * 2^-e.  NaN stays NaN; infinity
-becomes NaN in e4m3 and stays infinity in e5m2; neither counts towards amax.
+is the round-to-nearest-even 8-bit float of x * 2^-e.  NaN stays NaN,
+infinity becomes NaN, and neither counts towards amax.
 
 Which values of a matrix [R, C] share a scale:
   "row"   128 neighbours of a row       scales [R, ceil(C / 128)]

@@ -233,8 +233,8 @@ F64E_API int f64e_mm_nt_noalloc(double* out, const double* A, const double* Bt, 
  * finite magnitude amax is held as 8-bit codes and one scale 2^e, e the
  * smallest integer >= -127 with amax <= FMAX * 2^e (FMAX = 448 in e4m3, 57344
  * in e5m2; e = 0 for a block of zeros), stored as the byte e + 127.  A code is
- * the round-to-nearest-even 8-bit float of x * 2^-e; NaN stays NaN, infinity
- * becomes NaN in e4m3 and stays infinity in e5m2.  Rows of codes start on
+ * the round-to-nearest-even 8-bit float of x * 2^-e; NaN stays NaN, and
+ * infinity becomes NaN; neither counts towards amax.  Rows of codes start on
  * 16-byte boundaries (pitch a multiple of 16).  Nothing here allocates or
  * synchronizes, except f64e_fp8_status. */
 enum { F64E_F32 = 0, F64E_F16 = 1, F64E_BF16 = 2 }; /* element types */

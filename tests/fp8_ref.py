@@ -51,11 +51,7 @@ def quantize(x, blocks, code):
     ex = torch.floor(torch.log2(t.abs().clamp(min=2.0 ** emin))).clamp(min=emin)
     step = pow2(ex - man)
     v = torch.round(t / step) * step
-    if code == E4M3:
-        v = torch.where(torch.isinf(t), torch.full_like(v, float("nan")), v)
-    else:
-        v = torch.where(torch.isinf(t), t, v)
-    return v, e
+    return torch.where(torch.isinf(t), torch.full_like(v, float("nan")), v), e
 
 
 def values(codes, scales, blocks):
