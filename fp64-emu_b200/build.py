@@ -34,7 +34,7 @@ CXX = "/usr/bin/g++"
 
 CUDA_SOURCES = ["f64e_api.cu", "f64e_sizing.cu", "f64e_extract.cu", "f64e_gemm.cu", "f64e_gemm_check.cu",
                 "f64e_recon.cu", "f64e_deepk.cu", "f64e_noalloc.cu", "f64e_fp8_quant.cu", "f64e_fp8_gemm.cu",
-                "f64e_fp8_api.cu"]
+                "f64e_fp8_split.cu", "f64e_fp8_api.cu"]
 HEADERS = ["f64e_device.cuh", "f64e_params.h", "f64e_kernels.h", "f64e_crt64.cuh", "f64e_fp8.h", "f64e_fp8.cuh"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-ccbin", CXX,

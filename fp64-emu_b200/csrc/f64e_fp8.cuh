@@ -17,6 +17,7 @@
 
 #include "f64e.h"
 #include "f64e_device.cuh"
+#include "f64e_fp8.h"
 
 namespace f64e {
 
@@ -357,6 +358,42 @@ __device__ __forceinline__ void mma_mx_pair(uint32_t d_tmem, uint64_t a_desc, ui
           d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
       : "memory");
+}
+
+enum : int { kWaitScales = 6, kWaitScalesFree = 7 };   // status sites, beside kWait*
+
+// --------------------------------------------------------------- scales --
+// Scale words of `N` atoms (rows r0 + 128 n + lane, + 32, + 64, + 96), a word
+// the bytes of blocks 4 j .. 4 j + 3.  Rows and blocks outside the operand read
+// their nearest neighbour's scale: their codes are zeros, and no store uses
+// them.  So no load depends on a branch, and all of them are in flight at once:
+// taken one word after the other they, not the MMAs, set the kernel's pace
+// where scales are strided bytes (4096 x 4096 x 8192 with column scales on
+// both sides: 231 us instead of 125).
+template <int N>
+__device__ __forceinline__ void scale_atoms(const Fp8Operand& o, int rows, int nkb, int r0, int j, int lane,
+                                            bool words, uint4* atoms) {
+  const uint8_t* p[4 * N];
+#pragma unroll
+  for (int w = 0; w < 4 * N; w++)
+    p[w] = o.s + (int64_t)(min(r0 + w * 32 + lane, rows - 1) >> o.s_shift) * o.s_row;
+  uint32_t v[4 * N];
+  if (words && 4 * j + 4 <= nkb) {
+#pragma unroll
+    for (int w = 0; w < 4 * N; w++) v[w] = __ldg(reinterpret_cast<const uint32_t*>(p[w] + 4 * j));
+  } else {
+    uint32_t b[4 * N][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
+#pragma unroll
+      for (int w = 0; w < 4 * N; w++) b[w][i] = __ldg(p[w] + at);
+    }
+#pragma unroll
+    for (int w = 0; w < 4 * N; w++) v[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);
+  }
+#pragma unroll
+  for (int n = 0; n < N; n++) atoms[n] = make_uint4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
 }
 
 }  // namespace f64e

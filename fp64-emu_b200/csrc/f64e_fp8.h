@@ -65,7 +65,34 @@ struct Fp8GemmArgs {
 // Scratch bytes the product needs (0: none).
 int64_t fp8_gemm_workspace(const Fp8GemmArgs& g);
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s);
-// The device's status word of these products, cleared by the read; synchronizes.
+// The same product on one-CTA tiles whose K is split over a cluster
+// (f64e_fp8_split.cu), for few rows or columns.
+struct Fp8SplitPlan {
+  int cols;        // columns of a tile: the smaller dimension, a multiple of 16 up to 256
+  int split;       // CTAs that share a tile's K
+  bool use;
+};
+Fp8SplitPlan fp8_split_plan(const Fp8GemmArgs& g);
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, const Fp8SplitPlan& p, cudaStream_t s);
+// y = quantised(x) @ w^T for a few rows of x (at most kFusedRows): x is
+// quantised in row blocks by the CTAs that contract it.
+constexpr int kFusedRows = 32;
+struct Fp8LinearArgs {
+  Fp8GemmArgs g;   // b: the weights; a unused
+  const void* x;   // [M][ldx] of type x_type; the output has the same type
+  int64_t ldx;
+  int x_type;
+};
+cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s);
+
+// Host helpers shared by the two.
+bool fp8_encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
+                   int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle);
+bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K, int box_rows);
+bool fp8_scale_words(const Fp8Operand& o);
+
+// The device's status words of these products, cleared by the read; synchronizes.
+cudaError_t read_fp8_split_status(int* status, cudaStream_t s);
 cudaError_t read_fp8_status(int* status, cudaStream_t s);
 
 }  // namespace f64e

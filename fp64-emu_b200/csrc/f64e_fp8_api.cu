@@ -19,6 +19,7 @@ constexpr int64_t kMaxDim = (int64_t)1 << 30;   // tile coordinates are 32-bit
 
 int bad(const char* msg) { return report_error(F64E_ERR_ARGUMENT, msg); }
 int cuda_error(cudaError_t e) { return report_error(F64E_ERR_CUDA, cudaGetErrorString(e)); }
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 int64_t blocks_of(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
 
 const char* check_types(int x_type, int code) {
@@ -197,6 +198,58 @@ int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale,
   g.wait_limit_ns = wait_limit_ns();
   if (const int rc = device_sms(&g.sms)) return rc;
   const cudaError_t e = launch_fp8_gemm(g, workspace, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
+size_t f64e_fp8_linear_workspace_size(int64_t M, int64_t K) {
+  begin_call();
+  if (check_matrix(M, K)) {
+    bad(check_matrix(M, K));
+    return 0;
+  }
+  if (M <= kFusedRows) return 0;
+  return (size_t)(round_up(M * round_up(K, 16), 256) + M * blocks_of(K));
+}
+
+int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const void* w, const void* w_scale,
+                    void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  begin_call();
+  if (!p) return bad("fp8: null problem");
+  f64e_fp8_problem q = *p;   // the operand a: x's codes, row blocks
+  q.a.ld = round_up(std::max<int64_t>(q.K, 1), 16);
+  q.a.code = F64E_E4M3;
+  q.a.tile = 0;
+  q.a.k_major = 1;
+  q.a.scale_row = blocks_of(q.K);
+  q.a.scale_block = 1;
+  Fp8LinearArgs a{};
+  if (const int rc = check_problem(&q, &a.g)) return rc;
+  if (const char* m = check_matrix(q.M, q.K)) return bad(m);
+  if (q.M == 0 || q.N == 0) return F64E_OK;
+  if (q.K == 0) return bad("fp8: K must be at least 1");
+  if (!x || !w || !w_scale || !out) return bad("fp8: null pointer");
+  if (ldx < q.K) return bad("fp8: row pitch of x is below its columns");
+  if (reinterpret_cast<uintptr_t>(w) & 15) return bad("fp8: codes need 16-byte aligned rows");
+  if (q.M > kFusedRows) {
+    const size_t need = f64e_fp8_linear_workspace_size(q.M, q.K);
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
+      return report_error(F64E_ERR_WORKSPACE, "fp8: workspace missing, too small or not 256-byte aligned");
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + round_up(q.M * q.a.ld, 256);
+    if (const int rc = f64e_fp8_quantize(x, q.out_type, q.M, q.K, ldx, F64E_BLOCKS_ROW, F64E_E4M3, codes, q.a.ld,
+                                         scales, stream))
+      return rc;
+    return f64e_fp8_gemm(&q, codes, scales, w, w_scale, out, nullptr, 0, stream);
+  }
+  a.g.b.q = static_cast<const uint8_t*>(w);
+  a.g.b.s = static_cast<const uint8_t*>(w_scale);
+  a.g.out = out;
+  a.g.wait_limit_ns = wait_limit_ns();
+  a.x = x;
+  a.ldx = ldx;
+  a.x_type = q.out_type;
+  if (const int rc = device_sms(&a.g.sms)) return rc;
+  const cudaError_t e = launch_fp8_linear_few(a, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? F64E_OK : cuda_error(e);
 }
 

@@ -19,6 +19,42 @@ namespace f64e {
 // First wait that ran out in a product on this device (kWait*), 0 if none.
 __device__ int g_fp8_status;
 
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult qr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) != cudaSuccess ||
+        qr != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+bool fp8_encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
+               int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle) {
+  const EncodeFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
+  const cuuint64_t gstride[1] = {(cuuint64_t)pitch_bytes};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
+  const cuuint32_t estride[2] = {1, 1};
+  return fn(map, type, 2, base, gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// An operand as TMA sees it: boxes of 128 values of k by box_rows rows (128 when
+// MN-major) of a byte matrix with pitch ld (a multiple of 16), 128-byte
+// swizzle, zeros outside.
+bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K, int box_rows) {
+  return fp8_encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(o.q), o.kmajor ? K : rows,
+                   o.kmajor ? rows : K, o.ld, 128, o.kmajor ? box_rows : 128, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+bool fp8_scale_words(const Fp8Operand& o) {
+  return o.s_kb == 1 && o.s_row % 4 == 0 && (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
+}
+
 namespace {
 
 // ------------------------------------------------------------- epilogue --
@@ -93,40 +129,6 @@ __device__ __forceinline__ void stage_column(uint8_t* stage, int lane, const flo
   }
 }
 
-// --------------------------------------------------------------- scales --
-// Scale words of `N` atoms (rows r0 + 128 n + lane, + 32, + 64, + 96), a word
-// the bytes of blocks 4 j .. 4 j + 3.  Rows and blocks outside the operand read
-// their nearest neighbour's scale: their codes are zeros, and no store uses
-// them.  So no load depends on a branch, and all of them are in flight at once:
-// taken one word after the other they, not the MMAs, set the kernel's pace
-// where scales are strided bytes (4096 x 4096 x 8192 with column scales on
-// both sides: 231 us instead of 125).
-template <int N>
-__device__ __forceinline__ void scale_atoms(const Fp8Operand& o, int rows, int nkb, int r0, int j, int lane,
-                                            bool words, uint4* atoms) {
-  const uint8_t* p[4 * N];
-#pragma unroll
-  for (int w = 0; w < 4 * N; w++)
-    p[w] = o.s + (int64_t)(min(r0 + w * 32 + lane, rows - 1) >> o.s_shift) * o.s_row;
-  uint32_t v[4 * N];
-  if (words && 4 * j + 4 <= nkb) {
-#pragma unroll
-    for (int w = 0; w < 4 * N; w++) v[w] = __ldg(reinterpret_cast<const uint32_t*>(p[w] + 4 * j));
-  } else {
-    uint32_t b[4 * N][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
-#pragma unroll
-      for (int w = 0; w < 4 * N; w++) b[w][i] = __ldg(p[w] + at);
-    }
-#pragma unroll
-    for (int w = 0; w < 4 * N; w++) v[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);
-  }
-#pragma unroll
-  for (int n = 0; n < N; n++) atoms[n] = make_uint4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
-}
-
 // The kernel's view of a product: a tile has rows of operand a and columns of
 // operand b.  out element (row, col) is at row * ldo + col, or transposed.
 struct GemmK {
@@ -174,8 +176,6 @@ constexpr uint32_t ATOM = 512, SF_BYTES = 3 * ATOM;   // A's rows, B's rows 0-12
 constexpr uint32_t TILE_BYTES = PHALF * BK, STAGE_BYTES = 2 * TILE_BYTES;
 constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 224, SF_COL = 480, SF_COLS = 12;   // scales: two buffers of 4 + 8
 constexpr size_t PSMEM = 1024 + (size_t)STAGES * STAGE_BYTES + 2 * EPI_WARPS * kStage + SF_STAGES * SF_BYTES + 256;
-
-enum : int { kWaitScales = 6, kWaitScalesFree = 7 };
 
 __device__ __forceinline__ void tile_origin(int tile, int ntm, int ntn, int& m0, int& n0) {
   const int gsz = PGROUP_M * ntn;
@@ -528,55 +528,20 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   }
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult qr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &qr) != cudaSuccess ||
-        qr != cudaDriverEntryPointSuccess)
-      f = nullptr;
-    return reinterpret_cast<EncodeFn>(f);
-  }();
-  return fn;
-}
-bool encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
-               int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle) {
-  const EncodeFn fn = encode_fn();
-  if (!fn) return false;
-  const cuuint64_t gdim[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-  const cuuint64_t gstride[1] = {(cuuint64_t)pitch_bytes};
-  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_outer};
-  const cuuint32_t estride[2] = {1, 1};
-  return fn(map, type, 2, base, gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// An operand as TMA sees it: 128 x 128 boxes of a byte matrix with pitch ld (a
-// multiple of 16), 128-byte swizzle, zeros outside.
-bool encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K) {
-  return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(o.q), o.kmajor ? K : rows,
-                   o.kmajor ? rows : K, o.ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-}
 // The output in boxes of one staged block.
 template <int OUT, bool TRANS>
 bool encode_out(CUtensorMap* map, const GemmK& k) {
   constexpr int ES = OutOf<OUT>::kBytes, RB = TRANS ? 32 * ES : 64;
-  return encode_2d(map, ES == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, k.out,
+  return fp8_encode_2d(map, ES == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, k.out,
                    TRANS ? k.M : k.N, TRANS ? k.N : k.M, k.ldo * ES, RB / ES, (int)kStage / RB,
                    RB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-bool scale_words(const Fp8Operand& o) {
-  return o.s_kb == 1 && o.s_row % 4 == 0 && (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
 }
 
 template <int OUT, bool TRANS>
 cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   CUtensorMap ta, tb;
   CUtensorMap to = {};
-  if (!encode_codes(&ta, k.a, k.M, K) || !encode_codes(&tb, k.b, k.N, K) ||
+  if (!fp8_encode_codes(&ta, k.a, k.M, K, 128) || !fp8_encode_codes(&tb, k.b, k.N, K, 128) ||
       (k.tma_out && !encode_out<OUT, TRANS>(&to, k)))
     return cudaErrorInvalidValue;
   int dev = 0;
@@ -680,11 +645,13 @@ bool transpose_first(int64_t M, int64_t N, int64_t K, int sms) {
 }  // namespace
 
 int64_t fp8_gemm_workspace(const Fp8GemmArgs& g) {
-  if (g.a.kmajor || g.b.kmajor || !transpose_first(g.M, g.N, g.K, 148)) return 0;
+  if (g.a.kmajor || g.b.kmajor || fp8_split_plan(g).use || !transpose_first(g.M, g.N, g.K, 148)) return 0;
   return std::min(g.M, g.N) * round16(g.K);
 }
 
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s) {
+  const Fp8SplitPlan plan = fp8_split_plan(g);
+  if (plan.use) return launch_fp8_split(g, plan, s);
   GemmK k;
   k.a = g.a;
   k.b = g.b;
@@ -711,8 +678,8 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.out = static_cast<char*>(g.out);
   k.wait_limit_ns = g.wait_limit_ns;
   k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
-  k.a_words = scale_words(k.a);
-  k.b_words = scale_words(k.b);
+  k.a_words = fp8_scale_words(k.a);
+  k.b_words = fp8_scale_words(k.b);
   k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
   switch (g.out_type) {
     case F64E_F32: return launch_out<F64E_F32>(k, trans, g.K, g.sms, s);
@@ -723,9 +690,13 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
 
 cudaError_t read_fp8_status(int* status, cudaStream_t s) {
   static const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_fp8_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  int split = 0;
+  cudaError_t e = read_fp8_split_status(&split, s);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(status, g_fp8_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
   if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_fp8_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
-  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && !*status) *status = split;
+  return e;
 }
 
 }  // namespace f64e

@@ -1,0 +1,500 @@
+// Products of block-scaled 8-bit codes with few rows or columns: a served
+// layer on a handful of tokens, a small batch.
+//
+// A CTA computes 128 rows of the large ("wide") operand by all columns of the
+// small ("thin") one, up to 256, and a cluster of up to eight CTAs shares the
+// tile's K, so that a product with few tiles still draws on most SMs: bound by
+// reading the wide operand, it needs their copies in flight (10 stages of 16
+// KB each), not their tensor cores.  The partial sums meet in shared memory:
+// every CTA adds a share of the tile, in the order of the K ranges, so results
+// do not depend on timing and no scratch or second launch is needed.
+//
+// With x in 16 or 32 bits (a served layer on up to kFusedRows tokens), the
+// CTAs quantise the blocks of x they contract themselves: row blocks are 128
+// values of k, so a block is quantised within one step of the K loop.
+//   warp 0       TMA: 128 x 128 boxes of the wide operand (and the thin one's)
+//   warp 1       TMEM owner, scale copies and MMAs (tcgen05, cta_group::1)
+//   warps 2, 3   scales of the wide and the thin operand, four blocks of k a
+//                gather
+//   warps 4..7   quantisation of x; epilogue
+// Every wait is bounded; one that runs out records its site, and the CTA goes
+// on to the cluster barriers without storing.
+#include <algorithm>
+#include <map>
+#include <mutex>
+
+#include "f64e_fp8.cuh"
+#include "f64e_fp8.h"
+
+namespace f64e {
+
+// First wait that ran out in one of these kernels on this device, 0 if none.
+__device__ int g_fp8_split_status;
+
+namespace {
+
+constexpr int kThreads = 256, kBlock = kFp8Block, kRows = 128;
+constexpr int kMaxStages = 10, kMaxSplit = 8, kGroup = 4;
+constexpr uint32_t kWideBytes = kRows * kBlock, kAtom = 512;
+constexpr uint32_t kRing = 190 * 1024;   // shared memory for stages
+// More than half an SM's shared memory: no two kernels of this library that
+// hold TMEM share an SM.  A CTA that waited for TMEM held by a CTA of another
+// cluster, which waits at its cluster barrier for a CTA that waits in turn,
+// would wait for good.
+constexpr size_t kMinSmem = 120 * 1024;
+constexpr int kChunkBlocks = 16;         // blocks of k per accumulator, 32-bit outputs
+
+struct SplitArgs {
+  Fp8Operand w, x;      // wide, thin (fused: x's codes and scales unused)
+  int rows, cols;       // extents of the wide and the thin operand
+  int nkb;              // blocks of k
+  int bn, nst, split;   // columns of a tile, stages, CTAs per tile
+  int tiles_r;          // tiles along the wide operand
+  int nacc;             // accumulators (their sums are added at the end)
+  uint32_t tmem_cols, idesc;
+  int w_words, x_words;
+  char* out;
+  int64_t out_r, out_c;   // output strides (elements) along rows and columns
+  int vec;                // four rows of a column may be stored at once
+  const void* xf;         // fused: x [cols][ldx]
+  int64_t ldx, K;
+  int x_vec, x_wide;
+  uint32_t ring;          // bytes of shared memory before the scales: stages, then partial sums
+  uint64_t wait_limit_ns;
+};
+
+__device__ __forceinline__ void named_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ void named_arrive(int id, int threads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+// XT: type of x when the kernel quantises it, -1 for codes.
+template <int OUT, int XT>
+__global__ void __launch_bounds__(kThreads, 1)
+    fp8_split_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ CUtensorMap tmapX,
+                     const __grid_constant__ SplitArgs g) {
+  constexpr bool FUSED = XT >= 0;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_s = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
+  const uint32_t thin_bytes = g.bn * kBlock, stage_bytes = kWideBytes + thin_bytes;
+  const int atoms = g.bn > 128 ? 3 : 2;   // scale atoms of a stage: wide, thin (128 rows each)
+  uint8_t* sSF = smem + g.ring;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + g.nst * atoms * kAtom);
+  uint64_t* empty = full + kMaxStages;
+  uint64_t* sf_full = empty + kMaxStages;
+  uint64_t* acc_full = sf_full + kMaxStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)(blockIdx.x % g.split), tile = (int)(blockIdx.x / g.split);
+  const int r0 = (tile % g.tiles_r) * kRows, c0 = (tile / g.tiles_r) * g.bn;
+  const int kb0 = (int)((int64_t)g.nkb * rank / g.split), kb1 = (int)((int64_t)g.nkb * (rank + 1) / g.split);
+  const int cols = min(g.bn, g.cols - c0);
+  const int per = (kb1 - kb0 + g.nacc - 1) / g.nacc;   // blocks per accumulator
+  const uint64_t lim = g.wait_limit_ns;
+  int* status = &g_fp8_split_status;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < g.nst; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&sf_full[s], FUSED ? 5 : 2);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int i = 0;
+      for (int kb = kb0; kb < kb1; kb++, i++) {
+        const int s = i % g.nst;
+        if (i >= g.nst &&
+            (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitEmpty) || *abort_flag)) {
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* st = smem + s * stage_bytes;
+        const int k = kb * kBlock;
+        mbar_arrive_expect_tx(&full[s], FUSED ? kWideBytes : stage_bytes);
+        tma_load_2d(st, &tmapW, g.w.kmajor ? k : r0, g.w.kmajor ? r0 : k, &full[s]);
+        if (!FUSED) tma_load_2d(st + kWideBytes, &tmapX, k, c0, &full[s]);
+      }
+      // Every copy has landed before the CTA goes on (the MMAs waited for
+      // them too, unless a wait ran out).
+      for (int j = max(0, i - g.nst); j < i; j++)
+        mbar_wait_poll(&full[j % g.nst], (j / g.nst) & 1, drain_limit(lim), status, kWaitDrain);
+    }
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, g.tmem_cols);
+    tmem_relinquish();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+    named_arrive(1, 160);   // the epilogue's warps read the address behind it
+    const bool issuer = elect_one();
+    const uint32_t w_step = (g.w.kmajor ? 32 : 32 * kRows) >> 4;
+    const uint32_t sf_base = tmem + g.bn * g.nacc;
+    int s = 0, left = 0;
+    uint32_t ph = 0, d_tmem = tmem - g.bn, accumulate = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb++) {
+      if (left == 0) {
+        d_tmem += g.bn;
+        accumulate = 0;
+        left = per;
+      }
+      left--;
+      if (!mbar_wait_poll(&sf_full[s], ph, lim, status, kWaitScales) ||
+          !mbar_wait_poll(&full[s], ph, lim, status, kWaitFull)) {
+        ok = false;
+        break;
+      }
+      if (issuer) {
+        const uint32_t st = smem_u32(smem + s * stage_bytes), sf = smem_u32(sSF + s * atoms * kAtom);
+        const uint32_t sfa = sf_base + s * (4 * atoms), id = g.idesc | idesc_scale_byte(kb & 3);
+        copy_scales(sfa, smem_desc_scales(sf));
+        copy_scales(sfa + 4, smem_desc_scales(sf + kAtom));
+        if (atoms > 2) copy_scales(sfa + 8, smem_desc_scales(sf + 2 * kAtom));
+        const uint64_t dw = smem_desc_sw128(st), dx = smem_desc_sw128(st + kWideBytes);
+        mma_mx(d_tmem, dw, dx, id, sfa, sfa + 4, accumulate);
+#pragma unroll
+        for (int kk = 1; kk < kBlock / 32; kk++) mma_mx(d_tmem, dw + kk * w_step, dx + kk * 2, id, sfa, sfa + 4, 1);
+        tc_commit(&empty[s]);
+      }
+      __syncwarp();
+      accumulate = 1;
+      if (++s == g.nst) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    if (!ok) *abort_flag = 1;
+    if (issuer) {
+      tc_commit(acc_full);   // every MMA issued has completed when it arrives
+      mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitDrain);
+    }
+  } else if (warp == 2 || (warp == 3 && !FUSED)) {
+    // Scale words for four blocks of k at a time, written to every stage that
+    // uses them.
+    int i = 0;
+    bool ok = true;
+    uint4 atom[2] = {};
+    for (int kb = kb0; kb < kb1 && ok; kb++, i++) {
+      if (i == 0 || (kb & 3) == 0) {
+        if (warp == 2)
+          scale_atoms<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, g.w_words, atom);
+        else if (atoms > 2)
+          scale_atoms<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+        else
+          scale_atoms<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+      }
+      const int s = i % g.nst;
+      if (i >= g.nst &&
+          (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
+        *abort_flag = 1;
+        ok = false;
+        break;
+      }
+      uint8_t* dst = sSF + s * atoms * kAtom + (warp == 2 ? 0 : kAtom) + lane * 16;
+      *reinterpret_cast<uint4*>(dst) = atom[0];
+      if (warp == 3 && atoms > 2) *reinterpret_cast<uint4*>(dst + kAtom) = atom[1];
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sf_full[s]);
+    }
+  } else if (warp >= 4) {
+    if constexpr (FUSED) {
+      // Warp v quantises rows v, v + 4, .. of eight-lane groups: rows 4 v + 16 p
+      // + lane / 8, a block of 128 values a row; the blocks of a group of four
+      // are loaded together.
+      constexpr int PASSES = kFusedRows / 16;
+      const int l = lane & 7;
+      const typename Elem<XT>::type* x = static_cast<const typename Elem<XT>::type*>(g.xf);
+      int i = 0;
+      bool ok = true;
+      for (int kg = kb0; kg < kb1 && ok; kg += kGroup) {
+        uint32_t v[PASSES][kGroup][Elem<XT>::kWords];
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+          const int t = p * 16 + (warp - 4) * 4 + (lane >> 3);
+          if (p * 16 >= cols) break;
+#pragma unroll
+          for (int b = 0; b < kGroup; b++) {
+            const int64_t k = (int64_t)(kg + b) * kBlock + l * 16;
+            const typename Elem<XT>::type* p_x = x + (int64_t)(c0 + t) * g.ldx + k;
+            const int64_t n = t < cols && kg + b < kb1 ? g.K - k : 0;
+            if (g.x_vec && n >= 16)
+              load16<XT>(p_x, g.x_wide, v[p][b]);
+            else
+              load16_some<XT>(p_x, 1, n, v[p][b]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kGroup; b++) {
+          const int kb = kg + b;
+          if (kb >= kb1) break;
+          const int s = i % g.nst;
+          if (i >= g.nst &&
+              (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + s * stage_bytes + kWideBytes;
+          uint8_t* sf = sSF + s * atoms * kAtom + kAtom;
+#pragma unroll
+          for (int p = 0; p < PASSES; p++) {
+            const int t = p * 16 + (warp - 4) * 4 + (lane >> 3);
+            if (p * 16 >= cols) break;
+            float m = max16<XT>(v[p][b]);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            if (__any_sync(0xFFFFFFFFu, is_inf(m))) {
+              infs_to_nan<XT>(v[p][b]);
+              m = max16<XT>(v[p][b]);
+#pragma unroll
+              for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+            }
+            const int e = scale_exponent<F64E_E4M3>(m);
+            const float r = inverse_scale(e);
+            uint32_t c[8];
+            codes16<XT, F64E_E4M3>(v[p][b], [&](int) { return r; }, c);
+            *reinterpret_cast<uint4*>(st + t * kBlock + ((l ^ (t & 7)) << 4)) = row_of_codes(c);
+            if (l == 0) sf[(t & 31) * 16 + (t >> 5) * 4 + (kb & 3)] = (uint8_t)(e + 127);
+          }
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sf_full[s]);
+          i++;
+        }
+      }
+    }
+    // Partial sums to shared memory, [column][128 rows]; the stages are free:
+    // every MMA has completed.
+    const bool done = mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag;
+    named_sync(1, 160);
+    if (done) {
+      tc_fence_after();
+      const int q = warp & 3;
+      const uint32_t taddr = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(q * 32) << 16);
+      float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+      for (int c = 0; c < cols; c += 16) {
+        float sum[16];
+        for (int a = 0; a * per < kb1 - kb0; a++) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(taddr + a * g.bn + c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; k++) sum[k] = a == 0 ? __uint_as_float(v[k]) : sum[k] + __uint_as_float(v[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; k++) part[(c + k) * kRows] = sum[k];
+      }
+      tc_fence_before();
+    }
+  }
+
+  __syncwarp();
+  if (g.split > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(tmem_slot), g.tmem_cols);
+  }
+  // This CTA's share of the tile: four rows of a column a thread.
+  const int items = cols * (kRows / 4);
+  const int i0 = (int)((int64_t)items * rank / g.split), i1 = (int)((int64_t)items * (rank + 1) / g.split);
+  if (!*abort_flag) {
+    const uint32_t base = smem_u32(smem);
+    for (int i = i0 + (int)threadIdx.x; i < i1; i += kThreads) {
+      float4 v = *reinterpret_cast<const float4*>(smem + i * 16);
+      if (g.split > 1) {
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p = 0; p < g.split; p++) {
+          const float4 u = ld_cluster_f4(mapa_shared(base + i * 16, p));
+          v.x += u.x;
+          v.y += u.y;
+          v.z += u.z;
+          v.w += u.w;
+        }
+      }
+      const int c = c0 + i / (kRows / 4), r = r0 + i % (kRows / 4) * 4;
+      typename Elem<OUT>::type* o =
+          reinterpret_cast<typename Elem<OUT>::type*>(g.out) + (int64_t)r * g.out_r + (int64_t)c * g.out_c;
+      const float f[4] = {v.x, v.y, v.z, v.w};
+      if (g.vec && r + 4 <= g.rows) {
+        if (OUT == F64E_F32)
+          *reinterpret_cast<float4*>(o) = v;
+        else
+          *reinterpret_cast<uint2*>(o) = make_uint2(Elem<OUT>::pack(v.x, v.y), Elem<OUT>::pack(v.z, v.w));
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (r + k < g.rows) {
+            if (OUT == F64E_F32)
+              reinterpret_cast<uint32_t*>(o)[k * g.out_r] = Elem<OUT>::bits(f[k]);
+            else
+              reinterpret_cast<uint16_t*>(o)[k * g.out_r] = (uint16_t)Elem<OUT>::bits(f[k]);
+          }
+      }
+    }
+  }
+  if (g.split > 1) cluster_sync();   // the peers have read this CTA's sums
+}
+
+template <int OUT, int XT>
+cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const SplitArgs& k, int tiles, size_t smem,
+                          cudaStream_t s) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  {
+    // the shared-memory opt-in is a per-device attribute of the kernel
+    static std::mutex mtx;
+    static std::map<int, bool> done;
+    std::lock_guard<std::mutex> lk(mtx);
+    if (!done[dev]) {
+      e = cudaFuncSetAttribute(fp8_split_kernel<OUT, XT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+      if (e != cudaSuccess) return e;
+      done[dev] = true;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = k.split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(tiles * k.split), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fp8_split_kernel<OUT, XT>, tw, tx, k);
+}
+
+// The plan's numbers for wide rows by thin columns.
+cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Fp8SplitPlan& p, cudaStream_t s) {
+  CUtensorMap tw, tx = {};
+  if (!fp8_encode_codes(&tw, k.w, k.rows, K, kRows) ||
+      (x_type < 0 && !fp8_encode_codes(&tx, k.x, k.cols, K, p.cols)))
+    return cudaErrorInvalidValue;
+  k.nkb = (int)((K + kBlock - 1) / kBlock);
+  k.K = K;
+  k.bn = p.cols;
+  k.split = p.split;
+  k.tiles_r = (k.rows + kRows - 1) / kRows;
+  const int per_cta = (k.nkb + k.split - 1) / k.split;
+  const int atoms = k.bn > 128 ? 3 : 2;
+  const size_t stage = kWideBytes + (size_t)k.bn * kBlock;
+  k.nst = (int)std::min<int64_t>({kMaxStages, per_cta, (int64_t)(kRing / (stage + atoms * kAtom))});
+  // 32-bit outputs: a new accumulator every kChunkBlocks, as far as TMEM goes
+  const int sf_cols = k.nst * 4 * atoms;
+  k.nacc = out_type == F64E_F32
+               ? std::max(1, std::min((per_cta + kChunkBlocks - 1) / kChunkBlocks, (512 - sf_cols) / k.bn))
+               : 1;
+  k.tmem_cols = 32;
+  while ((int)k.tmem_cols < k.bn * k.nacc + sf_cols) k.tmem_cols *= 2;
+  k.idesc = idesc_mx(kRows, k.bn, k.w.code, k.x.code, !k.w.kmajor, 0);
+  k.w_words = fp8_scale_words(k.w);
+  k.x_words = x_type < 0 && fp8_scale_words(k.x);
+  const int es = out_type == F64E_F32 ? 4 : 2;
+  k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
+  k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kRows * 4);
+  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * atoms * kAtom + (3 * kMaxStages + 1) * 8 + 16);
+  const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
+  if (x_type >= 0) {
+    switch (x_type) {
+      case F64E_F32: return launch_kernel<F64E_F32, F64E_F32>(tw, tx, k, tiles, smem, s);
+      case F64E_F16: return launch_kernel<F64E_F16, F64E_F16>(tw, tx, k, tiles, smem, s);
+      default: return launch_kernel<F64E_BF16, F64E_BF16>(tw, tx, k, tiles, smem, s);
+    }
+  }
+  switch (out_type) {
+    case F64E_F32: return launch_kernel<F64E_F32, -1>(tw, tx, k, tiles, smem, s);
+    case F64E_F16: return launch_kernel<F64E_F16, -1>(tw, tx, k, tiles, smem, s);
+    default: return launch_kernel<F64E_BF16, -1>(tw, tx, k, tiles, smem, s);
+  }
+}
+
+int split_of(int64_t tiles, int64_t nkb, int sms) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplit, nkb, sms / std::max<int64_t>(tiles, 1)}));
+}
+
+}  // namespace
+
+Fp8SplitPlan fp8_split_plan(const Fp8GemmArgs& g) {
+  Fp8SplitPlan p = {};
+  const int64_t thin = std::min(g.M, g.N), wide = std::max(g.M, g.N), nkb = (g.K + kBlock - 1) / kBlock;
+  const Fp8Operand& t = g.M <= g.N ? g.a : g.b;
+  const int64_t tc = (thin + 255) / 256;
+  p.cols = (int)(((thin + tc - 1) / tc + 15) / 16 * 16);
+  const int64_t tiles = (wide + kRows - 1) / kRows * tc;
+  p.split = split_of(tiles, nkb, g.sms);
+  p.use = t.kmajor && thin <= 256;
+  return p;
+}
+
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, const Fp8SplitPlan& p, cudaStream_t s) {
+  SplitArgs k = {};
+  const bool a_thin = g.M <= g.N;
+  k.w = a_thin ? g.b : g.a;
+  k.x = a_thin ? g.a : g.b;
+  k.rows = (int)(a_thin ? g.N : g.M);
+  k.cols = (int)(a_thin ? g.M : g.N);
+  k.out = static_cast<char*>(g.out);
+  k.out_r = a_thin ? 1 : g.ldo;
+  k.out_c = a_thin ? g.ldo : 1;
+  k.wait_limit_ns = g.wait_limit_ns;
+  return launch(k, g.out_type, -1, g.K, p, s);
+}
+
+cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
+  const Fp8GemmArgs& g = a.g;
+  SplitArgs k = {};
+  k.w = g.b;
+  k.x.code = F64E_E4M3;
+  k.x.kmajor = 1;
+  k.rows = (int)g.N;
+  k.cols = (int)g.M;
+  k.out = static_cast<char*>(g.out);
+  k.out_r = 1;
+  k.out_c = g.ldo;
+  k.xf = a.x;
+  k.ldx = a.ldx;
+  const int64_t pitch = a.ldx * (a.x_type == F64E_F32 ? 4 : 2);
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.x);
+  k.x_vec = x % 16 == 0 && (pitch % 16 == 0 || g.M == 1);
+  k.x_wide = x % 32 == 0 && (pitch % 32 == 0 || g.M == 1);
+  k.wait_limit_ns = g.wait_limit_ns;
+  Fp8SplitPlan p = {};
+  p.cols = (int)((g.M + 15) / 16 * 16);
+  p.split = split_of((g.N + kRows - 1) / kRows, (g.K + kBlock - 1) / kBlock, g.sms);
+  return launch(k, a.x_type, a.x_type, g.K, p, s);
+}
+
+cudaError_t read_fp8_split_status(int* status, cudaStream_t s) {
+  static const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_fp8_split_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess)
+    e = cudaMemcpyToSymbolAsync(g_fp8_split_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+}
+
+}  // namespace f64e

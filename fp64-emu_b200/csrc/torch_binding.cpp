@@ -550,15 +550,29 @@ std::vector<int64_t> fp8_out_sizes(const at::Tensor& x, int64_t n) {
 
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
   fp8_check_linear(x, w, ws);
-  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
-  at::Tensor q, s, wq = w, wsc;
-  std::tie(q, s) = fp8_quantize(x2, F64E_BLOCKS_ROW, at::kFloat8_e4m3fn);
-  if (ws.has_value())
+  const c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor xr = fp8_rows(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}));
+  at::Tensor wq, wsc;
+  if (ws.has_value()) {
+    wq = w;
     wsc = *ws;
-  else
+  } else {
     std::tie(wq, wsc) = fp8_quantize(w, F64E_BLOCKS_TILE, at::kFloat8_e4m3fn);
-  at::Tensor y = fp8_mm(q, wq, s, wsc, kFp8NT, x.scalar_type());
-  return x.dim() == 2 ? y : y.view(fp8_out_sizes(x, w.size(0)));
+  }
+  const Fp8Held hw = fp8_hold(wq, wsc, 1);
+  f64e_fp8_problem p{};
+  p.M = xr.size(0);
+  p.N = w.size(0);
+  p.K = w.size(1);
+  p.out_type = fp8_type(x.scalar_type());
+  p.ldo = p.N;
+  p.b = hw.o;
+  const size_t nb = f64e_fp8_linear_workspace_size(p.M, p.K);
+  const at::Tensor work = nb ? at::empty({(int64_t)nb}, x.options().dtype(at::kByte)) : at::Tensor();
+  at::Tensor y = at::empty(fp8_out_sizes(x, p.N), x.options());
+  check(f64e_fp8_linear(&p, xr.data_ptr(), fp8_pitch(xr), hw.q.data_ptr(), wsc.data_ptr(), y.data_ptr(),
+                        nb ? work.data_ptr() : nullptr, nb, stream_of()));
+  return y;
 }
 
 // The same with gradients.  What the backward pass needs of x is kept in 8

@@ -296,6 +296,15 @@ F64E_API size_t f64e_fp8_workspace_size(const f64e_fp8_problem* p);
 F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B,
                            const void* b_scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* out [M, N] = x [M, K] @ w^T, a layer on M rows: x (row pitch ldx, of the
+ * type p->out_type) is quantised to e4m3 in row blocks, w is the operand p->b;
+ * p->a is not read.  Up to 32 rows are quantised by the product itself, in one
+ * launch; more need a workspace (256-byte aligned device memory of
+ * f64e_fp8_linear_workspace_size() bytes) for their codes. */
+F64E_API size_t f64e_fp8_linear_workspace_size(int64_t M, int64_t K);
+F64E_API int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const void* w,
+                             const void* w_scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Status of the 8-bit products on the current device: 0, or the site code of
  * the first bounded wait that ran out since the last read (the product's
  * output is then not valid).  The codes of f64e_status, plus 6 and 7 (waits
