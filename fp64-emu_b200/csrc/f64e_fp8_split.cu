@@ -16,7 +16,7 @@
 //   warp 1       TMEM owner, scale copies and MMAs (tcgen05, cta_group::1)
 //   warps 2, 3   scales of the wide and the thin operand, four blocks of k a
 //                gather
-//   warps 4..7   quantisation of x; epilogue
+//   warps 4..    quantisation of x (eight warps); epilogue (four)
 // Every wait is bounded; one that runs out records its site, and the CTA goes
 // on to the cluster barriers without storing.
 #include <algorithm>
@@ -33,8 +33,8 @@ __device__ int g_fp8_split_status;
 
 namespace {
 
-constexpr int kThreads = 256, kBlock = kFp8Block, kRows = 128;
-constexpr int kMaxStages = 10, kMaxSplit = 8, kGroup = 4;
+constexpr int kBlock = kFp8Block, kRows = 128;
+constexpr int kMaxStages = 10, kMaxSplit = 8;
 constexpr uint32_t kWideBytes = kRows * kBlock, kAtom = 512;
 constexpr uint32_t kRing = 190 * 1024;   // shared memory for stages
 // More than half an SM's shared memory: no two kernels of this library that
@@ -63,12 +63,6 @@ struct SplitArgs {
   uint64_t wait_limit_ns;
 };
 
-__device__ __forceinline__ void named_sync(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-__device__ __forceinline__ void named_arrive(int id, int threads) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
@@ -78,9 +72,14 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
+// Warps that quantise x (the epilogue's four among them); twice the registers
+// a row, in 32 bits, leave room for half as many.
+template <int XT>
+constexpr int kQuantWarps = XT == F64E_F16 || XT == F64E_BF16 ? 8 : 4;
+
 // XT: type of x when the kernel quantises it, -1 for codes.
 template <int OUT, int XT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     fp8_split_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ CUtensorMap tmapX,
                      const __grid_constant__ SplitArgs g) {
   constexpr bool FUSED = XT >= 0;
@@ -106,33 +105,90 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint64_t lim = g.wait_limit_ns;
   int* status = &g_fp8_split_status;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < g.nst; s++) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-      mbar_init(&sf_full[s], FUSED ? 5 : 2);
+  // Before the CTA meets: the copies that need no free stage, the first scales
+  // and the first blocks of x are on their way, and TMEM is allocated.
+  const int n = kb1 - kb0, head = min(n, g.nst);
+  auto load = [&](int i) {
+    const int s = i % g.nst, k = (kb0 + i) * kBlock;
+    uint8_t* st = smem + s * stage_bytes;
+    mbar_arrive_expect_tx(&full[s], FUSED ? kWideBytes : stage_bytes);
+    tma_load_2d(st, &tmapW, g.w.kmajor ? k : r0, g.w.kmajor ? r0 : k, &full[s]);
+    if (!FUSED) tma_load_2d(st + kWideBytes, &tmapX, k, c0, &full[s]);
+  };
+  uint4 atom[2] = {};
+  auto gather = [&](int kb) {
+    if (warp == 2)
+      scale_atoms<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, g.w_words, atom);
+    else if (atoms > 2)
+      scale_atoms<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+    else
+      scale_atoms<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+  };
+  // Blocks of x in registers: warp 4 + b takes every QW-th block of k, from
+  // the b-th on, of all rows: rows 4 p + lane / 8, eight lanes a block.
+  constexpr int QW = kQuantWarps<XT>;
+  constexpr int PASSES = kFusedRows / 4;
+  using EX = Elem<FUSED ? XT : F64E_BF16>;
+  const int l = lane & 7;
+  uint32_t v[PASSES][EX::kWords];
+  auto load_x = [&](int i) {
+    if constexpr (FUSED) {
+      const int64_t k = (int64_t)(kb0 + i) * kBlock + l * 16;
+      const typename EX::type* x = static_cast<const typename EX::type*>(g.xf) + (int64_t)(c0 + (lane >> 3)) * g.ldx + k;
+      const bool whole = g.x_vec && (int64_t)(kb0 + i + 1) * kBlock <= g.K;
+#pragma unroll
+      for (int p = 0; p < PASSES; p++) {
+        if (p * 4 >= cols) break;
+        const bool row = p * 4 + (lane >> 3) < cols;
+        if (whole) {
+          if (row) load16<XT>(x + p * 4 * g.ldx, g.x_wide, v[p]);
+        } else {
+          load16_some<XT>(x + p * 4 * g.ldx, 1, row ? g.K - k : 0, v[p]);
+        }
+      }
     }
-    mbar_init(acc_full, 1);
-    *abort_flag = 0;
-    fence_barrier_init();
+  };
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int s = 0; s < g.nst; s++) mbar_init(&full[s], 1);
+      fence_barrier_init();
+      for (int i = 0; i < head; i++) load(i);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      for (int s = 0; s < g.nst; s++) mbar_init(&empty[s], 1);
+      mbar_init(acc_full, 1);
+      *abort_flag = 0;
+      fence_barrier_init();
+    }
+    __syncwarp();
+    tmem_alloc(tmem_slot, g.tmem_cols);
+    tmem_relinquish();
+    tc_fence_before();
+  } else if (warp < 4) {
+    if (warp == 2 && lane == 0) {
+      for (int s = 0; s < g.nst; s++) mbar_init(&sf_full[s], 2);
+      fence_barrier_init();
+    }
+    if (warp == 2 || !FUSED) gather(kb0);
+  } else if (warp - 4 < n) {
+    load_x(warp - 4);
   }
+  __syncwarp();
   __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   if (warp == 0) {
     if (elect_one()) {
-      int i = 0;
-      for (int kb = kb0; kb < kb1; kb++, i++) {
+      int i = head;
+      for (; i < n; i++) {
         const int s = i % g.nst;
-        if (i >= g.nst &&
-            (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitEmpty) || *abort_flag)) {
+        if (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitEmpty) || *abort_flag) {
           *abort_flag = 1;
           break;
         }
-        uint8_t* st = smem + s * stage_bytes;
-        const int k = kb * kBlock;
-        mbar_arrive_expect_tx(&full[s], FUSED ? kWideBytes : stage_bytes);
-        tma_load_2d(st, &tmapW, g.w.kmajor ? k : r0, g.w.kmajor ? r0 : k, &full[s]);
-        if (!FUSED) tma_load_2d(st + kWideBytes, &tmapX, k, c0, &full[s]);
+        load(i);
       }
       // Every copy has landed before the CTA goes on (the MMAs waited for
       // them too, unless a wait ran out).
@@ -140,10 +196,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait_poll(&full[j % g.nst], (j / g.nst) & 1, drain_limit(lim), status, kWaitDrain);
     }
   } else if (warp == 1) {
-    tmem_alloc(tmem_slot, g.tmem_cols);
-    tmem_relinquish();
-    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
-    named_arrive(1, 160);   // the epilogue's warps read the address behind it
     const bool issuer = elect_one();
     const uint32_t w_step = (g.w.kmajor ? 32 : 32 * kRows) >> 4;
     const uint32_t sf_base = tmem + g.bn * g.nacc;
@@ -189,23 +241,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 2 || (warp == 3 && !FUSED)) {
     // Scale words for four blocks of k at a time, written to every stage that
     // uses them.
-    int i = 0;
-    bool ok = true;
-    uint4 atom[2] = {};
-    for (int kb = kb0; kb < kb1 && ok; kb++, i++) {
-      if (i == 0 || (kb & 3) == 0) {
-        if (warp == 2)
-          scale_atoms<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, g.w_words, atom);
-        else if (atoms > 2)
-          scale_atoms<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
-        else
-          scale_atoms<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
-      }
+    for (int i = 0; i < n; i++) {
+      if (i > 0 && ((kb0 + i) & 3) == 0) gather(kb0 + i);
       const int s = i % g.nst;
       if (i >= g.nst &&
           (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
         *abort_flag = 1;
-        ok = false;
         break;
       }
       uint8_t* dst = sSF + s * atoms * kAtom + (warp == 2 ? 0 : kAtom) + lane * 16;
@@ -217,79 +258,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 4) {
     if constexpr (FUSED) {
-      // Warp v quantises rows v, v + 4, .. of eight-lane groups: rows 4 v + 16 p
-      // + lane / 8, a block of 128 values a row; the blocks of a group of four
-      // are loaded together.
-      constexpr int PASSES = kFusedRows / 16;
-      const int l = lane & 7;
-      const typename Elem<XT>::type* x = static_cast<const typename Elem<XT>::type*>(g.xf);
-      int i = 0;
-      bool ok = true;
-      for (int kg = kb0; kg < kb1 && ok; kg += kGroup) {
-        uint32_t v[PASSES][kGroup][Elem<XT>::kWords];
+      // One warp a block: a lone warp issues an instruction every few cycles,
+      // so warps that each took a quarter of every block's rows, with all
+      // the arithmetic of a scale for each, set the kernel's pace on few rows
+      // (8192^2, one row: 1450 cycles a block of k, copies 800).
+      for (int i = warp - 4; i < n; i += QW) {
+        uint4 code[PASSES];
+        uint8_t scale[PASSES];
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
-          const int t = p * 16 + (warp - 4) * 4 + (lane >> 3);
-          if (p * 16 >= cols) break;
+          if (p * 4 >= cols) break;
+          float m = max16<XT>(v[p]);
 #pragma unroll
-          for (int b = 0; b < kGroup; b++) {
-            const int64_t k = (int64_t)(kg + b) * kBlock + l * 16;
-            const typename Elem<XT>::type* p_x = x + (int64_t)(c0 + t) * g.ldx + k;
-            const int64_t n = t < cols && kg + b < kb1 ? g.K - k : 0;
-            if (g.x_vec && n >= 16)
-              load16<XT>(p_x, g.x_wide, v[p][b]);
-            else
-              load16_some<XT>(p_x, 1, n, v[p][b]);
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < kGroup; b++) {
-          const int kb = kg + b;
-          if (kb >= kb1) break;
-          const int s = i % g.nst;
-          if (i >= g.nst &&
-              (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* st = smem + s * stage_bytes + kWideBytes;
-          uint8_t* sf = sSF + s * atoms * kAtom + kAtom;
-#pragma unroll
-          for (int p = 0; p < PASSES; p++) {
-            const int t = p * 16 + (warp - 4) * 4 + (lane >> 3);
-            if (p * 16 >= cols) break;
-            float m = max16<XT>(v[p][b]);
+          for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+          if (__any_sync(0xFFFFFFFFu, is_inf(m))) {
+            infs_to_nan<XT>(v[p]);
+            m = max16<XT>(v[p]);
 #pragma unroll
             for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            if (__any_sync(0xFFFFFFFFu, is_inf(m))) {
-              infs_to_nan<XT>(v[p][b]);
-              m = max16<XT>(v[p][b]);
-#pragma unroll
-              for (int o = 4; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            }
-            const int e = scale_exponent<F64E_E4M3>(m);
-            const float r = inverse_scale(e);
-            uint32_t c[8];
-            codes16<XT, F64E_E4M3>(v[p][b], [&](int) { return r; }, c);
-            *reinterpret_cast<uint4*>(st + t * kBlock + ((l ^ (t & 7)) << 4)) = row_of_codes(c);
-            if (l == 0) sf[(t & 31) * 16 + (t >> 5) * 4 + (kb & 3)] = (uint8_t)(e + 127);
           }
-          fence_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sf_full[s]);
-          i++;
+          const int e = scale_exponent<F64E_E4M3>(m);
+          const float r = inverse_scale(e);
+          uint32_t c[8];
+          codes16<XT, F64E_E4M3>(v[p], [&](int) { return r; }, c);
+          code[p] = row_of_codes(c);
+          scale[p] = (uint8_t)(e + 127);
         }
+        if (i + QW < n) load_x(i + QW);
+        const int s = i % g.nst;
+        if (i >= g.nst &&
+            (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
+          *abort_flag = 1;
+          break;
+        }
+        uint8_t* st = smem + s * stage_bytes + kWideBytes;
+        uint8_t* sf = sSF + s * atoms * kAtom + kAtom + ((kb0 + i) & 3);
+#pragma unroll
+        for (int p = 0; p < PASSES; p++) {
+          if (p * 4 >= cols) break;
+          const int t = p * 4 + (lane >> 3);
+          *reinterpret_cast<uint4*>(st + t * kBlock + ((l ^ (t & 7)) << 4)) = code[p];
+          if (l == 0) sf[t * 16] = scale[p];
+        }
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sf_full[s]);
       }
     }
     // Partial sums to shared memory, [column][128 rows]; the stages are free:
     // every MMA has completed.
-    const bool done = mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag;
-    named_sync(1, 160);
+    const bool done = warp < 8 && mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag;
     if (done) {
       tc_fence_after();
       const int q = warp & 3;
-      const uint32_t taddr = *reinterpret_cast<volatile uint32_t*>(tmem_slot) + ((uint32_t)(q * 32) << 16);
+      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
       float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
       for (int c = 0; c < cols; c += 16) {
         float sum[16];
@@ -314,14 +336,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(*reinterpret_cast<volatile uint32_t*>(tmem_slot), g.tmem_cols);
+    tmem_dealloc(tmem, g.tmem_cols);
   }
   // This CTA's share of the tile: four rows of a column a thread.
   const int items = cols * (kRows / 4);
   const int i0 = (int)((int64_t)items * rank / g.split), i1 = (int)((int64_t)items * (rank + 1) / g.split);
   if (!*abort_flag) {
     const uint32_t base = smem_u32(smem);
-    for (int i = i0 + (int)threadIdx.x; i < i1; i += kThreads) {
+    for (int i = i0 + (int)threadIdx.x; i < i1; i += 32 * (4 + QW)) {
       float4 v = *reinterpret_cast<const float4*>(smem + i * 16);
       if (g.split > 1) {
         v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -381,7 +403,7 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(tiles * k.split), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(32 * (4 + kQuantWarps<XT>), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
