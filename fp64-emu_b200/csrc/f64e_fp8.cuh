@@ -21,6 +21,14 @@
 
 namespace f64e {
 
+// --------------------------------------------------- overlapping launches --
+// These kernels are launched with programmatic stream serialization: a kernel
+// may be set up while the one before it in the stream drains.  It reads and
+// writes global memory only after launch_wait(), when that kernel has
+// completed; launch_next() lets the next one be set up.
+__device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ------------------------------------------------------------ scale bytes --
 // FMAX = 1.75 * 2^emax in both codes: e = p - emax for a largest magnitude
 // m * 2^p with m in [1, 1.75], one more above.  Subnormal magnitudes give

@@ -10,6 +10,28 @@
 
 namespace f64e {
 
+// Launch with programmatic stream serialization (launch_wait, launch_next in
+// f64e_fp8.cuh) and, where cluster > 0, in clusters.
+template <typename... P, typename... A>
+cudaError_t fp8_launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, unsigned cluster,
+                       cudaStream_t s, A... args) {
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 constexpr int kFp8Block = 128;  // values that share one scale
 
 // ---- quantisation (f64e_fp8_quant.cu) ----

@@ -251,6 +251,8 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   };
   __syncwarp();
   cluster_arrive_relaxed();
+  launch_next();
+  launch_wait();
   if (warp == 2 || warp == 3) gather(0);
   cluster_wait();
   const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
@@ -556,7 +558,6 @@ cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   cfg.gridDim = dim3(2 * (sms / 2), 1, 1);
   cfg.blockDim = dim3(PTHREADS, 1, 1);
   cfg.dynamicSmemBytes = PSMEM;
-  cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   // per device: the shared-memory opt-in and the resident cluster count
@@ -573,9 +574,9 @@ cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
     max_clusters = std::max(n, 1);
   }
   const int64_t tiles = (int64_t)((k.M + PBM - 1) / PBM) * ((k.N + BN - 1) / BN);
-  cfg.gridDim = dim3(2 * (unsigned)std::min<int64_t>(tiles, max_clusters), 1, 1);
+  const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, max_clusters);
   lk.unlock();
-  return cudaLaunchKernelEx(&cfg, fp8_gemm_pair_kernel<OUT, TRANS>, ta, tb, to, k);
+  return fp8_launch(fp8_gemm_pair_kernel<OUT, TRANS>, grid, PTHREADS, PSMEM, 2, s, ta, tb, to, k);
 }
 
 template <int OUT>
@@ -592,6 +593,8 @@ __global__ void __launch_bounds__(256) fp8_transpose_kernel(const uint8_t* q, in
   const int64_t r0 = (blockIdx.x % nrb) * 128, k0 = (blockIdx.x / nrb) * 128;
   const int rg = threadIdx.x & 31, kg0 = threadIdx.x >> 5;   // 4 rows by 4 k each
   uint32_t w[4][4];
+  launch_next();
+  launch_wait();
 #pragma unroll
   for (int u = 0; u < 4; u++)
 #pragma unroll
@@ -661,9 +664,8 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
     Fp8Operand& o = a_side ? k.a : k.b;
     const int64_t rows = a_side ? g.M : g.N, nrb = (rows + 127) / 128;
     uint8_t* t = static_cast<uint8_t*>(workspace);
-    fp8_transpose_kernel<<<(unsigned)(nrb * ((g.K + 127) / 128)), 256, 0, s>>>(o.q, o.ld, rows, g.K, t, round16(g.K),
-                                                                               nrb);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = fp8_launch(fp8_transpose_kernel, (unsigned)(nrb * ((g.K + 127) / 128)), 256, 0, 0, s, o.q, o.ld,
+                                     rows, g.K, t, round16(g.K), nrb);
     if (e != cudaSuccess) return e;
     o.q = t;
     o.ld = round16(g.K);

@@ -64,6 +64,8 @@ __global__ void __launch_bounds__(kThreads) fp8_quant_rows_kernel(const Fp8Quant
   uint8_t* q = a.q + row0 * a.ldq + col + l * 16;
   uint8_t* s = a.s + row0 * nkb + kb;
   uint32_t w[kRowPasses][Elem<T>::kWords];
+  launch_next();
+  launch_wait();
 #pragma unroll
   for (int u = 0; u < kRowPasses; u++)
     load_row<T, VEC>(x + u * a.ldx, l, row0 + u < a.rows ? a.cols - col : 0, wide, w[u]);
@@ -172,6 +174,8 @@ __global__ void __launch_bounds__(kThreads, T == F64E_F32 || MODE == kRowsCols ?
   const int64_t padded = (a.cols + 15) & ~(int64_t)15;
   const typename E::type* x = static_cast<const typename E::type*>(a.x) + (row0 + 4 * g) * a.ldx + col;
   uint32_t w[4][E::kWords];
+  launch_next();
+  launch_wait();
 #pragma unroll
   for (int u = 0; u < 4; u++)
     load_row<T, VEC>(x + u * a.ldx, l, row0 + 4 * g + u < a.rows ? a.cols - col : 0, wide, w[u]);
@@ -298,6 +302,8 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
   const int64_t n = a.cols - col;
   const uint8_t* q = a.q + (rb * kFp8Block + g) * a.ldq + col;
   uint32_t w[4][4];
+  launch_next();
+  launch_wait();
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
@@ -387,10 +393,8 @@ cudaError_t rows_of(const Fp8QuantArgs& a, cudaStream_t s) {
   const int64_t pitch = a.ldx * (int64_t)sizeof(typename Elem<T>::type);
   const bool wide = aligned(a.x, pitch, 32);
   if (aligned(a.x, pitch, 16))
-    fp8_quant_rows_kernel<T, CODE, true><<<grid, kThreads, 0, s>>>(a, nkb, ng, wide);
-  else
-    fp8_quant_rows_kernel<T, CODE, false><<<grid, kThreads, 0, s>>>(a, nkb, ng, wide);
-  return cudaGetLastError();
+    return fp8_launch(fp8_quant_rows_kernel<T, CODE, true>, grid, kThreads, 0, 0, s, a, nkb, ng, wide);
+  return fp8_launch(fp8_quant_rows_kernel<T, CODE, false>, grid, kThreads, 0, 0, s, a, nkb, ng, wide);
 }
 template <int T, int CODE, int MODE>
 cudaError_t squares_mode(const Fp8QuantArgs& a, cudaStream_t s) {
@@ -399,10 +403,8 @@ cudaError_t squares_mode(const Fp8QuantArgs& a, cudaStream_t s) {
   const int64_t pitch = a.ldx * (int64_t)sizeof(typename Elem<T>::type);
   const bool wide = aligned(a.x, pitch, 32);
   if (aligned(a.x, pitch, 16))
-    fp8_quant_squares_kernel<T, CODE, MODE, true><<<grid, kThreads, 0, s>>>(a, nkb, wide);
-  else
-    fp8_quant_squares_kernel<T, CODE, MODE, false><<<grid, kThreads, 0, s>>>(a, nkb, wide);
-  return cudaGetLastError();
+    return fp8_launch(fp8_quant_squares_kernel<T, CODE, MODE, true>, grid, kThreads, 0, 0, s, a, nkb, wide);
+  return fp8_launch(fp8_quant_squares_kernel<T, CODE, MODE, false>, grid, kThreads, 0, 0, s, a, nkb, wide);
 }
 template <int T, int CODE>
 cudaError_t squares_of(const Fp8QuantArgs& a, int tile, cudaStream_t s) {
@@ -417,10 +419,8 @@ cudaError_t dequant_of(const Fp8DequantArgs& a, cudaStream_t s) {
   const int64_t pitch = a.cols * (int64_t)sizeof(typename Elem<T>::type);
   const bool wide = aligned(a.out, pitch, 32);
   if (aligned(a.q, a.ldq, 16) && aligned(a.out, pitch, 16))
-    fp8_dequant_kernel<CODE, T, true><<<grid, kThreads, 0, s>>>(a, ncb, wide);
-  else
-    fp8_dequant_kernel<CODE, T, false><<<grid, kThreads, 0, s>>>(a, ncb, wide);
-  return cudaGetLastError();
+    return fp8_launch(fp8_dequant_kernel<CODE, T, true>, grid, kThreads, 0, 0, s, a, ncb, wide);
+  return fp8_launch(fp8_dequant_kernel<CODE, T, false>, grid, kThreads, 0, 0, s, a, ncb, wide);
 }
 
 }  // namespace

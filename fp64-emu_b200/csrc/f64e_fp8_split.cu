@@ -42,6 +42,9 @@ constexpr uint32_t kRing = 190 * 1024;   // shared memory for stages
 // cluster, which waits at its cluster barrier for a CTA that waits in turn,
 // would wait for good.
 constexpr size_t kMinSmem = 120 * 1024;
+// Floats from one column of partial sums to the next: four rows of eight
+// neighbouring columns lie in different banks.
+constexpr int kPitch = kRows + 4;
 constexpr int kChunkBlocks = 16;         // blocks of k per accumulator, 32-bit outputs
 
 struct SplitArgs {
@@ -148,10 +151,12 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       }
     }
   };
+  launch_next();
   if (warp == 0) {
     if (elect_one()) {
       for (int s = 0; s < g.nst; s++) mbar_init(&full[s], 1);
       fence_barrier_init();
+      launch_wait();
       for (int i = 0; i < head; i++) load(i);
     }
   } else if (warp == 1) {
@@ -170,10 +175,13 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       for (int s = 0; s < g.nst; s++) mbar_init(&sf_full[s], 2);
       fence_barrier_init();
     }
+    launch_wait();
     if (warp == 2 || !FUSED) gather(kb0);
-  } else if (warp - 4 < n) {
-    load_x(warp - 4);
+  } else {
+    launch_wait();
+    if (warp - 4 < n) load_x(warp - 4);
   }
+  launch_wait();
   __syncwarp();
   __syncthreads();
   tc_fence_after();
@@ -305,14 +313,14 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         if (lane == 0) mbar_arrive(&sf_full[s]);
       }
     }
-    // Partial sums to shared memory, [column][128 rows]; the stages are free:
+    // Partial sums to shared memory, by columns of 128 rows; the stages are free:
     // every MMA has completed.
     const bool done = warp < 8 && mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag;
     if (done) {
       tc_fence_after();
       const int q = warp & 3;
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-      float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;
+      float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;   // column pitch kPitch
       for (int c = 0; c < cols; c += 16) {
         float sum[16];
         for (int a = 0; a * per < kb1 - kb0; a++) {
@@ -323,7 +331,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
           for (int k = 0; k < 16; k++) sum[k] = a == 0 ? __uint_as_float(v[k]) : sum[k] + __uint_as_float(v[k]);
         }
 #pragma unroll
-        for (int k = 0; k < 16; k++) part[(c + k) * kRows] = sum[k];
+        for (int k = 0; k < 16; k++) part[(c + k) * kPitch] = sum[k];
       }
       tc_fence_before();
     }
@@ -338,41 +346,58 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     tc_fence_after();
     tmem_dealloc(tmem, g.tmem_cols);
   }
-  // This CTA's share of the tile: four rows of a column a thread.
+  // This CTA's share of the tile: four rows of a column a thread, neighbouring
+  // threads along the output's contiguous direction, four items in flight.
   const int items = cols * (kRows / 4);
   const int i0 = (int)((int64_t)items * rank / g.split), i1 = (int)((int64_t)items * (rank + 1) / g.split);
   if (!*abort_flag) {
+    constexpr int NT = 32 * (4 + QW), U = 4;
     const uint32_t base = smem_u32(smem);
-    for (int i = i0 + (int)threadIdx.x; i < i1; i += 32 * (4 + QW)) {
-      float4 v = *reinterpret_cast<const float4*>(smem + i * 16);
-      if (g.split > 1) {
-        v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p = 0; p < g.split; p++) {
-          const float4 u = ld_cluster_f4(mapa_shared(base + i * 16, p));
-          v.x += u.x;
-          v.y += u.y;
-          v.z += u.z;
-          v.w += u.w;
+    for (int i = i0 + (int)threadIdx.x; i < i1; i += NT * U) {
+      float4 v[U];
+      int c[U], r[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int j = min(i + u * NT, i1 - 1);
+        c[u] = g.out_c == 1 ? j % cols : j / (kRows / 4);
+        r[u] = (g.out_c == 1 ? j / cols : j % (kRows / 4)) * 4;
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      for (int p = 0; p < g.split; p++) {
+        const uint32_t from = mapa_shared(base, p);
+        float4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) w[u] = ld_cluster_f4(from + (c[u] * kPitch + r[u]) * 4);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          v[u].x += w[u].x;
+          v[u].y += w[u].y;
+          v[u].z += w[u].z;
+          v[u].w += w[u].w;
         }
       }
-      const int c = c0 + i / (kRows / 4), r = r0 + i % (kRows / 4) * 4;
-      typename Elem<OUT>::type* o =
-          reinterpret_cast<typename Elem<OUT>::type*>(g.out) + (int64_t)r * g.out_r + (int64_t)c * g.out_c;
-      const float f[4] = {v.x, v.y, v.z, v.w};
-      if (g.vec && r + 4 <= g.rows) {
-        if (OUT == F64E_F32)
-          *reinterpret_cast<float4*>(o) = v;
-        else
-          *reinterpret_cast<uint2*>(o) = make_uint2(Elem<OUT>::pack(v.x, v.y), Elem<OUT>::pack(v.z, v.w));
-      } else {
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (r + k < g.rows) {
-            if (OUT == F64E_F32)
-              reinterpret_cast<uint32_t*>(o)[k * g.out_r] = Elem<OUT>::bits(f[k]);
-            else
-              reinterpret_cast<uint16_t*>(o)[k * g.out_r] = (uint16_t)Elem<OUT>::bits(f[k]);
-          }
+      for (int u = 0; u < U; u++) {
+        if (i + u * NT >= i1) break;
+        const int row = r0 + r[u];
+        typename Elem<OUT>::type* o = reinterpret_cast<typename Elem<OUT>::type*>(g.out) + (int64_t)row * g.out_r +
+                                      (int64_t)(c0 + c[u]) * g.out_c;
+        const float f[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        if (g.vec && row + 4 <= g.rows) {
+          if (OUT == F64E_F32)
+            *reinterpret_cast<float4*>(o) = v[u];
+          else
+            *reinterpret_cast<uint2*>(o) = make_uint2(Elem<OUT>::pack(f[0], f[1]), Elem<OUT>::pack(f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; k++)
+            if (row + k < g.rows) {
+              if (OUT == F64E_F32)
+                reinterpret_cast<uint32_t*>(o)[k * g.out_r] = Elem<OUT>::bits(f[k]);
+              else
+                reinterpret_cast<uint16_t*>(o)[k * g.out_r] = (uint16_t)Elem<OUT>::bits(f[k]);
+            }
+        }
       }
     }
   }
@@ -396,19 +421,8 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
       done[dev] = true;
     }
   }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = k.split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)(tiles * k.split), 1, 1);
-  cfg.blockDim = dim3(32 * (4 + kQuantWarps<XT>), 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fp8_split_kernel<OUT, XT>, tw, tx, k);
+  return fp8_launch(fp8_split_kernel<OUT, XT>, (unsigned)(tiles * k.split), 32 * (4 + kQuantWarps<XT>), smem, k.split, s,
+                    tw, tx, k);
 }
 
 // The plan's numbers for wide rows by thin columns.
@@ -438,7 +452,7 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Fp8Sp
   k.x_words = x_type < 0 && fp8_scale_words(k.x);
   const int es = out_type == F64E_F32 ? 4 : 2;
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
-  k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kRows * 4);
+  k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);
   const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * atoms * kAtom + (3 * kMaxStages + 1) * 8 + 16);
   const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
   if (x_type >= 0) {
