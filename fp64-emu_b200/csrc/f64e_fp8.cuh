@@ -25,7 +25,9 @@ namespace f64e {
 // These kernels are launched with programmatic stream serialization: a kernel
 // may be set up while the one before it in the stream drains.  It reads and
 // writes global memory only after launch_wait(), when that kernel has
-// completed; launch_next() lets the next one be set up.
+// completed; launch_next() lets the next one be set up.  Loads of what an
+// earlier kernel wrote are plain ld.global: the non-coherent path (__ldg) may
+// hold lines from before that kernel's end, since no kernel begins in between.
 __device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -146,14 +148,15 @@ __device__ __forceinline__ void load16(const typename Elem<T>::type* p, bool wid
   if (wide) {
 #pragma unroll
     for (int i = 0; i < Elem<T>::kWords; i += 8)
-      asm("ld.global.nc.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
           : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]), "=r"(w[i + 6]),
             "=r"(w[i + 7])
-          : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+          : "l"(reinterpret_cast<const uint32_t*>(p) + i)
+          : "memory");
   } else {
 #pragma unroll
     for (int i = 0; i < Elem<T>::kWords; i += 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i / 4];
       w[i] = v.x;
       w[i + 1] = v.y;
       w[i + 2] = v.z;
@@ -167,13 +170,13 @@ template <int T>
 __device__ __forceinline__ void load16_some(const typename Elem<T>::type* p, int step, int64_t n, uint32_t* w) {
   if (Elem<T>::kWords == 16) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) w[i % Elem<T>::kWords] = i * step < n ? __ldg(reinterpret_cast<const uint32_t*>(p) + i * step) : 0;
+    for (int i = 0; i < 16; i++) w[i % Elem<T>::kWords] = i * step < n ? reinterpret_cast<const uint32_t*>(p)[i * step] : 0;
   } else {
     const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
     for (int i = 0; i < 16; i += 2) {
-      const uint32_t lo = i * step < n ? __ldg(u + i * step) : 0;
-      const uint32_t hi = (i + 1) * step < n ? __ldg(u + (i + 1) * step) : 0;
+      const uint32_t lo = i * step < n ? u[i * step] : 0;
+      const uint32_t hi = (i + 1) * step < n ? u[(i + 1) * step] : 0;
       w[i / 2] = lo | (hi << 16);
     }
   }
@@ -388,14 +391,14 @@ __device__ __forceinline__ void scale_atoms(const Fp8Operand& o, int rows, int n
   uint32_t v[4 * N];
   if (words && 4 * j + 4 <= nkb) {
 #pragma unroll
-    for (int w = 0; w < 4 * N; w++) v[w] = __ldg(reinterpret_cast<const uint32_t*>(p[w] + 4 * j));
+    for (int w = 0; w < 4 * N; w++) v[w] = *reinterpret_cast<const uint32_t*>(p[w] + 4 * j);
   } else {
     uint32_t b[4 * N][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
 #pragma unroll
-      for (int w = 0; w < 4 * N; w++) b[w][i] = __ldg(p[w] + at);
+      for (int w = 0; w < 4 * N; w++) b[w][i] = p[w][at];
     }
 #pragma unroll
     for (int w = 0; w < 4 * N; w++) v[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);

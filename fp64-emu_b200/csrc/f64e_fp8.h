@@ -89,16 +89,11 @@ int64_t fp8_gemm_workspace(const Fp8GemmArgs& g);
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s);
 // The same product on one-CTA tiles whose K is split over a cluster
 // (f64e_fp8_split.cu), for few rows or columns.
-struct Fp8SplitPlan {
-  int cols;        // columns of a tile: the smaller dimension, a multiple of 16 up to 256
-  int split;       // CTAs that share a tile's K
-  bool use;
-};
-Fp8SplitPlan fp8_split_plan(const Fp8GemmArgs& g);
-cudaError_t launch_fp8_split(const Fp8GemmArgs& g, const Fp8SplitPlan& p, cudaStream_t s);
+bool fp8_use_split(const Fp8GemmArgs& g);
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, cudaStream_t s);
 // y = quantised(x) @ w^T for a few rows of x (at most kFusedRows): x is
 // quantised in row blocks by the CTAs that contract it.
-constexpr int kFusedRows = 32;
+constexpr int kFusedRows = 16;
 struct Fp8LinearArgs {
   Fp8GemmArgs g;   // b: the weights; a unused
   const void* x;   // [M][ldx] of type x_type; the output has the same type

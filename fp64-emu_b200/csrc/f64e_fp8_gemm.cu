@@ -82,18 +82,26 @@ __device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, cha
                                              int cols) {
   constexpr int ES = OutOf<OUT>::kBytes, PER = 16 / ES, COLS = RB / ES;
   constexpr int ROWS = (int)kStage / RB, AT = 32 / COLS;   // staged rows, rows written at once
-  const int c = lane % COLS, ch = c / PER;
-#pragma unroll 4
-  for (int t = 0; t < ROWS; t += AT) {
-    const int r = t + lane / COLS;
-    const uint8_t* s = stage + staged_at<RB>(r, ch) + (c % PER) * ES;
-    char* o = out + ((int64_t)r * ldo + c) * ES;
-    if (r < rows && c < cols) {
-      if (ES == 4)
-        *reinterpret_cast<uint32_t*>(o) = *reinterpret_cast<const uint32_t*>(s);
-      else
-        *reinterpret_cast<uint16_t*>(o) = *reinterpret_cast<const uint16_t*>(s);
+  constexpr int U = ES == 4 ? 4 : 8;   // rows read before they are written
+  const int c = lane % COLS, ch = c / PER, r0 = lane / COLS;
+  if (c >= cols) return;
+  char* o = out + ((int64_t)r0 * ldo + c) * ES;
+#pragma unroll
+  for (int t = 0; t < ROWS / AT; t += U) {
+    uint32_t v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const uint8_t* s = stage + staged_at<RB>((t + u) * AT + r0, ch) + (c % PER) * ES;
+      v[u] = ES == 4 ? *reinterpret_cast<const uint32_t*>(s) : *reinterpret_cast<const uint16_t*>(s);
     }
+#pragma unroll
+    for (int u = 0; u < U; u++, o += AT * ldo * ES)
+      if ((t + u) * AT + r0 < rows) {
+        if (ES == 4)
+          *reinterpret_cast<uint32_t*>(o) = v[u];
+        else
+          *reinterpret_cast<uint16_t*>(o) = (uint16_t)v[u];
+      }
   }
 }
 
@@ -442,6 +450,9 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       auto put = [&](int p, const float* v) {
         constexpr int RB = TRANS ? 32 * ES : 64;
         const int col0 = n0 + column(p);
+        // Nothing to write; and every block that takes a buffer has a store,
+        // which the wait below counts on.
+        if (row0 >= g.M || col0 >= g.N) return;
         uint8_t* stage = staging + (2 * (warp - 4) + (puts++ & 1)) * kStage;
         if (g.tma_out) {   // the store before the last has been read
           if (lane == 0) tma_store_wait_read<1>();
@@ -454,7 +465,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
         if (g.tma_out) {
           fence_async_shared();
           __syncwarp();
-          if (lane == 0 && row0 < g.M && col0 < g.N) tma_store_2d(&tmapO, TRANS ? row0 : col0, TRANS ? col0 : row0, stage);
+          if (lane == 0) tma_store_2d(&tmapO, TRANS ? row0 : col0, TRANS ? col0 : row0, stage);
         } else {
           __syncwarp();
           if (TRANS)
@@ -604,11 +615,11 @@ __global__ void __launch_bounds__(256) fp8_transpose_kernel(const uint8_t* q, in
       uint32_t v = 0;
       if (k < K) {
         if (r + 4 <= rows) {
-          v = __ldg(reinterpret_cast<const uint32_t*>(p));
+          v = *reinterpret_cast<const uint32_t*>(p);
         } else {
 #pragma unroll
           for (int b = 0; b < 4; b++)
-            if (r + b < rows) v |= (uint32_t)__ldg(p + b) << (8 * b);
+            if (r + b < rows) v |= (uint32_t)p[b] << (8 * b);
         }
       }
       w[u][i] = v;
@@ -648,13 +659,12 @@ bool transpose_first(int64_t M, int64_t N, int64_t K, int sms) {
 }  // namespace
 
 int64_t fp8_gemm_workspace(const Fp8GemmArgs& g) {
-  if (g.a.kmajor || g.b.kmajor || fp8_split_plan(g).use || !transpose_first(g.M, g.N, g.K, 148)) return 0;
+  if (g.a.kmajor || g.b.kmajor || fp8_use_split(g) || !transpose_first(g.M, g.N, g.K, 148)) return 0;
   return std::min(g.M, g.N) * round16(g.K);
 }
 
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s) {
-  const Fp8SplitPlan plan = fp8_split_plan(g);
-  if (plan.use) return launch_fp8_split(g, plan, s);
+  if (fp8_use_split(g)) return launch_fp8_split(g, s);
   GemmK k;
   k.a = g.a;
   k.b = g.b;

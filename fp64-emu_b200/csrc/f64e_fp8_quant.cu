@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
     if (rb * kFp8Block + g + 32 * u >= a.rows) continue;
     const uint8_t* p = q + (int64_t)(32 * u) * a.ldq;
     if (VEC && n >= (l + 1) * 16) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + l * 16));
+      const uint4 v = *reinterpret_cast<const uint4*>(p + l * 16);
       w[u][0] = v.x;
       w[u][1] = v.y;
       w[u][2] = v.z;
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
     } else {
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        if (col_of<VEC>(l, i) < n) w[u][i >> 2] |= (uint32_t)__ldg(p + col_of<VEC>(l, i)) << (8 * (i & 3));
+        if (col_of<VEC>(l, i) < n) w[u][i >> 2] |= (uint32_t)p[col_of<VEC>(l, i)] << (8 * (i & 3));
     }
   }
   const bool per_col = a.blocks == F64E_BLOCKS_COL;
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const int c = col_of<VEC>(l, i);
-      sc[i] = c < n ? scale_of_byte(__ldg(s + c * a.s_col)) : 0.f;
+      sc[i] = c < n ? scale_of_byte(s[c * a.s_col]) : 0.f;
     }
   }
 #pragma unroll
@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
     const int64_t row = rb * kFp8Block + g + 32 * u;
     if (row >= a.rows) break;
     if (!per_col) {
-      const float one = scale_of_byte(__ldg(a.s + (a.blocks == F64E_BLOCKS_ROW ? row : rb) * a.s_row + cb * a.s_col));
+      const float one = scale_of_byte(a.s[(a.blocks == F64E_BLOCKS_ROW ? row : rb) * a.s_row + cb * a.s_col]);
 #pragma unroll
       for (int i = 0; i < 16; i++) sc[i] = one;
     }

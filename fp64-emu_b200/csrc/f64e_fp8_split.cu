@@ -20,6 +20,7 @@
 // Every wait is bounded; one that runs out records its site, and the CTA goes
 // on to the cluster barriers without storing.
 #include <algorithm>
+#include <array>
 #include <map>
 #include <mutex>
 
@@ -75,10 +76,9 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// Warps that quantise x (the epilogue's four among them); twice the registers
-// a row, in 32 bits, leave room for half as many.
+// Warps that quantise x, the epilogue's four among them.
 template <int XT>
-constexpr int kQuantWarps = XT == F64E_F16 || XT == F64E_BF16 ? 8 : 4;
+constexpr int kQuantWarps = XT >= 0 ? 8 : 4;
 
 // XT: type of x when the kernel quantises it, -1 for codes.
 template <int OUT, int XT>
@@ -425,17 +425,74 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
                     tw, tx, k);
 }
 
-// The plan's numbers for wide rows by thin columns.
-cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Fp8SplitPlan& p, cudaStream_t s) {
+// Clusters of `split` CTAs that the current device holds at once (a cluster's
+// CTAs share a GPC, so fewer than its SMs divided by the split).
+cudaError_t resident_clusters(int split, int sms, int* out) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  static std::mutex mtx;
+  static std::map<int, std::array<int, kMaxSplit + 1>> known;
+  std::lock_guard<std::mutex> lk(mtx);
+  int& n = known[dev][split];
+  if (n == 0) {
+    const size_t smem = 200 * 1024;   // any amount above half an SM's gives the same answer
+    e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(sms / split * split), 1, 1);
+    cfg.blockDim = dim3(32 * (4 + kQuantWarps<-1>), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int c = 0;
+    e = cudaOccupancyMaxActiveClusters(&c, fp8_split_kernel<F64E_BF16, -1>, &cfg);
+    if (e != cudaSuccess) return e;
+    n = std::max(c, 1);
+  }
+  *out = n;
+  return cudaSuccess;
+}
+
+// The split of least time, in cycles: waves of clusters times what a CTA does,
+// some 500 a block of k (its MMA warp's loop) or, of all CTAs together, the
+// copies' 5 a block (16 KB at the HBM rate), and 3000 to start up and add the
+// sums.  Measured on one row: 2048 x 8192 9.1 us with 7 CTAs a tile and 14.3
+// with 8, of which the device holds one cluster too few at once.
+cudaError_t choose_split(int64_t tiles, int64_t nkb, int sms, int* split) {
+  int64_t best = -1;
+  for (int s = 1; s <= kMaxSplit && s <= nkb; s++) {
+    int held = 0;
+    const cudaError_t e = resident_clusters(s, sms, &held);
+    if (e != cudaSuccess) return e;
+    const int64_t ctas = std::min<int64_t>(tiles, held) * s;
+    const int64_t cost = (tiles + held - 1) / held * ((nkb + s - 1) / s * std::max<int64_t>(500, 5 * ctas) + 3000);
+    if (best < 0 || cost < best) {
+      best = cost;
+      *split = s;
+    }
+  }
+  return cudaSuccess;
+}
+
+// rows x cols of k.w and k.x; cols_per_tile a multiple of 16.
+cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, int cols_per_tile, int sms, cudaStream_t s) {
   CUtensorMap tw, tx = {};
   if (!fp8_encode_codes(&tw, k.w, k.rows, K, kRows) ||
-      (x_type < 0 && !fp8_encode_codes(&tx, k.x, k.cols, K, p.cols)))
+      (x_type < 0 && !fp8_encode_codes(&tx, k.x, k.cols, K, cols_per_tile)))
     return cudaErrorInvalidValue;
   k.nkb = (int)((K + kBlock - 1) / kBlock);
   k.K = K;
-  k.bn = p.cols;
-  k.split = p.split;
+  k.bn = cols_per_tile;
   k.tiles_r = (k.rows + kRows - 1) / kRows;
+  const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
+  const cudaError_t e = choose_split(tiles, k.nkb, sms, &k.split);
+  if (e != cudaSuccess) return e;
   const int per_cta = (k.nkb + k.split - 1) / k.split;
   const int atoms = k.bn > 128 ? 3 : 2;
   const size_t stage = kWideBytes + (size_t)k.bn * kBlock;
@@ -454,7 +511,6 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Fp8Sp
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
   k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);
   const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * atoms * kAtom + (3 * kMaxStages + 1) * 8 + 16);
-  const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
   if (x_type >= 0) {
     switch (x_type) {
       case F64E_F32: return launch_kernel<F64E_F32, F64E_F32>(tw, tx, k, tiles, smem, s);
@@ -469,25 +525,14 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Fp8Sp
   }
 }
 
-int split_of(int64_t tiles, int64_t nkb, int sms) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplit, nkb, sms / std::max<int64_t>(tiles, 1)}));
-}
-
 }  // namespace
 
-Fp8SplitPlan fp8_split_plan(const Fp8GemmArgs& g) {
-  Fp8SplitPlan p = {};
-  const int64_t thin = std::min(g.M, g.N), wide = std::max(g.M, g.N), nkb = (g.K + kBlock - 1) / kBlock;
-  const Fp8Operand& t = g.M <= g.N ? g.a : g.b;
-  const int64_t tc = (thin + 255) / 256;
-  p.cols = (int)(((thin + tc - 1) / tc + 15) / 16 * 16);
-  const int64_t tiles = (wide + kRows - 1) / kRows * tc;
-  p.split = split_of(tiles, nkb, g.sms);
-  p.use = t.kmajor && thin <= 256;
-  return p;
+bool fp8_use_split(const Fp8GemmArgs& g) {
+  const Fp8Operand& thin = g.M <= g.N ? g.a : g.b;
+  return thin.kmajor && std::min(g.M, g.N) <= 256;
 }
 
-cudaError_t launch_fp8_split(const Fp8GemmArgs& g, const Fp8SplitPlan& p, cudaStream_t s) {
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, cudaStream_t s) {
   SplitArgs k = {};
   const bool a_thin = g.M <= g.N;
   k.w = a_thin ? g.b : g.a;
@@ -498,7 +543,7 @@ cudaError_t launch_fp8_split(const Fp8GemmArgs& g, const Fp8SplitPlan& p, cudaSt
   k.out_r = a_thin ? 1 : g.ldo;
   k.out_c = a_thin ? g.ldo : 1;
   k.wait_limit_ns = g.wait_limit_ns;
-  return launch(k, g.out_type, -1, g.K, p, s);
+  return launch(k, g.out_type, -1, g.K, (k.cols + 15) / 16 * 16, g.sms, s);
 }
 
 cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
@@ -519,10 +564,7 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
   k.x_vec = x % 16 == 0 && (pitch % 16 == 0 || g.M == 1);
   k.x_wide = x % 32 == 0 && (pitch % 32 == 0 || g.M == 1);
   k.wait_limit_ns = g.wait_limit_ns;
-  Fp8SplitPlan p = {};
-  p.cols = (int)((g.M + 15) / 16 * 16);
-  p.split = split_of((g.N + kRows - 1) / kRows, (g.K + kBlock - 1) / kBlock, g.sms);
-  return launch(k, a.x_type, a.x_type, g.K, p, s);
+  return launch(k, a.x_type, a.x_type, g.K, (k.cols + 15) / 16 * 16, g.sms, s);
 }
 
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s) {

@@ -367,6 +367,23 @@ def test_products_repeat_bit_for_bit():
             assert torch.equal(fp64_emu.mm_fp8(a, b, sa, sb, SF), first)
 
 
+@pytest.mark.parametrize("M,N", [(513, 384), (384, 513), (300, 289), (257, 257)])
+def test_products_whose_last_tile_is_nearly_empty(M, N):
+    """Most of a warp's output blocks lie outside the matrix there; the few inside must not share a buffer with them."""
+    a, sa, av = operand(M, 640, "row", E4, 1)
+    b, sb, bv = operand(640, N, "tile", E4, 2)
+    c, sc, cv = operand(N, 640, "tile", E4, 3)
+    for out in (SF, BF):
+        for _ in range(60):
+            first = fp64_emu.mm_nt_fp8(a, b, sa, sb, out)
+            second = fp64_emu.mm_fp8(a, c, sa, sc, out)
+        R.check_product(first, av, bv)
+        R.check_product(second, av, cv.t())
+        for _ in range(200):
+            assert torch.equal(fp64_emu.mm_nt_fp8(a, b, sa, sb, out), first)
+            assert torch.equal(fp64_emu.mm_fp8(a, c, sa, sc, out), second)
+
+
 def test_two_streams_at_once():
     a, sa, av = operand(300, 1024, "row", E4, 1)
     b, sb, bv = operand(512, 1024, "tile", E4, 2)
