@@ -374,37 +374,91 @@ __device__ __forceinline__ void mma_mx_pair(uint32_t d_tmem, uint64_t a_desc, ui
 enum : int { kWaitScales = 6, kWaitScalesFree = 7 };   // status sites, beside kWait*
 
 // --------------------------------------------------------------- scales --
-// Scale words of `N` atoms (rows r0 + 128 n + lane, + 32, + 64, + 96), a word
-// the bytes of blocks 4 j .. 4 j + 3.  Rows and blocks outside the operand read
-// their nearest neighbour's scale: their codes are zeros, and no store uses
-// them.  So no load depends on a branch, and all of them are in flight at once:
-// taken one word after the other they, not the MMAs, set the kernel's pace
-// where scales are strided bytes (4096 x 4096 x 8192 with column scales on
-// both sides: 231 us instead of 125).
+// Gathering the scales of `N` atoms (128 rows each, from r0) for blocks 4 j ..
+// 4 j + 3 of k, a warp, in two steps: loads into raw[4 N] registers, none of
+// which depends on a branch or on another, and, when the atoms' place is free,
+// the atoms themselves.  Taken one word after the other the scales, not the
+// MMAs, set the pace of a product (4096 x 4096 x 8192 with column scales on
+// both sides: 231 us instead of 125).  Rows and blocks outside the operand read
+// a neighbour's scale: their codes are zeros, and no store uses them.
+//   kScaleWords  four blocks' scales are one aligned word
+//   kScaleRows   four rows' scales are one aligned word (column blocks)
+//   kScaleTile   one scale for all rows of an atom
+//   kScaleBytes  any strides
 template <int N>
-__device__ __forceinline__ void scale_atoms(const Fp8Operand& o, int rows, int nkb, int r0, int j, int lane,
-                                            bool words, uint4* atoms) {
-  const uint8_t* p[4 * N];
+__device__ __forceinline__ void load_scales(const Fp8Operand& o, int rows, int nkb, int r0, int j, int lane,
+                                            uint32_t* raw) {
+  if (o.s_mode == kScaleRows) {
 #pragma unroll
-  for (int w = 0; w < 4 * N; w++)
-    p[w] = o.s + (int64_t)(min(r0 + w * 32 + lane, rows - 1) >> o.s_shift) * o.s_row;
-  uint32_t v[4 * N];
-  if (words && 4 * j + 4 <= nkb) {
+    for (int n = 0; n < N; n++) {
+      const uint8_t* p = o.s + min(r0 + n * 128 + lane * 4, rows - 4);
 #pragma unroll
-    for (int w = 0; w < 4 * N; w++) v[w] = *reinterpret_cast<const uint32_t*>(p[w] + 4 * j);
-  } else {
-    uint32_t b[4 * N][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
-#pragma unroll
-      for (int w = 0; w < 4 * N; w++) b[w][i] = p[w][at];
+      for (int i = 0; i < 4; i++)
+        raw[4 * n + i] = *reinterpret_cast<const uint32_t*>(p + (int64_t)min(4 * j + i, nkb - 1) * o.s_kb);
     }
+  } else if (o.s_mode == kScaleTile) {
 #pragma unroll
-    for (int w = 0; w < 4 * N; w++) v[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);
+    for (int n = 0; n < N; n++) {
+      const uint8_t* p = o.s + (int64_t)(min(r0 + n * 128, rows - 1) >> 7) * o.s_row;
+#pragma unroll
+      for (int i = 0; i < 4; i++) raw[4 * n + i] = p[(int64_t)min(4 * j + i, nkb - 1) * o.s_kb];
+    }
+  } else {
+    const uint8_t* p[4 * N];
+#pragma unroll
+    for (int w = 0; w < 4 * N; w++)
+      p[w] = o.s + (int64_t)(min(r0 + w * 32 + lane, rows - 1) >> o.s_shift) * o.s_row;
+    if (o.s_mode == kScaleWords && 4 * j + 4 <= nkb) {
+#pragma unroll
+      for (int w = 0; w < 4 * N; w++) raw[w] = *reinterpret_cast<const uint32_t*>(p[w] + 4 * j);
+    } else {
+      uint32_t b[4 * N][4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int64_t at = (int64_t)min(4 * j + i, nkb - 1) * o.s_kb;
+#pragma unroll
+        for (int w = 0; w < 4 * N; w++) b[w][i] = p[w][at];
+      }
+#pragma unroll
+      for (int w = 0; w < 4 * N; w++) raw[w] = b[w][0] | (b[w][1] << 8) | (b[w][2] << 16) | (b[w][3] << 24);
+    }
   }
+}
+// What was loaded as the atoms' words: row n * 128 + lane + 32 w in raw[4 n + w],
+// or, in kScaleRows, row n * 128 + 4 lane + w.
+template <int N>
+__device__ __forceinline__ void finish_scales(const Fp8Operand& o, uint32_t (&raw)[4 * N]) {
+  if (o.s_mode != kScaleRows && o.s_mode != kScaleTile) return;
 #pragma unroll
-  for (int n = 0; n < N; n++) atoms[n] = make_uint4(v[4 * n], v[4 * n + 1], v[4 * n + 2], v[4 * n + 3]);
+  for (int n = 0; n < N; n++) {
+    uint32_t* v = raw + 4 * n;
+    const uint32_t a = __byte_perm(v[0], v[1], 0x5140), b = __byte_perm(v[2], v[3], 0x5140);
+    const uint32_t c = __byte_perm(v[0], v[1], 0x7362), d = __byte_perm(v[2], v[3], 0x7362);
+    v[0] = __byte_perm(a, b, 0x5410);
+    if (o.s_mode == kScaleTile) {
+      v[1] = v[2] = v[3] = v[0];
+    } else {
+      v[1] = __byte_perm(a, b, 0x7632);
+      v[2] = __byte_perm(c, d, 0x5410);
+      v[3] = __byte_perm(c, d, 0x7632);
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_scales(const Fp8Operand& o, int lane, const uint32_t* words, uint8_t* atoms) {
+#pragma unroll
+  for (int n = 0; n < N; n++) {
+    const uint32_t* v = words + 4 * n;
+    if (o.s_mode == kScaleRows) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(atoms + n * 512 + (lane & 7) * 64 + (lane >> 3) * 4);
+      w[0] = v[0];
+      w[4] = v[1];
+      w[8] = v[2];
+      w[12] = v[3];
+    } else {
+      *reinterpret_cast<uint4*>(atoms + n * 512 + lane * 16) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+  }
 }
 
 }  // namespace f64e

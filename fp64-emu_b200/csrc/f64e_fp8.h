@@ -66,12 +66,14 @@ cudaError_t launch_fp8_dequant(const Fp8DequantArgs& a, int code, int out_type, 
 // One operand as the product sees it: `rows` output rows (or columns) by K
 // contracted values.  kmajor: codes [rows][ld], else [K][ld].  The scale of
 // (row r, contraction block kb) is s[(r >> s_shift) * s_row + kb * s_kb].
+enum { kScaleBytes = 0, kScaleWords = 1, kScaleRows = 2, kScaleTile = 3 };
 struct Fp8Operand {
   const uint8_t* q;
   int64_t ld;
   const uint8_t* s;
   int64_t s_row, s_kb;
   int s_shift;   // 0, or 7: one scale for 128 rows
+  int s_mode;    // how the products' kernels gather them (fp8_scale_mode)
   int code;
   int kmajor;
 };
@@ -106,7 +108,7 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s);
 bool fp8_encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
                    int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle);
 bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K, int box_rows);
-bool fp8_scale_words(const Fp8Operand& o);
+int fp8_scale_mode(const Fp8Operand& o, int64_t rows);
 
 // The device's status words of these products, cleared by the read; synchronizes.
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s);

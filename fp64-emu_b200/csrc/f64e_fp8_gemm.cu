@@ -51,8 +51,12 @@ bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64
   return fp8_encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(o.q), o.kmajor ? K : rows,
                    o.kmajor ? rows : K, o.ld, 128, o.kmajor ? box_rows : 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-bool fp8_scale_words(const Fp8Operand& o) {
-  return o.s_kb == 1 && o.s_row % 4 == 0 && (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
+int fp8_scale_mode(const Fp8Operand& o, int64_t rows) {
+  if (o.s_shift) return kScaleTile;
+  const bool base = (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
+  if (base && o.s_kb == 1 && o.s_row % 4 == 0) return kScaleWords;
+  if (base && o.s_row == 1 && o.s_kb % 4 == 0 && rows % 4 == 0) return kScaleRows;
+  return kScaleBytes;
 }
 
 namespace {
@@ -146,7 +150,6 @@ struct GemmK {
   char* out;
   uint64_t wait_limit_ns;
   uint32_t idesc;
-  int a_words, b_words;   // scales may be read four at a time
   int tma_out;            // the output's rows start on 16-byte boundaries
 };
 
@@ -207,7 +210,8 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSF + SF_STAGES * SF_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sf_full = empty_bar + STAGES;
-  uint64_t* sf_empty = sf_full + SF_STAGES;
+  uint64_t* sf_peer = sf_full + SF_STAGES;
+  uint64_t* sf_empty = sf_peer + SF_STAGES;
   uint64_t* acc_full = sf_empty + SF_STAGES;
   uint64_t* acc_empty = acc_full + 1;
   uint64_t* drain_bar = acc_empty + 1;
@@ -230,7 +234,8 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       mbar_init(&empty_bar[s], 1);
     }
     for (int s = 0; s < SF_STAGES; s++) {
-      mbar_init(&sf_full[s], 4);   // two loader warps of both CTAs
+      mbar_init(&sf_full[s], 2);   // the two loader warps
+      mbar_init(&sf_peer[s], 1);   // the other CTA's scales (leader)
       mbar_init(&sf_empty[s], 1);
     }
     mbar_init(acc_full, 1);
@@ -250,12 +255,12 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   const uint64_t lim = g.wait_limit_ns;
   int m0, n0;
   tile_origin(cluster, ntm, ntn, m0, n0);
-  uint4 atoms[2];
+  uint32_t raw_a[4], raw_b[8];   // scales on their way (warp 2: this CTA's rows of A, warp 3: B's)
   auto gather = [&](int kb) {
     if (warp == 2)
-      scale_atoms<1>(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, g.a_words, atoms);
+      load_scales<1>(g.a, g.M, g.nkb, m0 + PHALF * (int)rank, kb >> 2, lane, raw_a);
     else
-      scale_atoms<2>(g.b, g.N, g.nkb, n0, kb >> 2, lane, g.b_words, atoms);
+      load_scales<2>(g.b, g.N, g.nkb, n0, kb >> 2, lane, raw_b);
   };
   __syncwarp();
   cluster_arrive_relaxed();
@@ -264,15 +269,15 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   if (warp == 2 || warp == 3) gather(0);
   cluster_wait();
   const uint32_t full0 = mapa_shared(smem_u32(full_bar), 0);
-  const uint32_t sffull0 = mapa_shared(smem_u32(sf_full), 0);
+  const uint32_t sfpeer0 = mapa_shared(smem_u32(sf_peer), 0);
   const uint32_t accempty0 = mapa_shared(smem_u32(acc_empty), 0);
   auto stage_scales = [&](uint32_t ss) {
-    uint8_t* dst = sSF + ss * SF_BYTES + lane * 16;
     if (warp == 2) {
-      *reinterpret_cast<uint4*>(dst) = atoms[0];
+      finish_scales<1>(g.a, raw_a);
+      store_scales<1>(g.a, lane, raw_a, sSF + ss * SF_BYTES);
     } else {
-      *reinterpret_cast<uint4*>(dst + ATOM) = atoms[0];
-      *reinterpret_cast<uint4*>(dst + 2 * ATOM) = atoms[1];
+      finish_scales<2>(g.b, raw_b);
+      store_scales<2>(g.b, lane, raw_b, sSF + ss * SF_BYTES + ATOM);
     }
     fence_async_shared();
     __syncwarp();
@@ -351,8 +356,12 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           const int end = min(kb + chunk, g.nkb);
           uint32_t accumulate = 0;
           while (kb < end && ok) {   // a group of 4 blocks
-            // Its scales (group 0's came with the allocation's barrier).
-            if (gr > 0 && !mbar_wait_poll<true>(&sf_full[ss], sph ^ (ss == 0), lim, status, kWaitScales)) ok = false;
+            // Its scales, both CTAs' (group 0's came with the allocation's barrier).
+            if (gr > 0) {
+              const uint32_t par = sph ^ (ss == 0);
+              ok = mbar_wait_poll(&sf_full[ss], par, lim, status, kWaitScales) &&
+                   mbar_wait_poll<true>(&sf_peer[ss], par, lim, status, kWaitScales);
+            }
             // Two buffers in TMEM: the MMAs of the group before the last have
             // completed, by the ring (a stage is filled again only after
             // them) or, after short groups, by their own commit.
@@ -409,23 +418,64 @@ __global__ void __launch_bounds__(PTHREADS, 1)
         if (mbar_wait_poll(drain_bar, 0, drain_limit(lim), status, kWaitDrain) && ok)
           for (uint32_t r = 0; r < 2; r++) st_cluster_u32(mapa_shared(smem_u32((const void*)all_done), r), 1);
       }
+    } else {
+      // The other CTA passes on to the leader which of its scales are in place:
+      // a release at cluster scope takes too long (550 cycles or more) for the
+      // warps that gather them.
+      uint32_t ss = 1, par = 0;
+      for (int tile = cluster; tile < ntiles; tile += nclusters)
+        for (int kb = tile == cluster ? 4 : 0; kb < g.nkb; kb += 4) {
+          if (!mbar_wait_poll(&sf_full[ss], par ^ (ss == 0), lim, status, kWaitScales) || *abort_flag) {
+            *abort_flag = 1;
+            tile = ntiles;
+            break;
+          }
+          if (lane == 0) mbar_arrive_cluster(sfpeer0 + 8 * ss);
+          if (++ss == SF_STAGES) {
+            ss = 0;
+            par ^= 1;
+          }
+        }
     }
   } else if (warp < 4) {
-    // Scales: warp 2 gathers A's atom (this CTA's rows), warp 3 those of B.
-    uint32_t gr = 1;
-    bool ok = true;
-    for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
-      tile_origin(tile, ntm, ntn, m0, n0);
-      for (int kb = tile == cluster ? 4 : 0; kb < g.nkb; kb += 4, gr++) {
-        const uint32_t ss = gr % SF_STAGES;
-        gather(kb);
-        if (!mbar_wait_poll(&sf_empty[ss], ((gr / SF_STAGES) & 1) ^ 1, lim, status, kWaitScalesFree) || *abort_flag) {
-          *abort_flag = 1;
-          ok = false;
-          break;
-        }
-        stage_scales(ss);
-        if (lane == 0) mbar_arrive_cluster(sffull0 + 8 * ss);
+    // Scales, a group of 4 blocks after the other; the next group's loads are
+    // issued before this one's place is waited for.
+    int tile = cluster, kb = 0;
+    auto advance = [&]() {   // to the next group; its loads
+      kb += 4;
+      if (kb >= g.nkb) {
+        kb = 0;
+        tile += nclusters;
+        if (tile < ntiles) tile_origin(tile, ntm, ntn, m0, n0);
+      }
+      if (tile < ntiles) gather(kb);
+      return tile < ntiles;
+    };
+    uint32_t ss = 1, par = 1;   // group 0 is in place
+    for (bool more = advance(); more;) {
+      uint32_t now_a[4], now_b[8];
+#pragma unroll
+      for (int i = 0; i < 4; i++) now_a[i] = raw_a[i];
+#pragma unroll
+      for (int i = 0; i < 8; i++) now_b[i] = raw_b[i];
+      more = advance();
+      if (!mbar_wait_poll(&sf_empty[ss], par, lim, status, kWaitScalesFree) || *abort_flag) {
+        *abort_flag = 1;
+        break;
+      }
+      if (warp == 2) {
+        finish_scales<1>(g.a, now_a);
+        store_scales<1>(g.a, lane, now_a, sSF + ss * SF_BYTES);
+      } else {
+        finish_scales<2>(g.b, now_b);
+        store_scales<2>(g.b, lane, now_b, sSF + ss * SF_BYTES + ATOM);
+      }
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sf_full[ss]);
+      if (++ss == SF_STAGES) {
+        ss = 0;
+        par ^= 1;
       }
     }
   } else {
@@ -690,8 +740,8 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.out = static_cast<char*>(g.out);
   k.wait_limit_ns = g.wait_limit_ns;
   k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
-  k.a_words = fp8_scale_words(k.a);
-  k.b_words = fp8_scale_words(k.b);
+  k.a.s_mode = fp8_scale_mode(k.a, k.M);
+  k.b.s_mode = fp8_scale_mode(k.b, k.N);
   k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
   switch (g.out_type) {
     case F64E_F32: return launch_out<F64E_F32>(k, trans, g.K, g.sms, s);

@@ -56,7 +56,6 @@ struct SplitArgs {
   int tiles_r;          // tiles along the wide operand
   int nacc;             // accumulators (their sums are added at the end)
   uint32_t tmem_cols, idesc;
-  int w_words, x_words;
   char* out;
   int64_t out_r, out_c;   // output strides (elements) along rows and columns
   int vec;                // four rows of a column may be stored at once
@@ -111,21 +110,21 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
   // Before the CTA meets: the copies that need no free stage, the first scales
   // and the first blocks of x are on their way, and TMEM is allocated.
   const int n = kb1 - kb0, head = min(n, g.nst);
-  auto load = [&](int i) {
-    const int s = i % g.nst, k = (kb0 + i) * kBlock;
+  auto load = [&](int i, int s) {
+    const int k = (kb0 + i) * kBlock;
     uint8_t* st = smem + s * stage_bytes;
     mbar_arrive_expect_tx(&full[s], FUSED ? kWideBytes : stage_bytes);
     tma_load_2d(st, &tmapW, g.w.kmajor ? k : r0, g.w.kmajor ? r0 : k, &full[s]);
     if (!FUSED) tma_load_2d(st + kWideBytes, &tmapX, k, c0, &full[s]);
   };
-  uint4 atom[2] = {};
+  uint32_t raw_w[4] = {}, raw_x[8] = {};   // scales on their way (warp 2, warp 3)
   auto gather = [&](int kb) {
     if (warp == 2)
-      scale_atoms<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, g.w_words, atom);
+      load_scales<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, raw_w);
     else if (atoms > 2)
-      scale_atoms<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+      load_scales<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, raw_x);
     else
-      scale_atoms<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, g.x_words, atom);
+      load_scales<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, raw_x);
   };
   // Blocks of x in registers: warp 4 + b takes every QW-th block of k, from
   // the b-th on, of all rows: rows 4 p + lane / 8, eight lanes a block.
@@ -157,7 +156,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       for (int s = 0; s < g.nst; s++) mbar_init(&full[s], 1);
       fence_barrier_init();
       launch_wait();
-      for (int i = 0; i < head; i++) load(i);
+      for (int i = 0; i < head; i++) load(i, i);
     }
   } else if (warp == 1) {
     if (lane == 0) {
@@ -189,14 +188,18 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
 
   if (warp == 0) {
     if (elect_one()) {
-      int i = head;
+      int i = head, s = 0;
+      uint32_t par = 0;
       for (; i < n; i++) {
-        const int s = i % g.nst;
-        if (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitEmpty) || *abort_flag) {
+        if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitEmpty) || *abort_flag) {
           *abort_flag = 1;
           break;
         }
-        load(i);
+        load(i, s);
+        if (++s == g.nst) {
+          s = 0;
+          par ^= 1;
+        }
       }
       // Every copy has landed before the CTA goes on (the MMAs waited for
       // them too, unless a wait ran out).
@@ -248,21 +251,40 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     }
   } else if (warp == 2 || (warp == 3 && !FUSED)) {
     // Scale words for four blocks of k at a time, written to every stage that
-    // uses them.
-    for (int i = 0; i < n; i++) {
-      if (i > 0 && ((kb0 + i) & 3) == 0) gather(kb0 + i);
-      const int s = i % g.nst;
-      if (i >= g.nst &&
-          (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
+    // uses them; the next four's loads are issued before.  (Stages are counted,
+    // not divided for: this warp's steps are near the pace of the copies.)
+    uint32_t now_w[4], now_x[8], par = 1;
+    int s = 0;
+    for (int kb = kb0; kb < kb1; kb++) {
+      if (kb == kb0 || (kb & 3) == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) now_w[j] = raw_w[j];
+#pragma unroll
+        for (int j = 0; j < 8; j++) now_x[j] = raw_x[j];
+        if ((kb | 3) + 1 < kb1) gather((kb | 3) + 1);
+        if (warp == 2)
+          finish_scales<1>(g.w, now_w);
+        else
+          finish_scales<2>(g.x, now_x);   // (with one atom the second is not used)
+      }
+      if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
         *abort_flag = 1;
         break;
       }
-      uint8_t* dst = sSF + s * atoms * kAtom + (warp == 2 ? 0 : kAtom) + lane * 16;
-      *reinterpret_cast<uint4*>(dst) = atom[0];
-      if (warp == 3 && atoms > 2) *reinterpret_cast<uint4*>(dst + kAtom) = atom[1];
+      uint8_t* dst = sSF + s * atoms * kAtom;
+      if (warp == 2)
+        store_scales<1>(g.w, lane, now_w, dst);
+      else if (atoms > 2)
+        store_scales<2>(g.x, lane, now_x, dst + kAtom);
+      else
+        store_scales<1>(g.x, lane, now_x, dst + kAtom);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sf_full[s]);
+      if (++s == g.nst) {
+        s = 0;
+        par ^= 1;
+      }
     }
   } else if (warp >= 4) {
     if constexpr (FUSED) {
@@ -270,6 +292,12 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       // so warps that each took a quarter of every block's rows, with all
       // the arithmetic of a scale for each, set the kernel's pace on few rows
       // (8192^2, one row: 1450 cycles a block of k, copies 800).
+      int s = warp - 4;
+      uint32_t par = 1;
+      while (s >= g.nst) {
+        s -= g.nst;
+        par ^= 1;
+      }
       for (int i = warp - 4; i < n; i += QW) {
         uint4 code[PASSES];
         uint8_t scale[PASSES];
@@ -293,9 +321,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
           scale[p] = (uint8_t)(e + 127);
         }
         if (i + QW < n) load_x(i + QW);
-        const int s = i % g.nst;
-        if (i >= g.nst &&
-            (!mbar_wait_poll(&empty[s], (i / g.nst - 1) & 1, lim, status, kWaitScalesFree) || *abort_flag)) {
+        if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
           *abort_flag = 1;
           break;
         }
@@ -311,6 +337,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sf_full[s]);
+        for (s += QW; s >= g.nst; par ^= 1) s -= g.nst;
       }
     }
     // Partial sums to shared memory, by columns of 128 rows; the stages are free:
@@ -505,8 +532,8 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, int cols_pe
   k.tmem_cols = 32;
   while ((int)k.tmem_cols < k.bn * k.nacc + sf_cols) k.tmem_cols *= 2;
   k.idesc = idesc_mx(kRows, k.bn, k.w.code, k.x.code, !k.w.kmajor, 0);
-  k.w_words = fp8_scale_words(k.w);
-  k.x_words = x_type < 0 && fp8_scale_words(k.x);
+  k.w.s_mode = fp8_scale_mode(k.w, k.rows);
+  if (x_type < 0) k.x.s_mode = fp8_scale_mode(k.x, k.cols);
   const int es = out_type == F64E_F32 ? 4 : 2;
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
   k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);

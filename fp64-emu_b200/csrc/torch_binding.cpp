@@ -8,6 +8,7 @@
 // two-phase form used by the partitioned multi-GPU path and test aids.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -389,10 +390,16 @@ at::Tensor fp8_rows(const at::Tensor& x) {
 }
 int64_t fp8_pitch(const at::Tensor& x) { return x.size(0) <= 1 ? std::max<int64_t>(x.size(1), 1) : x.stride(0); }
 
+// A new tensor on x's device (current by the caller's guard) straight from the
+// allocator: these operators' small calls cost as much on the host as on the GPU.
+at::Tensor fp8_empty(const at::Tensor& x, at::IntArrayRef sizes, at::ScalarType type) {
+  if (!x.is_cuda()) return at::empty(sizes, x.options().dtype(type));
+  return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt);
+}
 // Codes [rows, cols] whose rows start on 16-byte boundaries.
 at::Tensor fp8_new_codes(const at::Tensor& x, int64_t rows, int64_t cols, at::ScalarType code) {
   const int64_t ld = (cols + 15) / 16 * 16;
-  at::Tensor q = at::empty({rows, ld}, x.options().dtype(code));
+  at::Tensor q = fp8_empty(x, {rows, ld}, code);
   return ld == cols ? q : q.as_strided({rows, cols}, {ld, 1});
 }
 int64_t fp8_code_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
@@ -407,8 +414,8 @@ std::tuple<at::Tensor, at::Tensor> fp8_quantize(const at::Tensor& x, int64_t blo
   const int64_t R = x.size(0), C = x.size(1);
   const at::Tensor xr = fp8_rows(x);
   at::Tensor q = fp8_new_codes(x, R, C, code);
-  at::Tensor s = at::empty({blocks == F64E_BLOCKS_ROW ? R : fp8_blocks(R), blocks == F64E_BLOCKS_COL ? C : fp8_blocks(C)},
-                           x.options().dtype(at::kFloat8_e8m0fnu));
+  at::Tensor s = fp8_empty(x, {blocks == F64E_BLOCKS_ROW ? R : fp8_blocks(R), blocks == F64E_BLOCKS_COL ? C : fp8_blocks(C)},
+                           at::kFloat8_e8m0fnu);
   check(f64e_fp8_quantize(xr.data_ptr(), fp8_type(x.scalar_type()), R, C, fp8_pitch(xr), (int32_t)blocks,
                           fp8_code(code), q.data_ptr(), fp8_code_pitch(C), s.data_ptr(), stream_of()));
   return {q, s};
@@ -425,8 +432,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> fp8_quantize_both(con
   const at::Tensor xr = fp8_rows(x);
   at::Tensor q = fp8_new_codes(x, R, C, code);
   at::Tensor qc = transposed ? fp8_new_codes(x, C, R, code).t() : fp8_new_codes(x, R, C, code);
-  const auto so = x.options().dtype(at::kFloat8_e8m0fnu);
-  at::Tensor s = at::empty({R, fp8_blocks(C)}, so), sc = at::empty({fp8_blocks(R), C}, so);
+  at::Tensor s = fp8_empty(x, {R, fp8_blocks(C)}, at::kFloat8_e8m0fnu);
+  at::Tensor sc = fp8_empty(x, {fp8_blocks(R), C}, at::kFloat8_e8m0fnu);
   check(f64e_fp8_quantize_both(xr.data_ptr(), fp8_type(x.scalar_type()), R, C, fp8_pitch(xr), fp8_code(code),
                                q.data_ptr(), s.data_ptr(), fp8_code_pitch(C), qc.data_ptr(), sc.data_ptr(), transposed,
                                fp8_code_pitch(transposed ? R : C), stream_of()));
@@ -447,7 +454,7 @@ at::Tensor fp8_dequantize(const at::Tensor& q, const at::Tensor& s, int64_t bloc
   TORCH_CHECK(s.device() == q.device(), "codes and scales must be on one device");
   const c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor qr = fp8_rows(q);
-  at::Tensor out = at::empty({R, C}, q.options().dtype(dtype));
+  at::Tensor out = fp8_empty(q, {R, C}, dtype);
   check(f64e_fp8_dequantize(qr.data_ptr(), fp8_code(q.scalar_type()), R, C, fp8_pitch(qr), (int32_t)blocks,
                             s.data_ptr(), s.stride(0), s.stride(1), out.data_ptr(), fp8_type(dtype), stream_of()));
   return out;
@@ -518,9 +525,9 @@ at::Tensor fp8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa
   p.ldo = p.N;
   p.a = ha.o;
   p.b = hb.o;
-  at::Tensor out = at::empty({p.M, p.N}, a.options().dtype(dtype));
+  at::Tensor out = fp8_empty(a, {p.M, p.N}, dtype);
   const size_t nb = f64e_fp8_workspace_size(&p);
-  const at::Tensor ws = nb ? at::empty({(int64_t)nb}, a.options().dtype(at::kByte)) : at::Tensor();
+  const at::Tensor ws = nb ? fp8_empty(a, {(int64_t)nb}, at::kByte) : at::Tensor();
   check(f64e_fp8_gemm(&p, ha.q.data_ptr(), sa.data_ptr(), hb.q.data_ptr(), sb.data_ptr(), out.data_ptr(),
                       nb ? ws.data_ptr() : nullptr, nb, stream_of()));
   return out;
@@ -568,8 +575,8 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optio
   p.ldo = p.N;
   p.b = hw.o;
   const size_t nb = f64e_fp8_linear_workspace_size(p.M, p.K);
-  const at::Tensor work = nb ? at::empty({(int64_t)nb}, x.options().dtype(at::kByte)) : at::Tensor();
-  at::Tensor y = at::empty(fp8_out_sizes(x, p.N), x.options());
+  const at::Tensor work = nb ? fp8_empty(x, {(int64_t)nb}, at::kByte) : at::Tensor();
+  at::Tensor y = fp8_empty(x, fp8_out_sizes(x, p.N), x.scalar_type());
   check(f64e_fp8_linear(&p, xr.data_ptr(), fp8_pitch(xr), hw.q.data_ptr(), wsc.data_ptr(), y.data_ptr(),
                         nb ? work.data_ptr() : nullptr, nb, stream_of()));
   return y;
