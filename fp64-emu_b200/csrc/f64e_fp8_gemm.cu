@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <type_traits>
 
 #include "f64e_fp8.cuh"
 #include "f64e_fp8.h"
@@ -80,32 +81,40 @@ __device__ __forceinline__ uint32_t staged_at(int row, int piece) {
 }
 
 // The staged rows to out (row pitch ldo elements), of which `rows` rows and
-// `cols` columns exist.
-template <int OUT, int RB>
+// `cols` columns exist, W bytes a lane.
+template <int OUT, int RB, int W>
 __device__ __forceinline__ void store_staged(const uint8_t* stage, int lane, char* out, int64_t ldo, int rows,
                                              int cols) {
-  constexpr int ES = OutOf<OUT>::kBytes, PER = 16 / ES, COLS = RB / ES;
-  constexpr int ROWS = (int)kStage / RB, AT = 32 / COLS;   // staged rows, rows written at once
-  constexpr int U = ES == 4 ? 4 : 8;   // rows read before they are written
-  const int c = lane % COLS, ch = c / PER, r0 = lane / COLS;
-  if (c >= cols) return;
-  char* o = out + ((int64_t)r0 * ldo + c) * ES;
+  constexpr int ES = OutOf<OUT>::kBytes, LANES = RB / W;                 // lanes of a row
+  constexpr int ROWS = (int)kStage / RB, AT = 32 / LANES < 1 ? 1 : 32 / LANES;   // staged rows, rows written at once
+  constexpr int U = W == 8 ? 2 : ES == 4 ? 4 : 8;                        // rows read before they are written
+  using Word = std::conditional_t<W == 8, uint2, std::conditional_t<W == 4, uint32_t, uint16_t>>;
+  const int at = lane % LANES * W, r0 = lane / LANES;
+  const int left = cols - at / ES;   // elements of this lane that exist
+  if (left <= 0) return;
+  char* o = out + (int64_t)r0 * ldo * ES + at;
 #pragma unroll
   for (int t = 0; t < ROWS / AT; t += U) {
-    uint32_t v[U];
+    Word v[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const uint8_t* s = stage + staged_at<RB>((t + u) * AT + r0, ch) + (c % PER) * ES;
-      v[u] = ES == 4 ? *reinterpret_cast<const uint32_t*>(s) : *reinterpret_cast<const uint16_t*>(s);
-    }
+    for (int u = 0; u < U; u++)
+      v[u] = *reinterpret_cast<const Word*>(stage + staged_at<RB>((t + u) * AT + r0, at >> 4) + (at & 15));
 #pragma unroll
-    for (int u = 0; u < U; u++, o += AT * ldo * ES)
-      if ((t + u) * AT + r0 < rows) {
-        if (ES == 4)
-          *reinterpret_cast<uint32_t*>(o) = v[u];
-        else
-          *reinterpret_cast<uint16_t*>(o) = (uint16_t)v[u];
+    for (int u = 0; u < U; u++, o += AT * ldo * ES) {
+      if ((t + u) * AT + r0 >= rows) continue;
+      if (left * ES >= W) {
+        *reinterpret_cast<Word*>(o) = v[u];
+      } else {
+#pragma unroll
+        for (int i = 0; i < W / ES; i++)
+          if (i < left) {
+            if (ES == 4)
+              reinterpret_cast<uint32_t*>(o)[i] = reinterpret_cast<const uint32_t*>(&v[u])[i];
+            else
+              reinterpret_cast<uint16_t*>(o)[i] = reinterpret_cast<const uint16_t*>(&v[u])[i];
+          }
       }
+    }
   }
 }
 
@@ -151,6 +160,7 @@ struct GemmK {
   uint64_t wait_limit_ns;
   uint32_t idesc;
   int tma_out;            // the output's rows start on 16-byte boundaries
+  int store_bytes;        // else: the boundaries they do start on, 2, 4 or 8
 };
 
 // --------------------------------------------------------------- CTA pair --
@@ -518,12 +528,15 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           if (lane == 0) tma_store_2d(&tmapO, TRANS ? row0 : col0, TRANS ? col0 : row0, stage);
         } else {
           __syncwarp();
-          if (TRANS)
-            store_staged<OUT, RB>(stage, lane, g.out + ((int64_t)col0 * g.ldo + row0) * ES, g.ldo, g.N - col0,
-                                  g.M - row0);
-          else
-            store_staged<OUT, RB>(stage, lane, g.out + ((int64_t)row0 * g.ldo + col0) * ES, g.ldo, g.M - row0,
-                                  g.N - col0);
+          const int orow = TRANS ? col0 : row0, ocol = TRANS ? row0 : col0;
+          const int rows = TRANS ? g.N - col0 : g.M - row0, cols = TRANS ? g.M - row0 : g.N - col0;
+          char* o = g.out + ((int64_t)orow * g.ldo + ocol) * ES;
+          if (g.store_bytes == 8)
+            store_staged<OUT, RB, 8>(stage, lane, o, g.ldo, rows, cols);
+          else if (g.store_bytes == 4)
+            store_staged<OUT, RB, 4>(stage, lane, o, g.ldo, rows, cols);
+          else if (ES == 2)
+            store_staged<OUT, RB, 2>(stage, lane, o, g.ldo, rows, cols);
           __syncwarp();
         }
       };
@@ -743,6 +756,9 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.a.s_mode = fp8_scale_mode(k.a, k.M);
   k.b.s_mode = fp8_scale_mode(k.b, k.N);
   k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
+  const int64_t pitch = g.ldo * (g.out_type == F64E_F32 ? 4 : 2);
+  k.store_bytes = 8;
+  while (reinterpret_cast<uintptr_t>(g.out) % k.store_bytes || pitch % k.store_bytes) k.store_bytes /= 2;
   switch (g.out_type) {
     case F64E_F32: return launch_out<F64E_F32>(k, trans, g.K, g.sms, s);
     case F64E_F16: return launch_out<F64E_F16>(k, trans, g.K, g.sms, s);

@@ -6,9 +6,9 @@
 // cycle, some 16 instructions a value at most, so a thread works on sixteen
 // neighbouring values at a time: one or two loads, packed magnitudes, and the
 // scale's arithmetic shared by all of them.
-// Where rows do not start on 16-byte boundaries (VEC = false) the same thread
-// takes every eighth value instead, so that neighbouring lanes still touch
-// neighbouring elements, and codes are put in order in shared memory.
+// Where rows do not start on 16-byte boundaries (VEC = false) a quantising
+// thread takes every eighth value instead, so that neighbouring lanes still
+// touch neighbouring elements, and codes are put in order in shared memory.
 #include "f64e_fp8.cuh"
 #include "f64e_fp8.h"
 
@@ -295,22 +295,23 @@ __global__ void __launch_bounds__(kThreads, T == F64E_F32 || MODE == kRowsCols ?
 // --------------------------------------------------------- dequantise ----
 // Sixteen columns of up to four rows of one row block a thread (rows g, g +
 // 32, .. of the 128), so column scales are read once for the four.
-template <int CODE, int T, bool VEC>
+template <int CODE, int T>
 __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantArgs a, int ncb, bool wide) {
   const int l = threadIdx.x & 7, g = threadIdx.x >> 3;
-  const int64_t rb = blockIdx.x / ncb, col = (int64_t)(blockIdx.x % ncb) * kFp8Block;
-  const int64_t n = a.cols - col;
+  const int64_t rb = blockIdx.x / ncb, cb = blockIdx.x % ncb, col = cb * kFp8Block + l * 16;
+  const int64_t n = a.cols - col;   // columns from here on: none, some, or sixteen and more
   const uint8_t* q = a.q + (rb * kFp8Block + g) * a.ldq + col;
   uint32_t w[4][4];
   launch_next();
   launch_wait();
+  if (n <= 0) return;
 #pragma unroll
   for (int u = 0; u < 4; u++) {
     w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
     if (rb * kFp8Block + g + 32 * u >= a.rows) continue;
     const uint8_t* p = q + (int64_t)(32 * u) * a.ldq;
-    if (VEC && n >= (l + 1) * 16) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + l * 16);
+    if (n >= 16) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
       w[u][0] = v.x;
       w[u][1] = v.y;
       w[u][2] = v.z;
@@ -318,19 +319,15 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
     } else {
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        if (col_of<VEC>(l, i) < n) w[u][i >> 2] |= (uint32_t)p[col_of<VEC>(l, i)] << (8 * (i & 3));
+        if (i < n) w[u][i >> 2] |= (uint32_t)p[i] << (8 * (i & 3));
     }
   }
   const bool per_col = a.blocks == F64E_BLOCKS_COL;
-  const int64_t cb = blockIdx.x % ncb;
   float sc[16];
   if (per_col) {
     const uint8_t* s = a.s + rb * a.s_row + col * a.s_col;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int c = col_of<VEC>(l, i);
-      sc[i] = c < n ? scale_of_byte(s[c * a.s_col]) : 0.f;
-    }
+    for (int i = 0; i < 16; i++) sc[i] = i < n ? scale_of_byte(s[i * a.s_col]) : 0.f;
   }
 #pragma unroll
   for (int u = 0; u < 4; u++) {
@@ -349,12 +346,12 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
       f[2 * i + 1] = v.y * sc[2 * i + 1];
     }
     typename Elem<T>::type* o = static_cast<typename Elem<T>::type*>(a.out) + row * a.cols + col;
-    if (VEC && n >= (l + 1) * 16) {
+    if (n >= 16) {
       uint32_t b[Elem<T>::kWords];
 #pragma unroll
       for (int i = 0; i < Elem<T>::kWords; i++)
         b[i] = T == F64E_F32 ? Elem<T>::bits(f[i]) : Elem<T>::pack(f[(2 * i) & 15], f[(2 * i + 1) & 15]);
-      uint32_t* ow = reinterpret_cast<uint32_t*>(o + l * 16);
+      uint32_t* ow = reinterpret_cast<uint32_t*>(o);
       if (wide) {
 #pragma unroll
         for (int i = 0; i < Elem<T>::kWords; i += 8)
@@ -368,15 +365,63 @@ __global__ void __launch_bounds__(kThreads) fp8_dequant_kernel(const Fp8DequantA
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int c = col_of<VEC>(l, i);
-        if (c < n) {
+      for (int i = 0; i < 16; i++)
+        if (i < n) {
           if (T == F64E_F32)
-            reinterpret_cast<uint32_t*>(o)[c] = Elem<T>::bits(f[i]);
+            reinterpret_cast<uint32_t*>(o)[i] = Elem<T>::bits(f[i]);
           else
-            reinterpret_cast<uint16_t*>(o)[c] = (uint16_t)Elem<T>::bits(f[i]);
+            reinterpret_cast<uint16_t*>(o)[i] = (uint16_t)Elem<T>::bits(f[i]);
         }
-      }
+    }
+  }
+}
+
+// Rows that start anywhere: a warp writes 32 neighbouring elements of a row at
+// a time (thread: columns lane, lane + 32, .. of sixteen rows).
+template <int CODE, int T>
+__global__ void __launch_bounds__(kThreads) fp8_dequant_any_kernel(const Fp8DequantArgs a, int ncb) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t rb = blockIdx.x / ncb, cb = blockIdx.x % ncb, col = cb * kFp8Block + lane;
+  const int64_t row0 = rb * kFp8Block + warp * 16;
+  const int n = (int)min((int64_t)16, a.rows - row0);
+  launch_next();
+  launch_wait();
+  const bool per_col = a.blocks == F64E_BLOCKS_COL;
+  float sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    sc[i] = per_col && col + 32 * i < a.cols ? scale_of_byte(a.s[rb * a.s_row + (col + 32 * i) * a.s_col]) : 0.f;
+  constexpr int U = 8;   // rows read before they are written: loads do not pass stores
+  const uint8_t* q = a.q + row0 * a.ldq + col;
+  typename Elem<T>::type* o = static_cast<typename Elem<T>::type*>(a.out) + row0 * a.cols + col;
+  bool there[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) there[i] = col + 32 * i < a.cols;
+  for (int u0 = 0; u0 < n; u0 += U) {
+    uint32_t c[U][4];
+    float one[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const bool row = u0 + u < n;
+      one[u] = per_col || !row ? 0.f
+                               : scale_of_byte(a.s[(a.blocks == F64E_BLOCKS_ROW ? row0 + u0 + u : rb) * a.s_row + cb * a.s_col]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) c[u][i] = row && there[i] ? q[32 * i] : 0;
+      q += a.ldq;
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (u0 + u >= n) break;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (there[i]) {
+          const float f = values2<CODE>(c[u][i]).x * (per_col ? sc[i] : one[u]);
+          if (T == F64E_F32)
+            reinterpret_cast<uint32_t*>(o)[32 * i] = Elem<T>::bits(f);
+          else
+            reinterpret_cast<uint16_t*>(o)[32 * i] = (uint16_t)Elem<T>::bits(f);
+        }
+      o += a.cols;
     }
   }
 }
@@ -419,8 +464,8 @@ cudaError_t dequant_of(const Fp8DequantArgs& a, cudaStream_t s) {
   const int64_t pitch = a.cols * (int64_t)sizeof(typename Elem<T>::type);
   const bool wide = aligned(a.out, pitch, 32);
   if (aligned(a.q, a.ldq, 16) && aligned(a.out, pitch, 16))
-    return fp8_launch(fp8_dequant_kernel<CODE, T, true>, grid, kThreads, 0, 0, s, a, ncb, wide);
-  return fp8_launch(fp8_dequant_kernel<CODE, T, false>, grid, kThreads, 0, 0, s, a, ncb, wide);
+    return fp8_launch(fp8_dequant_kernel<CODE, T>, grid, kThreads, 0, 0, s, a, ncb, wide);
+  return fp8_launch(fp8_dequant_any_kernel<CODE, T>, grid, kThreads, 0, 0, s, a, ncb);
 }
 
 }  // namespace
