@@ -225,10 +225,10 @@ int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const
   Fp8LinearArgs a{};
   if (const int rc = check_problem(&q, &a.g)) return rc;
   if (const char* m = check_matrix(q.M, q.K)) return bad(m);
+  if (ldx < q.K) return bad("fp8: row pitch of x is below its columns");
   if (q.M == 0 || q.N == 0) return F64E_OK;
   if (q.K == 0) return bad("fp8: K must be at least 1");
   if (!x || !w || !w_scale || !out) return bad("fp8: null pointer");
-  if (ldx < q.K) return bad("fp8: row pitch of x is below its columns");
   if (reinterpret_cast<uintptr_t>(w) & 15) return bad("fp8: codes need 16-byte aligned rows");
   if (q.M > kFusedRows) {
     const size_t need = f64e_fp8_linear_workspace_size(q.M, q.K);

@@ -159,7 +159,7 @@ struct GemmK {
   char* out;
   uint64_t wait_limit_ns;
   uint32_t idesc;
-  int tma_out;            // the output's rows start on 16-byte boundaries
+  int tma_out;            // the output's rows start and end on 16-byte boundaries
   int store_bytes;        // else: the boundaries they do start on, 2, 4 or 8
 };
 
@@ -755,8 +755,11 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
   k.a.s_mode = fp8_scale_mode(k.a, k.M);
   k.b.s_mode = fp8_scale_mode(k.b, k.N);
-  k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * (g.out_type == F64E_F32 ? 4 : 2) % 16 == 0;
-  const int64_t pitch = g.ldo * (g.out_type == F64E_F32 ? 4 : 2);
+  // A TMA store clips a row's end at 16 bytes: the output's columns must fill
+  // them (with a wider pitch, what follows would be overwritten).
+  const int es = g.out_type == F64E_F32 ? 4 : 2;
+  k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * es % 16 == 0 && g.N * es % 16 == 0;
+  const int64_t pitch = g.ldo * es;
   k.store_bytes = 8;
   while (reinterpret_cast<uintptr_t>(g.out) % k.store_bytes || pitch % k.store_bytes) k.store_bytes /= 2;
   switch (g.out_type) {

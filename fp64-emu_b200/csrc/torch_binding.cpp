@@ -533,6 +533,14 @@ at::Tensor fp8_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa
   return out;
 }
 
+// Status of the 8-bit products on a device (f64e_fp8_status).
+int64_t fp8_status(int64_t device) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  int32_t st = 0;
+  check(f64e_fp8_status(stream_of(), &st));
+  return st;
+}
+
 // ---- a layer held in 8 bits ----
 void fp8_check_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 2, "x must have at least one dimension and w two");
@@ -730,6 +738,8 @@ TORCH_LIBRARY(fp64_emu_b200, ops) {
   ops.def("fp8_dequantize(Tensor q, Tensor s, int blocks, ScalarType dtype) -> Tensor");
   ops.def("fp8_mm(Tensor a, Tensor b, Tensor sa, Tensor sb, int layout, ScalarType dtype) -> Tensor");
   ops.def("fp8_linear(Tensor x, Tensor w, Tensor? ws=None) -> Tensor");
+  ops.def("fp8_status(int device) -> int");
+  ops.impl("fp8_status", &fp8_status);
   ops.impl("fp64_emu_maxp", &maxp);
   ops.impl("fp64_emu_workspace_bytes", &workspace_bytes);
   ops.impl("fp64_emu_set_wait_limit_ns", &set_wait_limit_ns);

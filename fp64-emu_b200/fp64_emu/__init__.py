@@ -219,9 +219,9 @@ def plan(K: int, bits: int = 53) -> int:
 
 from .host import HostStream  # noqa: E402  (uses _defaults and _tables above)
 from .fp8 import (quantize_fp8, quantize_fp8_both, dequantize_fp8, mm_fp8, mm_nt_fp8,  # noqa: E402
-                  mm_tn_fp8, linear_fp8)
+                  mm_tn_fp8, linear_fp8, fp8_status)
 
 __all__ = ["mm", "mm_nt", "bmm", "bmm_nt", "mm_timed", "plan", "plan_config", "range_bits",
            "mm_host", "mm_nt_host", "bmm_host", "bmm_nt_host", "HostStream",
            "quantize_fp8", "quantize_fp8_both", "dequantize_fp8", "mm_fp8", "mm_nt_fp8", "mm_tn_fp8",
-           "linear_fp8"]
+           "linear_fp8", "fp8_status"]

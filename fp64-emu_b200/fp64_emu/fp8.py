@@ -86,3 +86,12 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor = None) -
     blocks and in column blocks,
         dx = q_row(dy) @ q_tile(w),    dw = q_col(dy)^T @ q_col(x)."""
     return _linear(x, w, w_scale)
+
+
+def fp8_status(device: torch.device = None) -> int:
+    """0, or the site code of the first bounded device wait of an 8-bit product
+    that ran out on the device (default: the current one) since the last call;
+    the outputs of that product are not valid then.  Waits for the current
+    stream."""
+    index = torch.cuda.current_device() if device is None else torch.device(device).index
+    return ops.fp8_status(torch.cuda.current_device() if index is None else index)

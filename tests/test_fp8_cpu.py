@@ -117,6 +117,9 @@ def lib():
     L.f64e_fp8_gemm.argtypes = [ctypes.POINTER(Problem), vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
     L.f64e_fp8_workspace_size.argtypes = [ctypes.POINTER(Problem)]
     L.f64e_fp8_workspace_size.restype = ctypes.c_size_t
+    L.f64e_fp8_linear.argtypes = [ctypes.POINTER(Problem), vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    L.f64e_fp8_linear_workspace_size.argtypes = [i64, i64]
+    L.f64e_fp8_linear_workspace_size.restype = ctypes.c_size_t
     L.f64e_last_error.restype = ctypes.c_char_p
     return L
 
@@ -199,6 +202,32 @@ def test_gemm_abi_workspace(lib):
         assert "workspace" in lib.f64e_last_error().decode()
     p.b.k_major, p.b.ld = 1, 16384
     assert lib.f64e_fp8_workspace_size(ctypes.byref(p)) == 0
+
+
+def test_linear_abi_refusals(lib):
+    call = lambda p, x=P, ldx=256, w=P, out=P, ws=P, nb=1 << 30: lib.f64e_fp8_linear(  # noqa: E731
+        p and ctypes.byref(p), x, ldx, w, P, out, ws, nb, None)
+    p = good()
+    assert call(None) == 1
+    for kw, msg in ((dict(x=None), "null"), (dict(out=None), "null"), (dict(ldx=255), "pitch of x"),
+                    (dict(w=P + 8), "16-byte")):
+        assert call(p, **kw) == 1
+        assert msg in lib.f64e_last_error().decode()
+    for field, value, msg in (("K", 0, "at least 1"), ("ldo", 5, "pitch of the output"), ("out_type", 9, "element type"),
+                              ("N", -1, "negative")):
+        q = good()
+        setattr(q, field, value)
+        assert call(q) == 1
+        assert msg in lib.f64e_last_error().decode()
+    need = lib.f64e_fp8_linear_workspace_size(64, 250)
+    assert need == 64 * 256 + 64 * 2
+    assert lib.f64e_fp8_linear_workspace_size(16, 250) == 0
+    for ws, nb in ((None, need), (P, lib.f64e_fp8_linear_workspace_size(64, 256) - 1), (P + 64, 1 << 20)):
+        assert call(good(), ws=ws, nb=nb) == 2
+        assert "workspace" in lib.f64e_last_error().decode()
+    p.M = 0
+    assert call(p, x=None, ldx=0, w=None, out=None, ws=None, nb=0) == 1   # its pitch is still wrong
+    assert call(p, x=None, w=None, out=None, ws=None, nb=0) == 0
 
 
 # ------------------------------------------------------------------ fakes --

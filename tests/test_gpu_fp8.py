@@ -627,3 +627,116 @@ def test_traces_under_compile():
     f = lambda x: torch.relu(fp64_emu.linear_fp8(x, w, s))  # noqa: E731
     x = data(20, 256, BF, 1, 1)
     assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))
+
+
+def test_layer_through_the_c_abi():
+    """Few rows (one launch) and many (with a workspace), into a wider output whose other columns stay as they were."""
+    import ctypes
+    import os
+    from test_fp8_cpu import Operand, Problem
+    L = ctypes.CDLL(os.path.join(os.path.dirname(fp64_emu.__file__), "libf64e.so"))
+    vp, i64 = ctypes.c_void_p, ctypes.c_int64
+    L.f64e_fp8_linear.argtypes = [ctypes.POINTER(Problem), vp, i64, vp, vp, vp, vp, ctypes.c_size_t, vp]
+    L.f64e_fp8_linear_workspace_size.argtypes = [i64, i64]
+    L.f64e_fp8_linear_workspace_size.restype = ctypes.c_size_t
+    N, K = 300, 500
+    w = data(N, K, BF, 2, 1)
+    q, s = fp64_emu.quantize_fp8(w, "tile")
+    for M in (1, 7, 16, 17, 300):
+        for wide in (N, N + 1, N + 20):
+            x = data(M, K, BF, 1, 1)
+            out = torch.full((M + 1, wide), 77.0, dtype=BF, device="cuda")
+            p = Problem(M, N, K, 2, wide, Operand(), Operand(q.stride(0), 0, 1, 1, s.stride(0), s.stride(1)))
+            nb = L.f64e_fp8_linear_workspace_size(M, K)
+            ws = torch.empty(max(nb, 1), dtype=torch.uint8, device="cuda")
+            rc = L.f64e_fp8_linear(ctypes.byref(p), x.data_ptr(), K, q.data_ptr(), s.data_ptr(), out.data_ptr(),
+                                   ws.data_ptr() if nb else None, nb, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            R.check_product(out[:M, :N].contiguous(), *layer_reference(x, w))
+            assert (out[:, N:] == 77).all() and (out[M] == 77).all()
+
+
+def test_status_is_clear():
+    a, sa, _ = operand(300, 256, "row", E4, 1)
+    b, sb, _ = operand(256, 256, "tile", E4, 2)
+    fp64_emu.mm_fp8(a, b, sa, sb)
+    fp64_emu.mm_fp8(a[:3], b, sa[:3], sb)
+    assert fp64_emu.fp8_status() == 0
+    assert fp64_emu.fp8_status("cuda:0") == 0
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of values, and of output: the last rows are right."""
+    rows, cols = 70003, 32784
+    x = torch.zeros(rows, cols, dtype=BF, device="cuda")
+    x[-200:] = data(200, cols, BF, 1, 2)
+    lo = rows // 128 * 128 - 128     # whole row blocks from here on
+    for blocks in ("row", "col", "tile"):
+        q, s = fp64_emu.quantize_fp8(x, blocks)
+        at = lo if blocks == "row" else lo // 128
+        check_codes(x[lo:], q[lo:], s[at:], blocks, E4)
+        back = fp64_emu.dequantize_fp8(q, s, blocks, BF)
+        assert torch.equal(back[lo:].double(), R.values(q[lo:], s[at:], blocks))
+        del back
+    q, s, qt, st = fp64_emu.quantize_fp8_both(x, transposed=True)
+    check_codes(x[lo:], q[lo:], s[lo:], "row", E4)
+    check_codes(x[lo:], qt[lo:], st[lo // 128:], "col", E4)
+    del x, qt, st
+    a, sa, av = operand(rows, 128, "row", E4, 3)
+    b, sb, bv = operand(cols, 128, "row", E4, 4)
+    out = fp64_emu.mm_fp8(a, b, sa, sb, SF)
+    R.check_product(out[-150:], av[-150:], bv.t())
+    del out
+    out = fp64_emu.mm_fp8(b[:4], q[:, :128].contiguous(), sb[:4], s[:, :1].contiguous(), SF)
+    R.check_product(out[:, -150:].contiguous(), bv[:4], R.values(q[-150:, :128], s[-150:, :1], "row").t())
+
+
+def test_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    x = data(40, 300, BF, 1, 1).to("cuda:1")
+    w = data(64, 300, BF, 2, 1).to("cuda:1")
+    assert torch.cuda.current_device() == 0
+    y = fp64_emu.linear_fp8(x, w)
+    assert y.device.index == 1
+    R.check_product(y, *layer_reference(x, w))
+    with pytest.raises(RuntimeError, match="on one device"):
+        fp64_emu.linear_fp8(x, w.to("cuda:0"))
+
+
+@pytest.mark.parametrize("alive", [False, True])
+def test_backward_captured_beside_an_eager_graph(alive):
+    """A whole step with .backward() in a graph, in a process of its own, with and without an eager graph of the same
+    leaves alive; torch refuses the second with an exception where it cannot do it, and nothing ends the process."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = %r
+import torch, fp64_emu
+x = torch.randn(64, 256, device="cuda").bfloat16().requires_grad_()
+w = torch.randn(128, 256, device="cuda").bfloat16().requires_grad_()
+dy = torch.randn(64, 128, device="cuda").bfloat16()
+eager = fp64_emu.linear_fp8(x, w) if %r else None
+side = torch.cuda.Stream()
+side.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(side):
+    fp64_emu.linear_fp8(x, w).backward(dy)
+torch.cuda.synchronize()
+want = x.grad.clone(), w.grad.clone()
+x.grad = w.grad = None
+g = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(g, stream=side):
+        fp64_emu.linear_fp8(x, w).backward(dy)
+    x.grad.zero_(); w.grad.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x.grad, want[0]) and torch.equal(w.grad, want[1])
+    print("replayed")
+except RuntimeError as e:
+    print("refused")
+""" % ([p for p in sys.path if p], alive)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-1500:]
+    assert "replayed" in r.stdout or (alive and "refused" in r.stdout), r.stdout
