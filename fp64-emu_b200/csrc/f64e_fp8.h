@@ -91,8 +91,9 @@ int64_t fp8_gemm_workspace(const Fp8GemmArgs& g);
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s);
 // The same product on one-CTA tiles whose K is split over a cluster
 // (f64e_fp8_split.cu), for few rows or columns.
-bool fp8_use_split(const Fp8GemmArgs& g);
-cudaError_t launch_fp8_split(const Fp8GemmArgs& g, cudaStream_t s);
+// Launches it unless the estimate of its cycles exceeds other_cost, or the
+// smaller operand is not K-major; done says which.
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, int64_t other_cost, bool* done, cudaStream_t s);
 // y = quantised(x) @ w^T for a few rows of x (at most kFusedRows): x is
 // quantised in row blocks by the CTAs that contract it.
 constexpr int kFusedRows = 16;
@@ -108,7 +109,8 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s);
 bool fp8_encode_2d(CUtensorMap* map, CUtensorMapDataType type, void* base, int64_t inner, int64_t outer,
                    int64_t pitch_bytes, int box_inner, int box_outer, CUtensorMapSwizzle swizzle);
 bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64_t K, int box_rows);
-int fp8_scale_mode(const Fp8Operand& o, int64_t rows);
+// whole_squares: tiles start at multiples of 128 rows.
+int fp8_scale_mode(const Fp8Operand& o, int64_t rows, bool whole_squares);
 
 // The device's status words of these products, cleared by the read; synchronizes.
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s);

@@ -52,11 +52,11 @@ bool fp8_encode_codes(CUtensorMap* map, const Fp8Operand& o, int64_t rows, int64
   return fp8_encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, const_cast<uint8_t*>(o.q), o.kmajor ? K : rows,
                    o.kmajor ? rows : K, o.ld, 128, o.kmajor ? box_rows : 128, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-int fp8_scale_mode(const Fp8Operand& o, int64_t rows) {
-  if (o.s_shift) return kScaleTile;
+int fp8_scale_mode(const Fp8Operand& o, int64_t rows, bool whole_squares) {
+  if (o.s_shift && whole_squares) return kScaleTile;
   const bool base = (reinterpret_cast<uintptr_t>(o.s) & 3) == 0;
   if (base && o.s_kb == 1 && o.s_row % 4 == 0) return kScaleWords;
-  if (base && o.s_row == 1 && o.s_kb % 4 == 0 && rows % 4 == 0) return kScaleRows;
+  if (base && !o.s_shift && o.s_row == 1 && o.s_kb % 4 == 0 && rows % 4 == 0) return kScaleRows;
   return kScaleBytes;
 }
 
@@ -468,18 +468,19 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       for (int i = 0; i < 4; i++) now_a[i] = raw_a[i];
 #pragma unroll
       for (int i = 0; i < 8; i++) now_b[i] = raw_b[i];
+      if (warp == 2)
+        finish_scales<1>(g.a, now_a);
+      else
+        finish_scales<2>(g.b, now_b);
       more = advance();
       if (!mbar_wait_poll(&sf_empty[ss], par, lim, status, kWaitScalesFree) || *abort_flag) {
         *abort_flag = 1;
         break;
       }
-      if (warp == 2) {
-        finish_scales<1>(g.a, now_a);
+      if (warp == 2)
         store_scales<1>(g.a, lane, now_a, sSF + ss * SF_BYTES);
-      } else {
-        finish_scales<2>(g.b, now_b);
+      else
         store_scales<2>(g.b, lane, now_b, sSF + ss * SF_BYTES + ATOM);
-      }
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sf_full[ss]);
@@ -722,12 +723,25 @@ bool transpose_first(int64_t M, int64_t N, int64_t K, int sms) {
 }  // namespace
 
 int64_t fp8_gemm_workspace(const Fp8GemmArgs& g) {
-  if (g.a.kmajor || g.b.kmajor || fp8_use_split(g) || !transpose_first(g.M, g.N, g.K, 148)) return 0;
+  if (g.a.kmajor || g.b.kmajor || !transpose_first(g.M, g.N, g.K, 148)) return 0;
   return std::min(g.M, g.N) * round16(g.K);
 }
 
 cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t s) {
-  if (fp8_use_split(g)) return launch_fp8_split(g, s);
+  // Fewer tiles than CTA pairs: perhaps smaller tiles with K split over more of
+  // the SMs.  What a wave of pairs takes, in cycles: 600 a block of k (512 of
+  // MMAs), 11000 to start and to write the last tile, and what rows of the
+  // output that are not on 16-byte boundaries add (measured: 777 x 2043 x 1234
+  // in 32 bits 17.2 us, 13.8 with 2048 columns, 11.4 on tiles of 128 x 112).
+  const int es = g.out_type == F64E_F32 ? 4 : 2;
+  const bool tma_out =
+      (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * es % 16 == 0 && g.N * es % 16 == 0;
+  if (((g.M + PBM - 1) / PBM) * ((g.N + BN - 1) / BN) <= g.sms / 2) {
+    bool done = false;
+    const int64_t pairs_cost = (g.K + BK - 1) / BK * 600 + 11000 + (tma_out ? 0 : es == 4 ? 8000 : 3000);
+    const cudaError_t e = launch_fp8_split(g, pairs_cost, &done, s);
+    if (e != cudaSuccess || done) return e;
+  }
   GemmK k;
   k.a = g.a;
   k.b = g.b;
@@ -753,12 +767,11 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   k.out = static_cast<char*>(g.out);
   k.wait_limit_ns = g.wait_limit_ns;
   k.idesc = idesc_mx(PBM, BN, k.a.code, k.b.code, !k.a.kmajor, !k.b.kmajor);
-  k.a.s_mode = fp8_scale_mode(k.a, k.M);
-  k.b.s_mode = fp8_scale_mode(k.b, k.N);
+  k.a.s_mode = fp8_scale_mode(k.a, k.M, true);
+  k.b.s_mode = fp8_scale_mode(k.b, k.N, true);
   // A TMA store clips a row's end at 16 bytes: the output's columns must fill
   // them (with a wider pitch, what follows would be overwritten).
-  const int es = g.out_type == F64E_F32 ? 4 : 2;
-  k.tma_out = (reinterpret_cast<uintptr_t>(g.out) & 15) == 0 && g.ldo * es % 16 == 0 && g.N * es % 16 == 0;
+  k.tma_out = tma_out;
   const int64_t pitch = g.ldo * es;
   k.store_bytes = 8;
   while (reinterpret_cast<uintptr_t>(g.out) % k.store_bytes || pitch % k.store_bytes) k.store_bytes /= 2;

@@ -1,11 +1,11 @@
 // Products of block-scaled 8-bit codes with few rows or columns: a served
 // layer on a handful of tokens, a small batch.
 //
-// A CTA computes 128 rows of the large ("wide") operand by all columns of the
-// small ("thin") one, up to 256, and a cluster of up to eight CTAs shares the
-// tile's K, so that a product with few tiles still draws on most SMs: bound by
-// reading the wide operand, it needs their copies in flight (10 stages of 16
-// KB each), not their tensor cores.  The partial sums meet in shared memory:
+// A CTA computes 128 rows of the large ("wide") operand by up to 128 columns of
+// the small ("thin") one, and a cluster of up to eight CTAs shares the tile's K,
+// so that a product with few tiles still draws on most SMs: bound by reading
+// the wide operand, it needs their copies in flight (10 stages of 16 KB each),
+// not their tensor cores.  The partial sums meet in shared memory:
 // every CTA adds a share of the tile, in the order of the K ranges, so results
 // do not depend on timing and no scratch or second launch is needed.
 //
@@ -35,7 +35,7 @@ __device__ int g_fp8_split_status;
 namespace {
 
 constexpr int kBlock = kFp8Block, kRows = 128;
-constexpr int kMaxStages = 10, kMaxSplit = 8;
+constexpr int kMaxStages = 10, kMaxSplit = 8, kMaxCols = 128;
 constexpr uint32_t kWideBytes = kRows * kBlock, kAtom = 512;
 constexpr uint32_t kRing = 190 * 1024;   // shared memory for stages
 // More than half an SM's shared memory: no two kernels of this library that
@@ -89,9 +89,8 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
   const uint32_t raw_s = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_s + 1023u) & ~1023u) - raw_s);
   const uint32_t thin_bytes = g.bn * kBlock, stage_bytes = kWideBytes + thin_bytes;
-  const int atoms = g.bn > 128 ? 3 : 2;   // scale atoms of a stage: wide, thin (128 rows each)
   uint8_t* sSF = smem + g.ring;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + g.nst * atoms * kAtom);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + g.nst * 2 * kAtom);
   uint64_t* empty = full + kMaxStages;
   uint64_t* sf_full = empty + kMaxStages;
   uint64_t* acc_full = sf_full + kMaxStages;
@@ -117,14 +116,12 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     tma_load_2d(st, &tmapW, g.w.kmajor ? k : r0, g.w.kmajor ? r0 : k, &full[s]);
     if (!FUSED) tma_load_2d(st + kWideBytes, &tmapX, k, c0, &full[s]);
   };
-  uint32_t raw_w[4] = {}, raw_x[8] = {};   // scales on their way (warp 2, warp 3)
+  uint32_t raw[4] = {};   // scales on their way (warp 2: wide, warp 3: thin)
   auto gather = [&](int kb) {
     if (warp == 2)
-      load_scales<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, raw_w);
-    else if (atoms > 2)
-      load_scales<2>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, raw_x);
+      load_scales<1>(g.w, g.rows, g.nkb, r0, kb >> 2, lane, raw);
     else
-      load_scales<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, raw_x);
+      load_scales<1>(g.x, g.cols, g.nkb, c0, kb >> 2, lane, raw);
   };
   // Blocks of x in registers: warp 4 + b takes every QW-th block of k, from
   // the b-th on, of all rows: rows 4 p + lane / 8, eight lanes a block.
@@ -226,11 +223,10 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         break;
       }
       if (issuer) {
-        const uint32_t st = smem_u32(smem + s * stage_bytes), sf = smem_u32(sSF + s * atoms * kAtom);
-        const uint32_t sfa = sf_base + s * (4 * atoms), id = g.idesc | idesc_scale_byte(kb & 3);
+        const uint32_t st = smem_u32(smem + s * stage_bytes), sf = smem_u32(sSF + s * 2 * kAtom);
+        const uint32_t sfa = sf_base + s * 8, id = g.idesc | idesc_scale_byte(kb & 3);
         copy_scales(sfa, smem_desc_scales(sf));
         copy_scales(sfa + 4, smem_desc_scales(sf + kAtom));
-        if (atoms > 2) copy_scales(sfa + 8, smem_desc_scales(sf + 2 * kAtom));
         const uint64_t dw = smem_desc_sw128(st), dx = smem_desc_sw128(st + kWideBytes);
         mma_mx(d_tmem, dw, dx, id, sfa, sfa + 4, accumulate);
 #pragma unroll
@@ -251,33 +247,24 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     }
   } else if (warp == 2 || (warp == 3 && !FUSED)) {
     // Scale words for four blocks of k at a time, written to every stage that
-    // uses them; the next four's loads are issued before.  (Stages are counted,
+    // uses them; the next four's loads are issued first, but after these have
+    // arrived (a wait for some loads is one for all).  (Stages are counted,
     // not divided for: this warp's steps are near the pace of the copies.)
-    uint32_t now_w[4], now_x[8], par = 1;
+    const Fp8Operand& o = warp == 2 ? g.w : g.x;
+    uint32_t now[4], par = 1;
     int s = 0;
     for (int kb = kb0; kb < kb1; kb++) {
       if (kb == kb0 || (kb & 3) == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) now_w[j] = raw_w[j];
-#pragma unroll
-        for (int j = 0; j < 8; j++) now_x[j] = raw_x[j];
+        for (int j = 0; j < 4; j++) now[j] = raw[j];
+        finish_scales<1>(o, now);
         if ((kb | 3) + 1 < kb1) gather((kb | 3) + 1);
-        if (warp == 2)
-          finish_scales<1>(g.w, now_w);
-        else
-          finish_scales<2>(g.x, now_x);   // (with one atom the second is not used)
       }
       if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
         *abort_flag = 1;
         break;
       }
-      uint8_t* dst = sSF + s * atoms * kAtom;
-      if (warp == 2)
-        store_scales<1>(g.w, lane, now_w, dst);
-      else if (atoms > 2)
-        store_scales<2>(g.x, lane, now_x, dst + kAtom);
-      else
-        store_scales<1>(g.x, lane, now_x, dst + kAtom);
+      store_scales<1>(o, lane, now, sSF + (s * 2 + warp - 2) * kAtom);
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sf_full[s]);
@@ -326,7 +313,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
           break;
         }
         uint8_t* st = smem + s * stage_bytes + kWideBytes;
-        uint8_t* sf = sSF + s * atoms * kAtom + kAtom + ((kb0 + i) & 3);
+        uint8_t* sf = sSF + s * 2 * kAtom + kAtom + ((kb0 + i) & 3);
 #pragma unroll
         for (int p = 0; p < PASSES; p++) {
           if (p * 4 >= cols) break;
@@ -348,17 +335,27 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       const int q = warp & 3;
       const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
       float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;   // column pitch kPitch
-      for (int c = 0; c < cols; c += 16) {
-        float sum[16];
-        for (int a = 0; a * per < kb1 - kb0; a++) {
-          uint32_t v[16];
-          tmem_ld_32x32b_x16(taddr + a * g.bn + c, v);
+      if (n <= per && g.bn % 32 == 0) {   // one accumulator, 32 columns at a time
+        for (int c = 0; c < cols; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(taddr + c, v);
           tmem_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 16; k++) sum[k] = a == 0 ? __uint_as_float(v[k]) : sum[k] + __uint_as_float(v[k]);
+          for (int k = 0; k < 32; k++) part[(c + k) * kPitch] = __uint_as_float(v[k]);
         }
+      } else {
+        for (int c = 0; c < cols; c += 16) {
+          float sum[16];
+          for (int a = 0; a * per < n; a++) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(taddr + a * g.bn + c, v);
+            tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 16; k++) part[(c + k) * kPitch] = sum[k];
+            for (int k = 0; k < 16; k++) sum[k] = a == 0 ? __uint_as_float(v[k]) : sum[k] + __uint_as_float(v[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < 16; k++) part[(c + k) * kPitch] = sum[k];
+        }
       }
       tc_fence_before();
     }
@@ -390,17 +387,25 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         r[u] = (g.out_c == 1 ? j / cols : j % (kRows / 4)) * 4;
         v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       }
-      for (int p = 0; p < g.split; p++) {
-        const uint32_t from = mapa_shared(base, p);
-        float4 w[U];
+      for (int p0 = 0; p0 < g.split; p0 += 4) {   // four CTAs' sums in flight, added in order
+        float4 w[4][U];
 #pragma unroll
-        for (int u = 0; u < U; u++) w[u] = ld_cluster_f4(from + (c[u] * kPitch + r[u]) * 4);
+        for (int p = 0; p < 4; p++) {
+          if (p0 + p >= g.split) break;
+          const uint32_t from = mapa_shared(base, p0 + p);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          v[u].x += w[u].x;
-          v[u].y += w[u].y;
-          v[u].z += w[u].z;
-          v[u].w += w[u].w;
+          for (int u = 0; u < U; u++) w[p][u] = ld_cluster_f4(from + (c[u] * kPitch + r[u]) * 4);
+        }
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+          if (p0 + p >= g.split) break;
+#pragma unroll
+          for (int u = 0; u < U; u++) {
+            v[u].x += w[p][u].x;
+            v[u].y += w[p][u].y;
+            v[u].z += w[p][u].z;
+            v[u].w += w[p][u].w;
+          }
         }
       }
 #pragma unroll
@@ -452,92 +457,109 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
                     tw, tx, k);
 }
 
-// Clusters of `split` CTAs that the current device holds at once (a cluster's
-// CTAs share a GPC, so fewer than its SMs divided by the split).
-cudaError_t resident_clusters(int split, int sms, int* out) {
+// held[n]: clusters of n CTAs that the current device holds at once (a
+// cluster's CTAs share a GPC, so fewer than its SMs divided by n).  Asked once.
+cudaError_t resident_clusters(int sms, const int** held) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   static std::mutex mtx;
   static std::map<int, std::array<int, kMaxSplit + 1>> known;
   std::lock_guard<std::mutex> lk(mtx);
-  int& n = known[dev][split];
-  if (n == 0) {
+  auto it = known.find(dev);
+  if (it == known.end()) {
+    std::array<int, kMaxSplit + 1> h{};
     const size_t smem = 200 * 1024;   // any amount above half an SM's gives the same answer
     e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(sms / split * split), 1, 1);
-    cfg.blockDim = dim3(32 * (4 + kQuantWarps<-1>), 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int c = 0;
-    e = cudaOccupancyMaxActiveClusters(&c, fp8_split_kernel<F64E_BF16, -1>, &cfg);
-    if (e != cudaSuccess) return e;
-    n = std::max(c, 1);
+    for (int n = 1; n <= kMaxSplit; n++) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = n;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3((unsigned)(sms / n * n), 1, 1);
+      cfg.blockDim = dim3(32 * (4 + kQuantWarps<-1>), 1, 1);
+      cfg.dynamicSmemBytes = smem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int c = 0;
+      e = cudaOccupancyMaxActiveClusters(&c, fp8_split_kernel<F64E_BF16, -1>, &cfg);
+      if (e != cudaSuccess) return e;
+      h[n] = std::max(c, 1);
+    }
+    it = known.emplace(dev, h).first;
   }
-  *out = n;
+  *held = it->second.data();
   return cudaSuccess;
 }
 
-// The split of least time, in cycles: waves of clusters times what a CTA does,
-// some 500 a block of k (its MMA warp's loop) or, of all CTAs together, the
-// copies' 5 a block (16 KB at the HBM rate), and 3000 to start up and add the
-// sums.  Measured on one row: 2048 x 8192 9.1 us with 7 CTAs a tile and 14.3
-// with 8, of which the device holds one cluster too few at once.
-cudaError_t choose_split(int64_t tiles, int64_t nkb, int sms, int* split) {
-  int64_t best = -1;
-  for (int s = 1; s <= kMaxSplit && s <= nkb; s++) {
-    int held = 0;
-    const cudaError_t e = resident_clusters(s, sms, &held);
-    if (e != cudaSuccess) return e;
-    const int64_t ctas = std::min<int64_t>(tiles, held) * s;
-    const int64_t cost = (tiles + held - 1) / held * ((nkb + s - 1) / s * std::max<int64_t>(500, 5 * ctas) + 3000);
-    if (best < 0 || cost < best) {
-      best = cost;
-      *split = s;
+// How a product is cut: columns of a tile (a multiple of 16) and CTAs that
+// share a tile's K.
+struct Plan {
+  int bn = 0, split = 0;
+  int64_t cost = -1;   // cycles, estimated
+};
+
+// The cut of least time.  A CTA takes, a block of k, some 500 cycles (its MMA
+// warp's loop) or all CTAs' copies of 16 KB and bn x 128 bytes at 5300 bytes a
+// cycle (the L2's rate); 7500 to start and to end, 12 a column to put its sums
+// down and 32 to fetch the others' (16 bytes a cycle between SMs).  Tiles have
+// up to 128 columns: with 256, stages of 48 KB leave too few in flight (1024 x
+// 2048 x 2048 14.6 us against 11.7).  Measured, both sides of a choice: 1024^3
+// 7.7 us with 64 columns, 8.7 with 128; 8 x 2048 x 8192 9.1 us with 7 CTAs a
+// tile, 14.3 with 8, of whose clusters the device holds one too few at once.
+cudaError_t plan_tiles(int64_t rows, int64_t cols, int64_t nkb, int sms, Plan* best) {
+  const int* held_of = nullptr;
+  const cudaError_t e = resident_clusters(sms, &held_of);
+  if (e != cudaSuccess) return e;
+  const int64_t t0 = (cols + kMaxCols - 1) / kMaxCols;
+  for (int64_t t = t0; t <= 2 * t0; t += t0) {
+    const int64_t bn = ((cols + t - 1) / t + 15) / 16 * 16;
+    if (t > t0 && bn < 48) break;
+    const int64_t tiles = (rows + kRows - 1) / kRows * ((cols + bn - 1) / bn);
+    for (int s = 1; s <= kMaxSplit && s <= nkb; s++) {
+      const int64_t held = held_of[s];
+      const int64_t ctas = std::min(tiles, held) * s;
+      const int64_t block = std::max<int64_t>(500, ctas * (kWideBytes + bn * kBlock) / 5300);
+      const int64_t cost =
+          (tiles + held - 1) / held * ((nkb + s - 1) / s * block + 7500 + 12 * bn + 32 * bn * (s - 1) / s);
+      if (best->cost < 0 || cost < best->cost) *best = {(int)bn, s, cost};
     }
   }
   return cudaSuccess;
 }
 
-// rows x cols of k.w and k.x; cols_per_tile a multiple of 16.
-cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, int cols_per_tile, int sms, cudaStream_t s) {
+// k.rows x k.cols of k.w and k.x.
+cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Plan& plan, cudaStream_t s) {
   CUtensorMap tw, tx = {};
   if (!fp8_encode_codes(&tw, k.w, k.rows, K, kRows) ||
-      (x_type < 0 && !fp8_encode_codes(&tx, k.x, k.cols, K, cols_per_tile)))
+      (x_type < 0 && !fp8_encode_codes(&tx, k.x, k.cols, K, plan.bn)))
     return cudaErrorInvalidValue;
   k.nkb = (int)((K + kBlock - 1) / kBlock);
   k.K = K;
-  k.bn = cols_per_tile;
+  k.bn = plan.bn;
+  k.split = plan.split;
   k.tiles_r = (k.rows + kRows - 1) / kRows;
   const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
-  const cudaError_t e = choose_split(tiles, k.nkb, sms, &k.split);
-  if (e != cudaSuccess) return e;
   const int per_cta = (k.nkb + k.split - 1) / k.split;
-  const int atoms = k.bn > 128 ? 3 : 2;
   const size_t stage = kWideBytes + (size_t)k.bn * kBlock;
-  k.nst = (int)std::min<int64_t>({kMaxStages, per_cta, (int64_t)(kRing / (stage + atoms * kAtom))});
+  k.nst = (int)std::min<int64_t>({kMaxStages, per_cta, (int64_t)(kRing / (stage + 2 * kAtom))});
   // 32-bit outputs: a new accumulator every kChunkBlocks, as far as TMEM goes
-  const int sf_cols = k.nst * 4 * atoms;
+  const int sf_cols = k.nst * 8;
   k.nacc = out_type == F64E_F32
                ? std::max(1, std::min((per_cta + kChunkBlocks - 1) / kChunkBlocks, (512 - sf_cols) / k.bn))
                : 1;
   k.tmem_cols = 32;
   while ((int)k.tmem_cols < k.bn * k.nacc + sf_cols) k.tmem_cols *= 2;
   k.idesc = idesc_mx(kRows, k.bn, k.w.code, k.x.code, !k.w.kmajor, 0);
-  k.w.s_mode = fp8_scale_mode(k.w, k.rows);
-  if (x_type < 0) k.x.s_mode = fp8_scale_mode(k.x, k.cols);
+  k.w.s_mode = fp8_scale_mode(k.w, k.rows, true);
+  if (x_type < 0) k.x.s_mode = fp8_scale_mode(k.x, k.cols, k.bn >= k.cols || k.bn % 128 == 0);
   const int es = out_type == F64E_F32 ? 4 : 2;
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
   k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);
-  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * atoms * kAtom + (3 * kMaxStages + 1) * 8 + 16);
+  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * 2 * kAtom + (3 * kMaxStages + 1) * 8 + 16);
   if (x_type >= 0) {
     switch (x_type) {
       case F64E_F32: return launch_kernel<F64E_F32, F64E_F32>(tw, tx, k, tiles, smem, s);
@@ -554,12 +576,13 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, int cols_pe
 
 }  // namespace
 
-bool fp8_use_split(const Fp8GemmArgs& g) {
-  const Fp8Operand& thin = g.M <= g.N ? g.a : g.b;
-  return thin.kmajor && std::min(g.M, g.N) <= 256;
-}
-
-cudaError_t launch_fp8_split(const Fp8GemmArgs& g, cudaStream_t s) {
+cudaError_t launch_fp8_split(const Fp8GemmArgs& g, int64_t other_cost, bool* done, cudaStream_t s) {
+  *done = false;
+  if (!(g.M <= g.N ? g.a : g.b).kmajor) return cudaSuccess;
+  Plan plan;
+  const cudaError_t e = plan_tiles(std::max(g.M, g.N), std::min(g.M, g.N), (g.K + kBlock - 1) / kBlock, g.sms, &plan);
+  if (e != cudaSuccess || plan.cost > other_cost) return e;
+  *done = true;
   SplitArgs k = {};
   const bool a_thin = g.M <= g.N;
   k.w = a_thin ? g.b : g.a;
@@ -570,7 +593,7 @@ cudaError_t launch_fp8_split(const Fp8GemmArgs& g, cudaStream_t s) {
   k.out_r = a_thin ? 1 : g.ldo;
   k.out_c = a_thin ? g.ldo : 1;
   k.wait_limit_ns = g.wait_limit_ns;
-  return launch(k, g.out_type, -1, g.K, (k.cols + 15) / 16 * 16, g.sms, s);
+  return launch(k, g.out_type, -1, g.K, plan, s);
 }
 
 cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
@@ -591,7 +614,9 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
   k.x_vec = x % 16 == 0 && (pitch % 16 == 0 || g.M == 1);
   k.x_wide = x % 32 == 0 && (pitch % 32 == 0 || g.M == 1);
   k.wait_limit_ns = g.wait_limit_ns;
-  return launch(k, a.x_type, a.x_type, g.K, (k.cols + 15) / 16 * 16, g.sms, s);
+  Plan plan;
+  const cudaError_t e = plan_tiles(g.N, g.M, (g.K + kBlock - 1) / kBlock, g.sms, &plan);
+  return e == cudaSuccess ? launch(k, a.x_type, a.x_type, g.K, plan, s) : e;
 }
 
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s) {
