@@ -247,18 +247,18 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     }
   } else if (warp == 2 || (warp == 3 && !FUSED)) {
     // Scale words for four blocks of k at a time, written to every stage that
-    // uses them; the next four's loads are issued first, but after these have
-    // arrived (a wait for some loads is one for all).  (Stages are counted,
+    // uses them; the next four's loads are issued once the first is handed over
+    // (a wait for some loads is one for all).  (Stages are counted,
     // not divided for: this warp's steps are near the pace of the copies.)
     const Fp8Operand& o = warp == 2 ? g.w : g.x;
     uint32_t now[4], par = 1;
     int s = 0;
     for (int kb = kb0; kb < kb1; kb++) {
-      if (kb == kb0 || (kb & 3) == 0) {
+      const bool first = kb == kb0 || (kb & 3) == 0;
+      if (first) {
 #pragma unroll
         for (int j = 0; j < 4; j++) now[j] = raw[j];
         finish_scales<1>(o, now);
-        if ((kb | 3) + 1 < kb1) gather((kb | 3) + 1);
       }
       if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
         *abort_flag = 1;
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       fence_async_shared();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sf_full[s]);
+      if (first && (kb | 3) + 1 < kb1) gather((kb | 3) + 1);
       if (++s == g.nst) {
         s = 0;
         par ^= 1;
