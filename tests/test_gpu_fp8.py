@@ -629,6 +629,53 @@ def test_traces_under_compile():
     assert torch.equal(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x))
 
 
+def test_training_step_traces_under_compile():
+    w = data(256, 384, BF, 2, 1).requires_grad_()
+    x = data(200, 384, BF, 1, 1).requires_grad_()
+    dy = data(200, 256, BF, 3, 1)
+    f = lambda x, w: torch.relu(fp64_emu.linear_fp8(x, w))  # noqa: E731
+    want = torch.autograd.grad(f(x, w), (x, w), dy)
+    got = torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True)(x, w), (x, w), dy)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_two_host_threads_at_once():
+    """Products, layers and backward passes from four threads, each on a stream of its own."""
+    import threading
+    w = data(512, 384, BF, 2, 1)
+    q, s = fp64_emu.quantize_fp8(w, "tile")
+    x = [data(m, 384, BF, 10 + m, 1) for m in (1, 17, 300, 700)]
+    want = [fp64_emu.linear_fp8(t, q, s) for t in x]
+    dy = [data(t.shape[0], 512, BF, 3, 1) for t in x]
+    grads = []
+    for t, d in zip(x, dy):
+        a, b = t.clone().requires_grad_(), w.clone().requires_grad_()
+        grads.append(torch.autograd.grad(fp64_emu.linear_fp8(a, b), (a, b), d))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    if not torch.equal(fp64_emu.linear_fp8(x[i], q, s), want[i]):
+                        wrong.append(i)
+                    a, b = x[i].clone().requires_grad_(), w.clone().requires_grad_()
+                    for g, h in zip(torch.autograd.grad(fp64_emu.linear_fp8(a, b), (a, b), dy[i]), grads[i]):
+                        if not torch.equal(g, h):
+                            wrong.append((i, "grad"))
+        except Exception as e:   # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong[:5]
+
+
 def test_layer_through_the_c_abi():
     """Few rows (one launch) and many (with a workspace), into a wider output whose other columns stay as they were."""
     import ctypes
