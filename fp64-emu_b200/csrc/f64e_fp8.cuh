@@ -378,8 +378,7 @@ enum : int { kWaitScales = 6, kWaitScalesFree = 7 };   // status sites, beside k
 // 4 j + 3 of k, a warp, in two steps: loads into raw[4 N] registers, none of
 // which depends on a branch or on another, and, when the atoms' place is free,
 // the atoms themselves.  Taken one word after the other the scales, not the
-// MMAs, set the pace of a product (4096 x 4096 x 8192 with column scales on
-// both sides: 231 us instead of 125).  Rows and blocks outside the operand read
+// MMAs, set the pace of a product with column scales on both sides.  Rows and blocks outside the operand read
 // a neighbour's scale: their codes are zeros, and no store uses them.
 //   kScaleWords  four blocks' scales are one aligned word
 //   kScaleRows   four rows' scales are one aligned word (column blocks)
