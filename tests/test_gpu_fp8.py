@@ -439,6 +439,26 @@ def test_layer_with_kept_weights(dtype, M):
             R.check_product(fp64_emu.linear_fp8(xs, q, s), *layer_reference(xs, w))
 
 
+@pytest.mark.parametrize("M", [1, 5, 16, 17, 70])
+def test_layer_with_kept_weights_stored_otherwise(M):
+    for N, K in ((300, 520), (1000, 2100), (129, 257)):
+        w, x = data(N, K, BF, 2, 1), data(M, K, BF, 1, 1)
+        q, s = fp64_emu.quantize_fp8(w, "tile")
+        nb, kb = s.shape
+        by_columns = torch.empty(K, (N + 15) // 16 * 16, dtype=torch.uint8, device="cuda")[:, :N].t()
+        odd = torch.empty(N, K + 3, dtype=torch.uint8, device="cuda")[:, 3:]
+        for store in (by_columns, odd):
+            store.copy_(q.view(torch.uint8))
+        scales = torch.empty(kb, 2 * nb, dtype=torch.uint8, device="cuda")[:, ::2].t()
+        scales.copy_(s.view(torch.uint8))
+        assert scales.stride() == (2, 2 * nb)
+        want = layer_reference(x, w)
+        for codes in (by_columns, odd):
+            for sc in (s, scales.view(s.dtype)):
+                y = fp64_emu.linear_fp8(x, codes.view(q.dtype), sc)
+                R.check_product(y, *want)
+
+
 def test_layer_with_kept_weights_special_values():
     w = data(300, 520, BF, 2, 1)
     q, s = fp64_emu.quantize_fp8(w, "tile")
