@@ -43,6 +43,11 @@ const char* check_codes(const void* q, int64_t ldq, int64_t cols) {
   return nullptr;
 }
 
+// Kernels read and write whole elements: an address inside one would fault.
+const char* check_elements(const void* x, int type) {
+  return reinterpret_cast<uintptr_t>(x) % (type == F64E_F32 ? 4 : 2) ? "fp8: values are not aligned to their type" : nullptr;
+}
+
 // Sizes, types and pitches of a product; fills everything but the pointers.
 int check_problem(const f64e_fp8_problem* p, Fp8GemmArgs* g) {
   if (!p) return bad("fp8: null problem");
@@ -89,6 +94,7 @@ int f64e_fp8_quantize(const void* x, int32_t x_type, int64_t rows, int64_t cols,
   if (rows == 0 || cols == 0) return F64E_OK;
   if (!x || !q || !scale) return bad("fp8: null pointer");
   if (ldx < cols) return bad("fp8: row pitch of x is below its columns");
+  if (const char* m = check_elements(x, x_type)) return bad(m);
   if (const char* m = check_codes(q, ldq, cols)) return bad(m);
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
@@ -122,6 +128,7 @@ int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows, int64_t 
   if (rows == 0 || cols == 0) return F64E_OK;
   if (!x || !q_row || !scale_row || !q_col || !scale_col) return bad("fp8: null pointer");
   if (ldx < cols) return bad("fp8: row pitch of x is below its columns");
+  if (const char* m = check_elements(x, x_type)) return bad(m);
   if (const char* m = check_codes(q_row, ldq, cols)) return bad(m);
   if (transposed != 0 && transposed != 1) return bad("fp8: transposed must be 0 or 1");
   if (const char* m = check_codes(q_col, ld_col, transposed ? rows : cols)) return bad(m);
@@ -154,6 +161,7 @@ int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int64_t cols,
   if (rows == 0 || cols == 0) return F64E_OK;
   if (!q || !scale || !out) return bad("fp8: null pointer");
   if (ldq < cols) return bad("fp8: row pitch of the codes is below their columns");
+  if (const char* m = check_elements(out, out_type)) return bad(m);
   int sms = 0;
   if (const int rc = device_sms(&sms)) return rc;
   Fp8DequantArgs a{};
@@ -187,6 +195,7 @@ int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale,
   if (!A || !a_scale || !B || !b_scale || !out) return bad("fp8: null pointer");
   if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15))
     return bad("fp8: codes need 16-byte aligned rows");
+  if (const char* m = check_elements(out, p->out_type)) return bad(m);
   g.a.q = static_cast<const uint8_t*>(A);
   g.a.s = static_cast<const uint8_t*>(a_scale);
   g.b.q = static_cast<const uint8_t*>(B);
@@ -230,6 +239,8 @@ int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const
   if (q.K == 0) return bad("fp8: K must be at least 1");
   if (!x || !w || !w_scale || !out) return bad("fp8: null pointer");
   if (reinterpret_cast<uintptr_t>(w) & 15) return bad("fp8: codes need 16-byte aligned rows");
+  for (const void* v : {x, static_cast<const void*>(out)})
+    if (const char* m = check_elements(v, q.out_type)) return bad(m);
   if (q.M > kFusedRows) {
     const size_t need = f64e_fp8_linear_workspace_size(q.M, q.K);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))

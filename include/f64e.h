@@ -235,7 +235,8 @@ F64E_API int f64e_mm_nt_noalloc(double* out, const double* A, const double* Bt, 
  * in e5m2; e = 0 for a block of zeros), stored as the byte e + 127.  A code is
  * the round-to-nearest-even 8-bit float of x * 2^-e; NaN stays NaN, and
  * infinity becomes NaN; neither counts towards amax.  Rows of codes start on
- * 16-byte boundaries (pitch a multiple of 16).  Nothing here allocates or
+ * 16-byte boundaries (pitch a multiple of 16); values are aligned to their
+ * type (an address inside an element is refused).  Nothing here allocates or
  * synchronizes, except f64e_fp8_status. */
 enum { F64E_F32 = 0, F64E_F16 = 1, F64E_BF16 = 2 }; /* element types */
 enum { F64E_E4M3 = 0, F64E_E5M2 = 1 };              /* codes */

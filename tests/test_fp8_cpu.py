@@ -247,3 +247,18 @@ def test_fake_kernels_give_shapes_and_types():
         assert fp64_emu.mm_fp8(q, q, s, s).shape == (200, 200)
         assert fp64_emu.mm_tn_fp8(qc, qc, sc, sc, torch.float32).shape == (300, 300)
         assert fp64_emu.linear_fp8(torch.empty(2, 7, 300, device="cuda"), x.float()).shape == (2, 7, 200)
+
+
+@pytest.mark.parametrize("kind,off", [(0, 1), (0, 2), (1, 1), (2, 1)])
+def test_c_abi_refuses_addresses_inside_an_element(lib, kind, off):
+    """kind: F64E_F32, F64E_F16, F64E_BF16.  Refused on the host: no device is asked."""
+    bad = P + off
+    p = Problem(64, 64, 256, kind, 64, Operand(256, 0, 0, 1, 2, 1), Operand(256, 0, 1, 1, 2, 1))
+    calls = (lambda: lib.f64e_fp8_quantize(bad, kind, 64, 256, 256, 0, 0, P, 256, P, None),
+             lambda: lib.f64e_fp8_quantize_both(bad, kind, 64, 256, 256, 0, P, P, 256, P, P, 0, 256, None),
+             lambda: lib.f64e_fp8_dequantize(P, 0, 64, 256, 256, 0, P, 2, 1, bad, kind, None),
+             lambda: lib.f64e_fp8_gemm(ctypes.byref(p), P, P, P, P, bad, None, 0, None),
+             lambda: lib.f64e_fp8_linear(ctypes.byref(p), bad, 256, P, P, P, P, 1 << 30, None),
+             lambda: lib.f64e_fp8_linear(ctypes.byref(p), P, 256, P, P, bad, P, 1 << 30, None))
+    for call in calls:
+        assert call() == 1 and b"not aligned to their type" in lib.f64e_last_error()
