@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   // TMEM: allocated by both CTAs once both run, the permit given up at the end
   // (see residue_gemm_pair_kernel).
   const bool uses_tmem = warp == 1 || warp >= 4;
+  __syncwarp();
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, TMEM_COLS);
     tc_fence_before();
@@ -577,9 +578,9 @@ __global__ void __launch_bounds__(PTHREADS, 1)
     if (lane == 0) tma_store_wait();   // shared memory outlives the stores
   }
 
-  __syncwarp();
   if (!uses_tmem) cluster_wait();   // the allocation's barrier
   tc_fence_before();
+  __syncwarp();
   cluster_sync();   // the leader's MMAs have drained; the peer's stage count is visible
   if (!*all_done) {
     // A wait ran out.  Every copy of the pair lands before either CTA releases

@@ -434,6 +434,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       }
     }
   }
+  __syncwarp();   // the loop's trips differ by lane, and the barrier is one for whole warps
   if (g.split > 1) cluster_sync();   // the peers have read this CTA's sums
 }
 

@@ -262,3 +262,24 @@ def test_c_abi_refuses_addresses_inside_an_element(lib, kind, off):
              lambda: lib.f64e_fp8_linear(ctypes.byref(p), P, 256, P, P, bad, P, 1 << 30, None))
     for call in calls:
         assert call() == 1 and b"not aligned to their type" in lib.f64e_last_error()
+
+
+# ---------------------------------------------------------------- sources --
+def source(name):
+    """A kernel source without its comments."""
+    import re
+    with open(os.path.join(ROOT, "fp64-emu_b200", "csrc", name)) as f:
+        return re.sub(r"//[^\n]*", "", f.read())
+
+
+@pytest.mark.parametrize("name", ["f64e_fp8_gemm.cu", "f64e_fp8_split.cu"])
+def test_whole_warp_barriers_follow_a_warp_barrier(name):
+    """cluster_sync and the TMEM allocation are .aligned: all lanes of a warp execute them together.  Loops, waits and
+    branches before them may have parted the lanes, so nothing but a condition stands between __syncwarp and them."""
+    import re
+    text = source(name)
+    calls = list(re.finditer(r"\b(cluster_sync|tmem_alloc|tmem_alloc_pair)\(", text))
+    assert len(calls) >= 3
+    for m in calls:
+        assert re.search(r"__syncwarp\(\);\s*(if \((?:[^(){};]|\([^(){};]*\))*\)\s*\{?\s*)?$", text[:m.start()]), \
+            text[max(0, m.start() - 200):m.end()]
