@@ -260,6 +260,12 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, u
     }
   }
 }
+// What a wait gave, for the whole warp: true where all of its lanes have what
+// they waited for.  A lane that gives up, or reads the abort flag a moment
+// later than its neighbours, must not part from them: tcgen05 loads, barriers
+// and __syncwarp behind the wait need all 32.  Every wait that is not one
+// elected thread's goes through it.
+__device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xFFFFFFFFu, ok) != 0; }
 
 // 128 x 128-byte box of a 2-D map at (x, y): x along the contiguous direction.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {

@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         left = per;
       }
       left--;
-      if (!mbar_wait_poll(&sf_full[s], ph, lim, status, kWaitScales) ||
-          !mbar_wait_poll(&full[s], ph, lim, status, kWaitFull)) {
+      if (!warp_all(mbar_wait_poll(&sf_full[s], ph, lim, status, kWaitScales) &&
+                    mbar_wait_poll(&full[s], ph, lim, status, kWaitFull))) {
         ok = false;
         break;
       }
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         for (int j = 0; j < 4; j++) now[j] = raw[j];
         finish_scales<1>(o, now);
       }
-      if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
+      if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) && !*abort_flag)) {
         *abort_flag = 1;
         break;
       }
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
           scale[p] = (uint8_t)(e + 127);
         }
         if (i + QW < n) load_x(i + QW);
-        if (!mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) || *abort_flag) {
+        if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) && !*abort_flag)) {
           *abort_flag = 1;
           break;
         }
@@ -330,7 +330,8 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     }
     // Partial sums to shared memory, by columns of 128 rows; the stages are free:
     // every MMA has completed.
-    const bool done = warp < 8 && mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag;
+    const bool done =
+        warp < 8 && warp_all(mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag);
     if (done) {
       tc_fence_after();
       const int q = warp & 3;

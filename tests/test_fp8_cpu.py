@@ -283,3 +283,38 @@ def test_whole_warp_barriers_follow_a_warp_barrier(name):
     for m in calls:
         assert re.search(r"__syncwarp\(\);\s*(if \((?:[^(){};]|\([^(){};]*\))*\)\s*\{?\s*)?$", text[:m.start()]), \
             text[max(0, m.start() - 200):m.end()]
+
+
+def enclosing(text, at):
+    """What stands before each of the blocks that hold position `at`, innermost first."""
+    heads, depth = [], 0
+    for i in range(at - 1, -1, -1):
+        if text[i] == "}":
+            depth += 1
+        elif text[i] == "{":
+            if depth:
+                depth -= 1
+            else:
+                heads.append(text[max(text.rfind(c, 0, i) for c in ";{}") + 1:i])
+    return heads
+
+
+@pytest.mark.parametrize("name", ["f64e_fp8_gemm.cu", "f64e_fp8_split.cu"])
+def test_a_warp_that_waits_decides_as_one(name):
+    """A bounded wait either belongs to one elected thread or its outcome is agreed on by the warp: lanes that parted
+    when it runs out would reach the aligned instructions behind it in parts."""
+    import re
+    text = source(name)
+    waits = [m.start() for m in re.finditer(r"\bmbar_wait_poll\b", text)]
+    assert len(waits) >= 6
+    for at in waits:
+        statement = text[max(text.rfind(c, 0, at) for c in ";{}"):at]
+        one_thread = any(re.search(r"if \((producer\b|issuer\b|elect_one\(\))", h) for h in enclosing(text, at))
+        assert one_thread or "warp_all(" in statement, text[max(0, at - 200):at + 80]
+    # and so is the abort flag: read with a wait's outcome, by an elected thread, or behind the CTA's last barrier
+    for m in re.finditer(r"[!|& (]\*abort_flag\b(?! =)", text):
+        statement = text[max(text.rfind(c, 0, m.start()) for c in ";{}"):m.start()]
+        one_thread = any(re.search(r"if \((producer\b|issuer\b|elect_one\(\))", h) for h in enclosing(text, m.start()))
+        behind = text.rfind("cluster_sync", 0, m.start()) > text.rfind("mbar_wait_poll", 0, m.start())
+        if "volatile int" not in statement:
+            assert one_thread or behind or "warp_all(" in statement, text[max(0, m.start() - 200):m.end()]
