@@ -405,7 +405,6 @@ __global__ void __launch_bounds__(PTHREADS, 1)
                   mma_mx_pair(d_tmem, da + kk * a_step, db + kk * b_step, id, sf, sf + 4, 1);
                 tc_commit_pair(&empty_bar[s], 0x3);
               }
-              __syncwarp();
               accumulate = 1;
               if (++s == STAGES) {
                 s = 0;

@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         for (int kk = 1; kk < kBlock / 32; kk++) mma_mx(d_tmem, dw + kk * w_step, dx + kk * 2, id, sfa, sfa + 4, 1);
         tc_commit(&empty[s]);
       }
-      __syncwarp();
       accumulate = 1;
       if (++s == g.nst) {
         s = 0;
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         for (int j = 0; j < 4; j++) now[j] = raw[j];
         finish_scales<1>(o, now);
       }
-      if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) && !*abort_flag)) {
+      if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree))) {
         *abort_flag = 1;
         break;
       }
@@ -309,7 +308,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
           scale[p] = (uint8_t)(e + 127);
         }
         if (i + QW < n) load_x(i + QW);
-        if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree) && !*abort_flag)) {
+        if (!warp_all(mbar_wait_poll(&empty[s], par, lim, status, kWaitScalesFree))) {
           *abort_flag = 1;
           break;
         }
