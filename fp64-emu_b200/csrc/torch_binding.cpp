@@ -10,6 +10,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -680,7 +681,16 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   }
 };
 
+// A tangent would be lost below this kernel: the result would count as a constant.
+void fp8_check_no_tangent(const at::Tensor& t) {
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), "linear_fp8 has no forward-mode derivative");
+}
+
 at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode()) {
+    fp8_check_no_tangent(x);
+    fp8_check_no_tangent(w);
+  }
   if (at::GradMode::is_enabled() && (x.requires_grad() || (w.requires_grad() && !ws.has_value()))) {
     fp8_check_linear(x, w, ws);
     return Fp8Linear::apply(x, w, ws);

@@ -84,7 +84,8 @@ def linear_fp8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor = None) -
     gradient x is kept in 8 bits, with blocks along its rows (the tokens):
     one byte a value instead of x itself.  With gradients dy quantised in row
     blocks and in column blocks,
-        dx = q_row(dy) @ q_tile(w),    dw = q_col(dy)^T @ q_col(x)."""
+        dx = q_row(dy) @ q_tile(w),    dw = q_col(dy)^T @ q_col(x).
+    There is no second derivative and no forward mode: both are refused."""
     return _linear(x, w, w_scale)
 
 

@@ -318,3 +318,28 @@ def test_a_warp_that_waits_decides_as_one(name):
         behind = text.rfind("cluster_sync", 0, m.start()) > text.rfind("mbar_wait_poll", 0, m.start())
         if "volatile int" not in statement:
             assert one_thread or behind or "warp_all(" in statement, text[max(0, m.start() - 200):m.end()]
+
+
+# ----------------------------------------------------------- derivatives --
+@pytest.mark.parametrize("which", ["x", "w", "both"])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_layer_refuses_forward_mode(which, requires_grad):
+    """A tangent is refused, not dropped, whether or not the input requires grad too, and without reverse mode on."""
+    import torch.autograd.forward_ad as fw
+    x, w = torch.ones(2, 4, requires_grad=requires_grad), torch.ones(3, 4, requires_grad=requires_grad)
+    with fw.dual_level():
+        a = fw.make_dual(x, torch.ones(2, 4)) if which != "w" else x
+        b = fw.make_dual(w, torch.ones(3, 4)) if which != "x" else w
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                fp64_emu.linear_fp8(a, b)
+    if not requires_grad and which != "both":
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(lambda t: fp64_emu.linear_fp8(*((t, w) if which == "x" else (x, t))),
+                           (x if which == "x" else w,), (torch.ones_like(x if which == "x" else w),))
+
+
+def test_layer_refuses_forward_mode_beside_kept_weights():
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        fp64_emu.linear_fp8(fw.make_dual(torch.ones(2, 4), torch.ones(2, 4)), codes(3, 4), scales(1, 1))
