@@ -554,7 +554,6 @@ void fp8_check_linear(const at::Tensor& x, const at::Tensor& w, const std::optio
   } else {
     fp8_check_float(w, "w");
   }
-  fp8_check_cuda(x, "x");
   TORCH_CHECK(w.device() == x.device() && (!ws.has_value() || ws->device() == x.device()),
               "x, w and its scales must be on one device");
 }
@@ -566,6 +565,7 @@ std::vector<int64_t> fp8_out_sizes(const at::Tensor& x, int64_t n) {
 
 at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
   fp8_check_linear(x, w, ws);
+  fp8_check_cuda(x, "x");
   const c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor xr = fp8_rows(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}));
   at::Tensor wq, wsc;
@@ -692,7 +692,7 @@ at::Tensor fp8_linear_autograd(const at::Tensor& x, const at::Tensor& w, const s
     fp8_check_no_tangent(w);
   }
   if (at::GradMode::is_enabled() && (x.requires_grad() || (w.requires_grad() && !ws.has_value()))) {
-    fp8_check_linear(x, w, ws);
+    fp8_check_linear(x, w, ws);   // the device is asked for by the operators it calls: shapes alone (meta) pass
     return Fp8Linear::apply(x, w, ws);
   }
   at::AutoDispatchBelowADInplaceOrView below;

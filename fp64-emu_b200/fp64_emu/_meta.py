@@ -63,4 +63,6 @@ def _fake_fp8_mm(a, b, sa, sb, layout, dtype):
 
 @torch.library.register_fake("fp64_emu_b200::fp8_linear")
 def _fake_linear(x, w, ws=None):
+    torch._check(w.device == x.device and (ws is None or ws.device == x.device),
+                 lambda: "x, w and its scales must be on one device")
     return torch.empty((*x.shape[:-1], w.shape[0]), dtype=x.dtype, device=x.device)

@@ -343,3 +343,28 @@ def test_layer_refuses_forward_mode_beside_kept_weights():
     import torch.autograd.forward_ad as fw
     with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         fp64_emu.linear_fp8(fw.make_dual(torch.ones(2, 4), torch.ones(2, 4)), codes(3, 4), scales(1, 1))
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("shape", [(40, 300), (5, 8, 300), (300,)])
+def test_layer_and_gradients_on_meta_tensors(shape, kept):
+    """Shapes and types of the output and the gradients without a device, as without gradients."""
+    x = torch.empty(shape, dtype=torch.bfloat16, device="meta", requires_grad=True)
+    if kept:
+        w, s = torch.empty(200, 300, dtype=E4, device="meta"), torch.empty(2, 3, dtype=E8, device="meta")
+    else:
+        w, s = torch.empty(200, 300, device="meta", requires_grad=True), None
+    with torch.no_grad():
+        assert fp64_emu.linear_fp8(x, w, s).shape == (*shape[:-1], 200)
+    y = fp64_emu.linear_fp8(x, w, s)
+    assert y.shape == (*shape[:-1], 200) and y.dtype == torch.bfloat16 and y.requires_grad
+    wanted = (x,) if kept else (x, w)
+    for t, g in zip(wanted, torch.autograd.grad(y, wanted, torch.empty_like(y))):
+        assert g.shape == t.shape and g.dtype == t.dtype and g.is_meta
+
+
+def test_layer_on_two_devices_is_refused():
+    for grad in (False, True):
+        x = torch.zeros(2, 4, requires_grad=grad)
+        with pytest.raises(RuntimeError, match="on one device"):
+            fp64_emu.linear_fp8(x, torch.zeros(3, 4, device="meta"))
