@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -650,8 +651,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()),
-                "linear_fp8 has no second derivative");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()), kNoSecond);
     at::AutoDispatchBelowADInplaceOrView below;
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &wq = saved[0], &wsc = saved[1], &qc = saved[2], &sc = saved[3];
@@ -677,7 +677,18 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
                            : at::zeros({g.size(1), qc.size(1)}, g.options().dtype(wt));
       }
     }
-    return {dx, dw, at::Tensor()};
+    return {once(dx), once(dw), at::Tensor()};
+  }
+
+ private:
+  static constexpr const char* kNoSecond = "linear_fp8 has no second derivative";
+  // Where a graph of the backward pass is asked for (create_graph): dx depends
+  // on w and dw on x, so a gradient is not a constant, and differentiating it
+  // ends with an error instead of leaving it out.
+  static at::Tensor once(at::Tensor grad) {
+    if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
+    grad.set_requires_grad(true);
+    return torch::autograd::DelayedError(kNoSecond, 1).apply({grad})[0];
   }
 };
 

@@ -368,3 +368,32 @@ def test_layer_on_two_devices_is_refused():
         x = torch.zeros(2, 4, requires_grad=grad)
         with pytest.raises(RuntimeError, match="on one device"):
             fp64_emu.linear_fp8(x, torch.zeros(3, 4, device="meta"))
+
+
+def meta_layer(kept=False):
+    x = torch.empty(6, 40, device="meta", requires_grad=True)
+    if kept:
+        return x, torch.empty(20, 40, dtype=E4, device="meta"), torch.empty(1, 1, dtype=E8, device="meta")
+    return x, torch.empty(20, 40, device="meta", requires_grad=True), None
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_layer_second_derivative_is_refused_not_left_out(kept):
+    """A gradient taken with create_graph depends on the inputs: differentiating it, alone or beside the loss, is
+    refused, also where the output's gradient is a constant."""
+    x, w, s = meta_layer(kept)
+    y = fp64_emu.linear_fp8(x, w, s)
+    grads = torch.autograd.grad(y, (x,) if kept else (x, w), torch.empty_like(y), create_graph=True)
+    for g in grads:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (g * g).sum().backward(retain_graph=True)
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            (y.sum() + (g * g).sum()).backward(retain_graph=True)
+
+
+def test_layer_first_derivative_under_create_graph():
+    x, w, _ = meta_layer()
+    fp64_emu.linear_fp8(x, w).sum().backward(create_graph=True)
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape
+    dx, = torch.autograd.grad(fp64_emu.linear_fp8(x, w).sum(), x)
+    assert not dx.requires_grad
