@@ -380,6 +380,7 @@ int fp8_code(at::ScalarType t) {
 // Shapes of a product's operands: A [M, K] B [N, K], A [M, K] B [K, N], A [K, M] B [K, N].
 enum { kFp8NT = 0, kFp8NN = 1, kFp8TN = 2 };
 int64_t fp8_blocks(int64_t n) { return (n + 127) / 128; }
+c10::SymInt fp8_blocks(const c10::SymInt& n) { return (n + 127) / 128; }
 
 void fp8_check_float(const at::Tensor& x, const char* what) {
   TORCH_CHECK(fp8_type(x.scalar_type()) >= 0, what, " must be float32, float16 or bfloat16");
@@ -473,9 +474,9 @@ void fp8_check_operand(const at::Tensor& q, const at::Tensor& s, int kdim, const
   TORCH_CHECK(q.dim() == 2 && s.dim() == 2, name, ": codes and scales must be matrices");
   TORCH_CHECK(fp8_code(q.scalar_type()) >= 0, name, ": codes must be float8_e4m3fn or float8_e5m2");
   TORCH_CHECK(s.scalar_type() == at::kFloat8_e8m0fnu, name, ": scales must be float8_e8m0fnu (powers of two)");
-  const int64_t r = q.size(1 - kdim), k = q.size(kdim), sr = s.size(1 - kdim), sk = s.size(kdim);
-  TORCH_CHECK(sk == fp8_blocks(k) && (sr == r || sr == fp8_blocks(r)), name, ": scales of shape ", s.sizes(),
-              " do not fit codes of shape ", q.sizes(), " with blocks of 128 along the contracted dimension");
+  const c10::SymInt r = q.sym_size(1 - kdim), k = q.sym_size(kdim), sr = s.sym_size(1 - kdim), sk = s.sym_size(kdim);
+  TORCH_CHECK(sk == fp8_blocks(k) && (sr == r || sr == fp8_blocks(r)), name, ": scales of shape ", s.sym_sizes(),
+              " do not fit codes of shape ", q.sym_sizes(), " with blocks of 128 along the contracted dimension");
 }
 // Whether the rows of the stored codes start on 16-byte boundaries, with
 // `fast` the contiguous dimension.
@@ -544,14 +545,17 @@ int64_t fp8_status(int64_t device) {
 }
 
 // ---- a layer held in 8 bits ----
+// Sizes are read as symbols wherever the layer's autograd kernel comes by: it
+// also runs while a compiler traces it, and a number read there would tie the
+// traced program to the batch size at hand.
 void fp8_check_linear(const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& ws) {
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 2, "x must have at least one dimension and w two");
   fp8_check_float(x, "x");
-  TORCH_CHECK(x.size(-1) == w.size(1), "x's last dimension and w's differ");
-  TORCH_CHECK(w.size(0) >= 1 && w.size(1) >= 1, "w must not be empty");
+  TORCH_CHECK(x.sym_size(-1) == w.sym_size(1), "x's last dimension and w's differ");
+  TORCH_CHECK(w.sym_size(0) >= 1 && w.sym_size(1) >= 1, "w must not be empty");
   if (ws.has_value()) {
     fp8_check_operand(w, *ws, 1, "w");
-    TORCH_CHECK(ws->size(0) == fp8_blocks(w.size(0)), "w: kept weights need one scale per 128 x 128 square");
+    TORCH_CHECK(ws->sym_size(0) == fp8_blocks(w.sym_size(0)), "w: kept weights need one scale per 128 x 128 square");
   } else {
     fp8_check_float(w, "w");
   }
@@ -626,11 +630,22 @@ at::Tensor call_linear(const at::Tensor& x, const at::Tensor& w, const std::opti
   return op.call(x, w, ws);
 }
 
+// x [..., K] as a matrix, and rows [n, N] with x's leading dimensions.
+at::Tensor fp8_matrix(const at::Tensor& x) {
+  return x.dim() == 2 ? x : x.reshape_symint({c10::SymInt(-1), x.sym_size(-1)});
+}
+at::Tensor fp8_shaped_like(const at::Tensor& rows, const at::Tensor& x) {
+  if (x.dim() == 2) return rows;
+  std::vector<c10::SymInt> v = x.sym_sizes().vec();
+  v.back() = rows.sym_size(1);
+  return rows.view_symint(v);
+}
+
 struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const std::optional<at::Tensor>& ws) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+    const at::Tensor x2 = fp8_matrix(x);
     const bool want_w = w.requires_grad() && !ws.has_value();
     at::Tensor q, s, qc, sc, wq = w, wsc;
     if (want_w)
@@ -644,10 +659,9 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     at::Tensor y = call_mm(q, wq, s, wsc, kFp8NT, x.scalar_type());
     const bool want_x = x.requires_grad();
     ctx->save_for_backward({want_x ? wq : at::Tensor(), want_x ? wsc : at::Tensor(), qc, sc});
-    ctx->saved_data["x_sizes"] = x.sizes().vec();
     ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
     ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
-    return x.dim() == 2 ? y : y.view(fp8_out_sizes(x, w.size(0)));
+    return fp8_shaped_like(y, x);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
@@ -658,7 +672,7 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
     const bool want_x = wq.defined(), want_w = qc.defined();
     at::Tensor dx, dw;
     if (grads[0].defined() && (want_x || want_w)) {
-      const at::Tensor g = grads[0].dim() == 2 ? grads[0] : grads[0].reshape({-1, grads[0].size(-1)});
+      const at::Tensor g = fp8_matrix(grads[0]);
       at::Tensor q, s, gc, gsc;
       if (want_x && want_w)
         std::tie(q, s, gc, gsc) = call_quantize_both(g, true);
@@ -668,13 +682,13 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
         std::tie(gc, gsc) = call_quantize(g, F64E_BLOCKS_COL);
       if (want_x) {
         dx = call_mm(q, wq, s, wsc, kFp8NN, (at::ScalarType)ctx->saved_data["x_type"].toInt());
-        const auto sizes = ctx->saved_data["x_sizes"].toIntVector();
-        if (sizes.size() != 2) dx = dx.view(sizes);
+        dx = fp8_shaped_like(dx, grads[0]);
       }
       if (want_w) {
         const auto wt = (at::ScalarType)ctx->saved_data["w_type"].toInt();
-        dw = g.size(0) > 0 ? call_mm(gc, qc, gsc, sc, kFp8TN, wt)
-                           : at::zeros({g.size(1), qc.size(1)}, g.options().dtype(wt));
+        dw = TORCH_GUARD_OR_TRUE(g.sym_size(0).sym_gt(0))
+                 ? call_mm(gc, qc, gsc, sc, kFp8TN, wt)
+                 : at::zeros_symint({g.sym_size(1), qc.sym_size(1)}, g.options().dtype(wt));
       }
     }
     return {once(dx), once(dw), at::Tensor()};

@@ -397,3 +397,35 @@ def test_layer_first_derivative_under_create_graph():
     assert x.grad.shape == x.shape and w.grad.shape == w.shape
     dx, = torch.autograd.grad(fp64_emu.linear_fp8(x, w).sum(), x)
     assert not dx.requires_grad
+
+
+def symbolic(shape, dynamic, dtype=torch.float32):
+    """A fake tensor that requires grad, the dimensions in `dynamic` symbolic, and its shape environment."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
+    env = ShapeEnv()
+    mode = FakeTensorMode(shape_env=env)
+    x = mode.from_tensor(torch.empty(shape, dtype=dtype), symbolic_context=StatelessSymbolicContext(
+        dynamic_sizes=[DimDynamic.DYNAMIC if d in dynamic else DimDynamic.STATIC for d in range(len(shape))]))
+    return x.requires_grad_(), mode, env
+
+
+@pytest.mark.parametrize("shape,dynamic", [((20, 384), (0,)), ((4, 20, 384), (1,)), ((4, 20, 384), (0, 1))])
+@pytest.mark.parametrize("kept", [False, True])
+def test_layer_and_gradients_keep_dynamic_dimensions(shape, dynamic, kept):
+    """Tracing with a batch size left open: no guard ties it to the size at hand, in either direction."""
+    x, mode, env = symbolic(shape, dynamic)
+    with mode:
+        if kept:
+            w, s = torch.empty(256, 384, dtype=E4), torch.empty(2, 3, dtype=E8)
+        else:
+            w, s = torch.empty(256, 384, requires_grad=True), None
+        y = fp64_emu.linear_fp8(x, w, s)
+        wanted = (x,) if kept else (x, w)
+        grads = torch.autograd.grad(y, wanted, torch.empty_like(y))
+    for d in dynamic:
+        assert isinstance(y.shape[d], torch.SymInt) and isinstance(grads[0].shape[d], torch.SymInt)
+        assert y.shape[d].node.expr == x.shape[d].node.expr == grads[0].shape[d].node.expr
+    assert [g.shape for g in grads] == [t.shape for t in wanted]
+    assert y.shape[-1] == 256
+    assert not env.guards, env.guards

@@ -807,3 +807,32 @@ except RuntimeError as e:
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-1500:]
     assert "replayed" in r.stdout or (alive and "refused" in r.stdout), r.stdout
+
+
+def test_training_step_compiled_for_any_batch():
+    """One traced program for all batch sizes: a dimension marked dynamic stays so, values and gradients are the eager ones."""
+    w = data(256, 384, BF, 2, 1).requires_grad_()
+    f = lambda x, w: torch.relu(fp64_emu.linear_fp8(x, w))  # noqa: E731
+    traced = torch.compile(f, backend="aot_eager", fullgraph=True)
+    for shape in ((200, 384), (33, 384), (1021, 384)):
+        x = data(*shape, BF, 1, 1).requires_grad_()
+        dy = data(shape[0], 256, BF, 3, 1)
+        torch._dynamo.mark_dynamic(x, 0)
+        y, want = traced(x, w), f(x, w)
+        assert torch.equal(y, want)
+        for got, right in zip(torch.autograd.grad(y, (x, w), dy), torch.autograd.grad(want, (x, w), dy)):
+            assert torch.equal(got, right)
+
+
+def test_layer_refuses_tangents_and_second_derivatives():
+    import torch.autograd.forward_ad as fw
+    x, w = data(20, 384, BF, 1, 1), data(256, 384, BF, 2, 1)
+    with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        fp64_emu.linear_fp8(fw.make_dual(x, torch.ones_like(x)), w)
+    x.requires_grad_()
+    y = fp64_emu.linear_fp8(x, w)
+    plain, = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    assert torch.equal(dx.detach(), plain)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        (y.float().sum() + (dx.float() ** 2).sum()).backward()
