@@ -217,8 +217,8 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         left = per;
       }
       left--;
-      if (!warp_all(mbar_wait_poll(&sf_full[s], ph, lim, status, kWaitScales) &&
-                    mbar_wait_poll(&full[s], ph, lim, status, kWaitFull))) {
+      if (!mbar_wait_lane(&sf_full[s], ph, lim, status, kWaitScales) ||
+          !mbar_wait_lane(&full[s], ph, lim, status, kWaitFull)) {
         ok = false;
         break;
       }
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         ph ^= 1;
       }
     }
-    if (!ok) *abort_flag = 1;
+    if (!warp_all(ok)) *abort_flag = 1;
     if (issuer) {
       tc_commit(acc_full);   // every MMA issued has completed when it arrives
       mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitDrain);

@@ -295,7 +295,11 @@ def enclosing(text, at):
             if depth:
                 depth -= 1
             else:
-                heads.append(text[max(text.rfind(c, 0, i) for c in ";{}") + 1:i])
+                j, parens = i, 0
+                while j > 0 and (parens or text[j - 1] not in ";{}"):
+                    j -= 1
+                    parens += {")": 1, "(": -1}.get(text[j], 0)
+                heads.append(text[j:i])
     return heads
 
 
@@ -306,7 +310,20 @@ def test_a_warp_that_waits_decides_as_one(name):
     import re
     text = source(name)
     waits = [m.start() for m in re.finditer(r"\bmbar_wait_poll\b", text)]
-    assert len(waits) >= 6
+    lanes = [m.start() for m in re.finditer(r"\bmbar_wait_lane\b", text)]
+    assert len(waits) >= 6 and len(lanes) >= 2
+    for at in lanes:
+        # a loop without an instruction for whole warps, whose lanes agree behind it
+        loop = [h for h in enclosing(text, at) if re.search(r"\bfor \(", h)][-1]
+        start = text.rfind(loop, 0, at) + len(loop)
+        depth, end = 0, start
+        while True:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+            if depth == 0:
+                break
+        assert not re.search(r"_sync\(|__syncwarp|cluster_arrive|cluster_wait|tmem_|elect_one|warp_all", text[start:end])
+        assert re.match(r"\s*(ok = warp_all\(ok\)|if \(!warp_all\(ok\)\))", text[end:]), text[end:end + 80]
     for at in waits:
         statement = text[max(text.rfind(c, 0, at) for c in ";{}"):at]
         one_thread = any(re.search(r"if \((producer\b|issuer\b|elect_one\(\))", h) for h in enclosing(text, at))
