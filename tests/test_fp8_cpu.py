@@ -334,7 +334,7 @@ def test_a_warp_that_waits_decides_as_one(name):
         one_thread = any(re.search(r"if \((producer\b|issuer\b|elect_one\(\))", h) for h in enclosing(text, m.start()))
         behind = text.rfind("cluster_sync", 0, m.start()) > text.rfind("mbar_wait_poll", 0, m.start())
         if "volatile int" not in statement:
-            assert one_thread or behind or "warp_all(" in statement, text[max(0, m.start() - 200):m.end()]
+            assert one_thread or behind or "warp_all(" in statement or "mbar_wait_lane(" in statement, text[max(0, m.start() - 200):m.end()]
 
 
 # ----------------------------------------------------------- derivatives --
