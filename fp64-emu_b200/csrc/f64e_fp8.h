@@ -94,9 +94,11 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
 // Launches it unless the estimate of its cycles exceeds other_cost, or the
 // smaller operand is not K-major; done says which.
 cudaError_t launch_fp8_split(const Fp8GemmArgs& g, int64_t other_cost, bool* done, cudaStream_t s);
-// y = quantised(x) @ w^T for a few rows of x (at most kFusedRows): x is
-// quantised in row blocks by the CTAs that contract it.
+// y = quantised(x) @ w^T for a few rows of x (at most kFusedRows) of up to
+// kFusedMaxK values (what TMEM holds of the parts of 32-bit sums, over the
+// largest split): x is quantised in row blocks by the CTAs that contract it.
 constexpr int kFusedRows = 16;
+constexpr int64_t kFusedMaxK = 442368;
 struct Fp8LinearArgs {
   Fp8GemmArgs g;   // b: the weights; a unused
   const void* x;   // [M][ldx] of type x_type; the output has the same type

@@ -216,7 +216,7 @@ size_t f64e_fp8_linear_workspace_size(int64_t M, int64_t K) {
     bad(check_matrix(M, K));
     return 0;
   }
-  if (M <= kFusedRows) return 0;
+  if (M <= kFusedRows && K <= kFusedMaxK) return 0;
   return (size_t)(round_up(M * round_up(K, 16), 256) + M * blocks_of(K));
 }
 
@@ -241,7 +241,7 @@ int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const
   if (reinterpret_cast<uintptr_t>(w) & 15) return bad("fp8: codes need 16-byte aligned rows");
   for (const void* v : {x, static_cast<const void*>(out)})
     if (const char* m = check_elements(v, q.out_type)) return bad(m);
-  if (q.M > kFusedRows) {
+  if (q.M > kFusedRows || q.K > kFusedMaxK) {
     const size_t need = f64e_fp8_linear_workspace_size(q.M, q.K);
     if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
       return report_error(F64E_ERR_WORKSPACE, "fp8: workspace missing, too small or not 256-byte aligned");

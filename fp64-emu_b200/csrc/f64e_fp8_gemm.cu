@@ -183,16 +183,17 @@ struct GemmK {
 // operands' roles exchanged (TRANS), or after a transposition of one operand
 // (launch_fp8_gemm).
 // Sums: the tensor core truncates what an addition shifts out, an error that
-// grows with the number of additions (measured at K = 16384: 3e-6 of the
-// result's norm).  For 32-bit outputs the accumulator therefore restarts after
-// kChunk blocks of k and the parts are added in registers; 16-bit outputs keep
-// one accumulator, since their own rounding is 100 times that.
+// grows with the number of additions (part_blocks in f64e_fp8_split.cu has the
+// measurements).  An accumulator therefore restarts after kChunk blocks of k
+// for 32-bit outputs and kLongChunk for 16-bit ones, whose own rounding is far
+// larger, and the parts are added in registers (PARTS; 16-bit outputs of up to
+// kLongChunk blocks are stored straight from their one accumulator).
 // Every wait is bounded; one that runs out records its site and unwinds the
 // CTA: copies and MMAs in flight are waited for before TMEM is freed (see the
 // end of the kernel).
 constexpr int BK = kFp8Block, BN = 256, PBM = 256, PHALF = 128, STAGES = 5, SF_STAGES = 4, PGROUP_M = 8;
 constexpr int EPI_WARPS = 8, PTHREADS = 32 * (4 + EPI_WARPS);
-constexpr int kChunk = 16;   // 2048 values of k
+constexpr int kChunk = 16, kLongChunk = 1024;   // 2048 and 131072 values of k
 constexpr uint32_t ATOM = 512, SF_BYTES = 3 * ATOM;   // A's rows, B's rows 0-127, 128-255
 constexpr uint32_t TILE_BYTES = PHALF * BK, STAGE_BYTES = 2 * TILE_BYTES;
 constexpr uint32_t TMEM_COLS = 512, ACC_COLS = 224, SF_COL = 480, SF_COLS = 12;   // scales: two buffers of 4 + 8
@@ -206,7 +207,7 @@ __device__ __forceinline__ void tile_origin(int tile, int ntm, int ntn, int& m0,
   n0 = (o / mh) * BN;
 }
 
-template <int OUT, bool TRANS>
+template <int OUT, bool TRANS, bool PARTS>
 __global__ void __launch_bounds__(PTHREADS, 1)
     fp8_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmapA, const __grid_constant__ CUtensorMap tmapB,
                          const __grid_constant__ CUtensorMap tmapO, const __grid_constant__ GemmK g) {
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
   const bool leader = rank == 0;
   const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   const int ntm = (g.M + PBM - 1) / PBM, ntn = (g.N + BN - 1) / BN, ntiles = ntm * ntn;
-  const int chunk = OUT == F64E_F32 ? kChunk : g.nkb;   // blocks of k per accumulator
+  const int chunk = !PARTS ? g.nkb : OUT == F64E_F32 ? kChunk : kLongChunk;   // blocks of k per accumulator
   int* status = &g_fp8_status;
 
   if (threadIdx.x == 0) {
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           __syncwarp();
         }
       };
-      float sum[OUT == F64E_F32 ? NP : 1][COLS];
+      float sum[PARTS ? NP : 1][COLS];
       for (int kb = 0; kb < g.nkb; kb += chunk, it++) {
         if (!warp_all(mbar_wait_poll(acc_full, it & 1, lim, status, kWaitAccFull) && !*abort_flag)) {
           *abort_flag = 1;
@@ -553,14 +554,17 @@ __global__ void __launch_bounds__(PTHREADS, 1)
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (it & 1) * ACC_COLS;
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-          if (OUT == F64E_F32) {
-            uint32_t v[16];
-            tmem_ld_32x32b_x16(taddr + column(p), v);
-            tmem_wait_ld();
-            if (p == 1) release();   // 32 columns
+          if constexpr (PARTS) {
 #pragma unroll
-            for (int k = 0; k < 16; k++)
-              sum[p][k] = kb == 0 ? __uint_as_float(v[k]) : sum[p][k] + __uint_as_float(v[k]);
+            for (int c = 0; c < COLS; c += 16) {
+              uint32_t v[16];
+              tmem_ld_32x32b_x16(taddr + column(p) + c, v);
+              tmem_wait_ld();
+              if (p * COLS + c == 16) release();   // 32 columns
+#pragma unroll
+              for (int k = 0; k < 16; k++)
+                sum[p][c + k] = kb == 0 ? __uint_as_float(v[k]) : sum[p][c + k] + __uint_as_float(v[k]);
+            }
           } else {
             uint32_t v[32];
             tmem_ld_32x32b_x32(taddr + column(p), v);
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           }
         }
       }
-      if (OUT == F64E_F32 && ok) {
+      if (PARTS && ok) {
 #pragma unroll
         for (int p = 0; p < NP; p++) put(p, sum[p]);
       }
@@ -615,7 +619,7 @@ bool encode_out(CUtensorMap* map, const GemmK& k) {
                    RB == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int OUT, bool TRANS>
+template <int OUT, bool TRANS, bool PARTS>
 cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   CUtensorMap ta, tb;
   CUtensorMap to = {};
@@ -642,22 +646,25 @@ cudaError_t launch_pair(const GemmK& k, int64_t K, int sms, cudaStream_t s) {
   std::unique_lock<std::mutex> lk(mtx);
   int& max_clusters = clusters_of.emplace(dev, -1).first->second;
   if (max_clusters < 0) {
-    e = cudaFuncSetAttribute(fp8_gemm_pair_kernel<OUT, TRANS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PSMEM);
+    e = cudaFuncSetAttribute(fp8_gemm_pair_kernel<OUT, TRANS, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PSMEM);
     if (e != cudaSuccess) return e;
     int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel<OUT, TRANS>, &cfg);
+    e = cudaOccupancyMaxActiveClusters(&n, fp8_gemm_pair_kernel<OUT, TRANS, PARTS>, &cfg);
     if (e != cudaSuccess) return e;
     max_clusters = std::max(n, 1);
   }
   const int64_t tiles = (int64_t)((k.M + PBM - 1) / PBM) * ((k.N + BN - 1) / BN);
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(tiles, max_clusters);
   lk.unlock();
-  return fp8_launch(fp8_gemm_pair_kernel<OUT, TRANS>, grid, PTHREADS, PSMEM, 2, s, ta, tb, to, k);
+  return fp8_launch(fp8_gemm_pair_kernel<OUT, TRANS, PARTS>, grid, PTHREADS, PSMEM, 2, s, ta, tb, to, k);
 }
 
 template <int OUT>
 cudaError_t launch_out(const GemmK& k, bool trans, int64_t K, int sms, cudaStream_t s) {
-  return trans ? launch_pair<OUT, true>(k, K, sms, s) : launch_pair<OUT, false>(k, K, sms, s);
+  if (OUT == F64E_F32 || k.nkb > kLongChunk)
+    return trans ? launch_pair<OUT, true, true>(k, K, sms, s) : launch_pair<OUT, false, true>(k, K, sms, s);
+  constexpr bool parts = OUT == F64E_F32;   // no such instance without parts
+  return trans ? launch_pair<OUT, true, parts>(k, K, sms, s) : launch_pair<OUT, false, parts>(k, K, sms, s);
 }
 
 // ------------------------------------------------------ transposed copies --

@@ -46,7 +46,11 @@ constexpr size_t kMinSmem = 120 * 1024;
 // Floats from one column of partial sums to the next: four rows of eight
 // neighbouring columns lie in different banks.
 constexpr int kPitch = kRows + 4;
-constexpr int kChunkBlocks = 16;         // blocks of k per accumulator, 32-bit outputs
+// Accumulators of a CTA: each holds part_blocks() blocks of k at most.  Parts
+// that TMEM holds beside one another wait there for the end; more of them take
+// turns in two accumulators, and the epilogue's warps, idle until then, add
+// each part to a sum kept in TMEM too.
+constexpr int kTurnParts = 3;            // two accumulators and the sum
 
 struct SplitArgs {
   Fp8Operand w, x;      // wide, thin (fused: x's codes and scales unused)
@@ -54,7 +58,8 @@ struct SplitArgs {
   int nkb;              // blocks of k
   int bn, nst, split;   // columns of a tile, stages, CTAs per tile
   int tiles_r;          // tiles along the wide operand
-  int nacc;             // accumulators (their sums are added at the end)
+  int nacc;             // accumulators (their sums are added at the end), or:
+  int turns;            // blocks of a part, where parts take turns in two of them; 0
   uint32_t tmem_cols, idesc;
   char* out;
   int64_t out_r, out_c;   // output strides (elements) along rows and columns
@@ -79,8 +84,10 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 template <int XT>
 constexpr int kQuantWarps = XT >= 0 ? 8 : 4;
 
-// XT: type of x when the kernel quantises it, -1 for codes.
-template <int OUT, int XT>
+// XT: type of x when the kernel quantises it, -1 for codes.  TURNS: parts take
+// turns in two accumulators (an instance of its own: that code inline cost the
+// others, 8 us kernels whose instructions are fetched anew each time, 0.1 us).
+template <int OUT, int XT, bool TURNS>
 __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     fp8_split_kernel(const __grid_constant__ CUtensorMap tmapW, const __grid_constant__ CUtensorMap tmapX,
                      const __grid_constant__ SplitArgs g) {
@@ -94,7 +101,9 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
   uint64_t* empty = full + kMaxStages;
   uint64_t* sf_full = empty + kMaxStages;
   uint64_t* acc_full = sf_full + kMaxStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* part_full = acc_full + 1;   // [2], and the part's accumulator read: [2]
+  uint64_t* part_empty = part_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(part_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -102,7 +111,8 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
   const int r0 = (tile % g.tiles_r) * kRows, c0 = (tile / g.tiles_r) * g.bn;
   const int kb0 = (int)((int64_t)g.nkb * rank / g.split), kb1 = (int)((int64_t)g.nkb * (rank + 1) / g.split);
   const int cols = min(g.bn, g.cols - c0);
-  const int per = (kb1 - kb0 + g.nacc - 1) / g.nacc;   // blocks per accumulator
+  const int turns = TURNS ? g.turns : 0;
+  const int per = turns ? turns : (kb1 - kb0 + g.nacc - 1) / g.nacc;   // blocks per accumulator
   const uint64_t lim = g.wait_limit_ns;
   int* status = &g_fp8_split_status;
 
@@ -159,6 +169,10 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     if (lane == 0) {
       for (int s = 0; s < g.nst; s++) mbar_init(&empty[s], 1);
       mbar_init(acc_full, 1);
+      for (int i = 0; i < 2 && TURNS; i++) {
+        mbar_init(&part_full[i], 1);
+        mbar_init(&part_empty[i], 4);   // the epilogue's warps
+      }
       *abort_flag = 0;
       fence_barrier_init();
     }
@@ -209,10 +223,24 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
     const uint32_t sf_base = tmem + g.bn * g.nacc;
     int s = 0, left = 0;
     uint32_t ph = 0, d_tmem = tmem - g.bn, accumulate = 0;
+    int part = -1;   // where they take turns: the part at work
     bool ok = true;
     for (int kb = kb0; kb < kb1; kb++) {
       if (left == 0) {
-        d_tmem += g.bn;
+        if (TURNS) {
+          if (part >= 0 && issuer) tc_commit(&part_full[part & 1]);
+          part++;
+          // the accumulator's last part but one has been read
+          if (part >= 2 &&
+              !mbar_wait_lane(&part_empty[part & 1], ((part >> 1) + 1) & 1, lim, status, kWaitAccEmpty)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          d_tmem = tmem + (part & 1) * g.bn;
+        } else {
+          d_tmem += g.bn;
+        }
         accumulate = 0;
         left = per;
       }
@@ -327,16 +355,51 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
         for (s += QW; s >= g.nst; par ^= 1) s -= g.nst;
       }
     }
+    const int q = warp & 3;
+    const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
+    bool done = warp < 8;
+    const int parts = n <= per ? 1 : (n + per - 1) / per;
+    // What the end adds: all parts in their order, or the sum kept so far and the last part.
+    const int terms = TURNS ? min(parts, 2) : parts;
+    uint32_t term0 = taddr, term_step = g.bn;
+    if (TURNS && parts > 1) {
+      term0 += 2 * g.bn;
+      term_step = ((parts - 1) & 1) * g.bn - 2 * g.bn;
+    }
+    if (TURNS) {
+      // All parts but the last: the first to the sum's columns, others added.
+      for (int a = 0; a + 1 < parts && done; a++) {
+        const int i = a & 1;
+        done = warp_all(mbar_wait_poll(&part_full[i], (a >> 1) & 1, lim, status, kWaitAccFull) && !*abort_flag);
+        if (!done) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        for (int c = 0; c < cols; c += 16) {
+          uint32_t v[16], w[16];
+          tmem_ld_32x32b_x16(taddr + i * g.bn + c, v);
+          if (a > 0) tmem_ld_32x32b_x16(taddr + 2 * g.bn + c, w);
+          tmem_wait_ld();
+          if (a > 0) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(w[k]) + __uint_as_float(v[k]));
+          }
+          tmem_st_32x32b_x16(taddr + 2 * g.bn + c, v);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&part_empty[i]);
+      }
+    }
     // Partial sums to shared memory, by columns of 128 rows; the stages are free:
     // every MMA has completed.
-    const bool done =
-        warp < 8 && warp_all(mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag);
+    done = done && warp_all(mbar_wait_poll(acc_full, 0, drain_limit(lim), status, kWaitAccFull) && !*abort_flag);
     if (done) {
       tc_fence_after();
-      const int q = warp & 3;
-      const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
       float* part = reinterpret_cast<float*>(smem) + q * 32 + lane;   // column pitch kPitch
-      if (n <= per && g.bn % 32 == 0) {   // one accumulator, 32 columns at a time
+      if (parts == 1 && g.bn % 32 == 0) {   // one accumulator, 32 columns at a time
         for (int c = 0; c < cols; c += 32) {
           uint32_t v[32];
           tmem_ld_32x32b_x32(taddr + c, v);
@@ -347,9 +410,9 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
       } else {
         for (int c = 0; c < cols; c += 16) {
           float sum[16];
-          for (int a = 0; a * per < n; a++) {
+          for (int a = 0; a < terms; a++) {
             uint32_t v[16];
-            tmem_ld_32x32b_x16(taddr + a * g.bn + c, v);
+            tmem_ld_32x32b_x16(term0 + a * term_step + c, v);
             tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 16; k++) sum[k] = a == 0 ? __uint_as_float(v[k]) : sum[k] + __uint_as_float(v[k]);
@@ -438,7 +501,7 @@ __global__ void __launch_bounds__(32 * (4 + kQuantWarps<XT>), 1)
   if (g.split > 1) cluster_sync();   // the peers have read this CTA's sums
 }
 
-template <int OUT, int XT>
+template <int OUT, int XT, bool TURNS>
 cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const SplitArgs& k, int tiles, size_t smem,
                           cudaStream_t s) {
   int dev = 0;
@@ -450,13 +513,20 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
     static std::map<int, bool> done;
     std::lock_guard<std::mutex> lk(mtx);
     if (!done[dev]) {
-      e = cudaFuncSetAttribute(fp8_split_kernel<OUT, XT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+      e = cudaFuncSetAttribute(fp8_split_kernel<OUT, XT, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
       if (e != cudaSuccess) return e;
       done[dev] = true;
     }
   }
-  return fp8_launch(fp8_split_kernel<OUT, XT>, (unsigned)(tiles * k.split), 32 * (4 + kQuantWarps<XT>), smem, k.split, s,
+  return fp8_launch(fp8_split_kernel<OUT, XT, TURNS>, (unsigned)(tiles * k.split), 32 * (4 + kQuantWarps<XT>), smem, k.split, s,
                     tw, tx, k);
+}
+
+template <int OUT>
+cudaError_t launch_codes(const CUtensorMap& tw, const CUtensorMap& tx, const SplitArgs& k, int tiles, size_t smem,
+                         cudaStream_t s) {
+  return k.turns ? launch_kernel<OUT, -1, true>(tw, tx, k, tiles, smem, s)
+                 : launch_kernel<OUT, -1, false>(tw, tx, k, tiles, smem, s);
 }
 
 // held[n]: clusters of n CTAs that the current device holds at once (a
@@ -472,7 +542,7 @@ cudaError_t resident_clusters(int sms, const int** held) {
   if (it == known.end()) {
     std::array<int, kMaxSplit + 1> h{};
     const size_t smem = 200 * 1024;   // any amount above half an SM's gives the same answer
-    e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
     if (e != cudaSuccess) return e;
     for (int n = 1; n <= kMaxSplit; n++) {
       cudaLaunchConfig_t cfg = {};
@@ -487,7 +557,7 @@ cudaError_t resident_clusters(int sms, const int** held) {
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int c = 0;
-      e = cudaOccupancyMaxActiveClusters(&c, fp8_split_kernel<F64E_BF16, -1>, &cfg);
+      e = cudaOccupancyMaxActiveClusters(&c, fp8_split_kernel<F64E_BF16, -1, false>, &cfg);
       if (e != cudaSuccess) return e;
       h[n] = std::max(c, 1);
     }
@@ -512,7 +582,8 @@ struct Plan {
 // 2048 x 2048 14.6 us against 11.7).  Measured, both sides of a choice: 1024^3
 // 7.7 us with 64 columns, 8.7 with 128; 8 x 2048 x 8192 9.1 us with 7 CTAs a
 // tile, 14.3 with 8, of whose clusters the device holds one too few at once.
-cudaError_t plan_tiles(int64_t rows, int64_t cols, int64_t nkb, int sms, Plan* best) {
+// most: blocks of k that a CTA may take at most (0: any number).
+cudaError_t plan_tiles(int64_t rows, int64_t cols, int64_t nkb, int sms, int64_t most, Plan* best) {
   const int* held_of = nullptr;
   const cudaError_t e = resident_clusters(sms, &held_of);
   if (e != cudaSuccess) return e;
@@ -522,6 +593,7 @@ cudaError_t plan_tiles(int64_t rows, int64_t cols, int64_t nkb, int sms, Plan* b
     if (t > t0 && bn < 48) break;
     const int64_t tiles = (rows + kRows - 1) / kRows * ((cols + bn - 1) / bn);
     for (int s = 1; s <= kMaxSplit && s <= nkb; s++) {
+      if (most > 0 && (nkb + s - 1) / s > most) continue;
       const int64_t held = held_of[s];
       const int64_t ctas = std::min(tiles, held) * s;
       const int64_t block = std::max<int64_t>(500, ctas * (kWideBytes + bn * kBlock) / 5300);
@@ -532,6 +604,23 @@ cudaError_t plan_tiles(int64_t rows, int64_t cols, int64_t nkb, int sms, Plan* b
   }
   return cudaSuccess;
 }
+
+// Blocks of k that one accumulator may hold.  The tensor core truncates what an
+// addition shifts out, always towards zero: measured on random 2048 x 2048 x K,
+// sums in one accumulator come out too small by 7e-8 of themselves at K = 2048
+// (a 32-bit product of torch is off by 6e-8), 6e-6 at 65536, 4e-5 at 262144 and
+// 2e-4 at 2^20, as much as rounding to float16 (2.1e-4).  Parts of 2048 values
+// for 32-bit outputs, and of 131072 for 16-bit ones: too small by 1.6e-5.
+constexpr int part_blocks(int out_type) { return out_type == F64E_F32 ? 16 : 1024; }
+
+int stages_of(int bn, int per_cta) {
+  return (int)std::min<int64_t>({kMaxStages, per_cta, (int64_t)(kRing / (kWideBytes + bn * kBlock + 2 * kAtom))});
+}
+// Accumulators of bn columns that TMEM holds beside the stages' scales.
+int held_parts(int bn, int stages) { return (512 - stages * 8) / bn; }
+static_assert((512 - 8 * (int)(kRing / (kWideBytes + kMaxCols * kBlock + 2 * kAtom))) / kMaxCols >= kTurnParts &&
+                  (512 - 8 * kMaxStages) / 16 * 16 * kMaxSplit * kBlock >= kFusedMaxK,
+              "three accumulators fit beside any stages, and all parts of a fused product beside one another");
 
 // k.rows x k.cols of k.w and k.x.
 cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Plan& plan, cudaStream_t s) {
@@ -547,12 +636,14 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Plan&
   const int tiles = k.tiles_r * ((k.cols + k.bn - 1) / k.bn);
   const int per_cta = (k.nkb + k.split - 1) / k.split;
   const size_t stage = kWideBytes + (size_t)k.bn * kBlock;
-  k.nst = (int)std::min<int64_t>({kMaxStages, per_cta, (int64_t)(kRing / (stage + 2 * kAtom))});
-  // 32-bit outputs: a new accumulator every kChunkBlocks, as far as TMEM goes
+  k.nst = stages_of(k.bn, per_cta);
   const int sf_cols = k.nst * 8;
-  k.nacc = out_type == F64E_F32
-               ? std::max(1, std::min((per_cta + kChunkBlocks - 1) / kChunkBlocks, (512 - sf_cols) / k.bn))
-               : 1;
+  k.nacc = (per_cta + part_blocks(out_type) - 1) / part_blocks(out_type);
+  if (k.nacc > held_parts(k.bn, k.nst)) {
+    if (x_type >= 0) return cudaErrorInvalidValue;   // excluded by the plan
+    k.nacc = kTurnParts;
+    k.turns = part_blocks(out_type);
+  }
   k.tmem_cols = 32;
   while ((int)k.tmem_cols < k.bn * k.nacc + sf_cols) k.tmem_cols *= 2;
   k.idesc = idesc_mx(kRows, k.bn, k.w.code, k.x.code, !k.w.kmajor, 0);
@@ -561,18 +652,18 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Plan&
   const int es = out_type == F64E_F32 ? 4 : 2;
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
   k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);
-  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * 2 * kAtom + (3 * kMaxStages + 1) * 8 + 16);
+  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * 2 * kAtom + (3 * kMaxStages + 5) * 8 + 16);
   if (x_type >= 0) {
     switch (x_type) {
-      case F64E_F32: return launch_kernel<F64E_F32, F64E_F32>(tw, tx, k, tiles, smem, s);
-      case F64E_F16: return launch_kernel<F64E_F16, F64E_F16>(tw, tx, k, tiles, smem, s);
-      default: return launch_kernel<F64E_BF16, F64E_BF16>(tw, tx, k, tiles, smem, s);
+      case F64E_F32: return launch_kernel<F64E_F32, F64E_F32, false>(tw, tx, k, tiles, smem, s);
+      case F64E_F16: return launch_kernel<F64E_F16, F64E_F16, false>(tw, tx, k, tiles, smem, s);
+      default: return launch_kernel<F64E_BF16, F64E_BF16, false>(tw, tx, k, tiles, smem, s);
     }
   }
   switch (out_type) {
-    case F64E_F32: return launch_kernel<F64E_F32, -1>(tw, tx, k, tiles, smem, s);
-    case F64E_F16: return launch_kernel<F64E_F16, -1>(tw, tx, k, tiles, smem, s);
-    default: return launch_kernel<F64E_BF16, -1>(tw, tx, k, tiles, smem, s);
+    case F64E_F32: return launch_codes<F64E_F32>(tw, tx, k, tiles, smem, s);
+    case F64E_F16: return launch_codes<F64E_F16>(tw, tx, k, tiles, smem, s);
+    default: return launch_codes<F64E_BF16>(tw, tx, k, tiles, smem, s);
   }
 }
 
@@ -582,7 +673,7 @@ cudaError_t launch_fp8_split(const Fp8GemmArgs& g, int64_t other_cost, bool* don
   *done = false;
   if (!(g.M <= g.N ? g.a : g.b).kmajor) return cudaSuccess;
   Plan plan;
-  const cudaError_t e = plan_tiles(std::max(g.M, g.N), std::min(g.M, g.N), (g.K + kBlock - 1) / kBlock, g.sms, &plan);
+  const cudaError_t e = plan_tiles(std::max(g.M, g.N), std::min(g.M, g.N), (g.K + kBlock - 1) / kBlock, g.sms, 0, &plan);
   if (e != cudaSuccess || plan.cost > other_cost) return e;
   *done = true;
   SplitArgs k = {};
@@ -617,7 +708,9 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
   k.x_wide = x % 32 == 0 && (pitch % 32 == 0 || g.M == 1);
   k.wait_limit_ns = g.wait_limit_ns;
   Plan plan;
-  const cudaError_t e = plan_tiles(g.N, g.M, (g.K + kBlock - 1) / kBlock, g.sms, &plan);
+  // Its warps 4 to 7 quantise x until the end, so its parts are all kept.
+  const int64_t most = (int64_t)held_parts(16, kMaxStages) * part_blocks(a.x_type);
+  const cudaError_t e = plan_tiles(g.N, g.M, (g.K + kBlock - 1) / kBlock, g.sms, most, &plan);
   return e == cudaSuccess ? launch(k, a.x_type, a.x_type, g.K, plan, s) : e;
 }
 

@@ -299,9 +299,9 @@ F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void*
 
 /* out [M, N] = x [M, K] @ w^T, a layer on M rows: x (row pitch ldx, of the
  * type p->out_type) is quantised to e4m3 in row blocks, w is the operand p->b;
- * p->a is not read.  Up to 16 rows are quantised by the product itself, in one
- * launch; more need a workspace (256-byte aligned device memory of
- * f64e_fp8_linear_workspace_size() bytes) for their codes. */
+ * p->a is not read.  Up to 16 rows of up to 442368 values are quantised by the
+ * product itself, in one launch; more need a workspace (256-byte aligned device
+ * memory of f64e_fp8_linear_workspace_size() bytes) for their codes. */
 F64E_API size_t f64e_fp8_linear_workspace_size(int64_t M, int64_t K);
 F64E_API int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const void* w,
                              const void* w_scale, void* out, void* workspace, size_t workspace_bytes, void* stream);

@@ -446,3 +446,13 @@ def test_layer_and_gradients_keep_dynamic_dimensions(shape, dynamic, kept):
     assert [g.shape for g in grads] == [t.shape for t in wanted]
     assert y.shape[-1] == 256
     assert not env.guards, env.guards
+
+
+def test_linear_abi_workspace_over_long_k(lib):
+    """Few rows of more than 442368 values are quantised before the product, into a workspace."""
+    assert lib.f64e_fp8_linear_workspace_size(16, 442368) == 0
+    need = lib.f64e_fp8_linear_workspace_size(4, 442369)
+    assert need == (4 * 442384 + 255) // 256 * 256 + 4 * 3457
+    p = Problem(4, 64, 442369, 0, 64, Operand(), Operand(442384, 0, 1, 1, 3457, 1))
+    assert lib.f64e_fp8_linear(ctypes.byref(p), P, 442369, P, P, P, P, need - 1, None) == 2
+    assert "workspace" in lib.f64e_last_error().decode()

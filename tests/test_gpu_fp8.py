@@ -836,3 +836,105 @@ def test_layer_refuses_tangents_and_second_derivatives():
     assert torch.equal(dx.detach(), plain)
     with pytest.raises(RuntimeError, match="no second derivative"):
         (y.float().sum() + (dx.float() ** 2).sum()).backward()
+
+
+# ------------------------------------------------------------------ long K --
+def whole_numbers(rows, cols, seed, per_row):
+    """Integers of -2 .. 2 times a power of two for each block of 128 columns (and each row): exact as codes."""
+    g = gen(seed)
+    v = torch.randint(-2, 3, (rows, cols), generator=g, device="cuda").float()
+    m = torch.randint(0, 4, (rows if per_row else 1, (cols + 127) // 128), generator=g, device="cuda").float()
+    return v * torch.exp2(m).repeat_interleave(128, 1)[:, :cols]
+
+
+def exact_product(a, b):
+    """a @ b^T in 64 bits; every partial sum in whatever order is a whole number below 2^24, so 32-bit sums are exact."""
+    want = sum(a[:, k:k + 16384].double() @ b[:, k:k + 16384].double().t() for k in range(0, a.shape[1], 16384))
+    most = sum(a[:, k:k + 16384].abs().double() @ b[:, k:k + 16384].abs().double().t()
+               for k in range(0, a.shape[1], 16384))
+    assert float(most.max()) < 2 ** 24
+    return want.float()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 256, 65576), (128, 128, 65576), (128, 128, 131112), (256, 200, 65576),
+                                   (1024, 1024, 131072), (16, 40, 300000), (2309, 2311, 4136)])
+@pytest.mark.parametrize("layout", ["nt", "tn"])
+def test_products_over_long_k_are_exact_for_whole_numbers(M, N, K, layout):
+    """A block, a part of the sums or a scale that is left out, taken twice or taken from a neighbour shows."""
+    a, b = whole_numbers(M, K, M, True), whole_numbers(N, K, N + 1, True)
+    want = exact_product(a, b)
+    if layout == "nt":
+        (qa, sa), (qb, sb) = fp64_emu.quantize_fp8(a), fp64_emu.quantize_fp8(b)
+        del a, b
+        got = fp64_emu.mm_fp8(qa, qb, sa, sb, SF)
+    else:
+        qa, sa = fp64_emu.quantize_fp8(a.t().contiguous(), "col")
+        qb, sb = fp64_emu.quantize_fp8(b.t().contiguous(), "col")
+        del a, b
+        got = fp64_emu.mm_tn_fp8(qa, qb, sa, sb, SF)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 70000), (4, 130, 442368), (4, 130, 442500), (16, 20000, 60000)])
+def test_layer_over_long_k_is_exact_for_whole_numbers(M, N, K):
+    """Few rows, quantised in the product up to K = 442368 and before it beyond."""
+    x, w = whole_numbers(M, K, 1, True), whole_numbers(N, K, 2, False)
+    want = exact_product(x, w)
+    q, s = fp64_emu.quantize_fp8(w, "tile")
+    del w
+    assert torch.equal(fp64_emu.linear_fp8(x, q, s), want)
+
+
+def one_large_many_small(K, large, small):
+    """[1, K]: `large`, then `small` at every 32nd place; codes and scales of its row blocks."""
+    v = torch.zeros(1, K, device="cuda")
+    v[0, 1::32] = small
+    v[0, 0] = large
+    q, s = fp64_emu.quantize_fp8(v)
+    assert torch.equal(fp64_emu.dequantize_fp8(q, s, "row", SF), v)
+    return q.view(torch.uint8), s.view(torch.uint8)
+
+
+def same_rows(layout, rows, q, s):
+    """`rows` times that row: [rows, K] with row blocks, or [K, rows] with column blocks."""
+    q, s = q.expand(rows, -1), s.expand(rows, -1)
+    if layout == "tn":
+        q, s = q.t(), s.t()
+    return q.contiguous().view(E4), s.contiguous().view(E8)
+
+
+@pytest.mark.parametrize("layout,M,N,K", [("nt", 128, 128, 262144), ("nt", 1024, 1024, 131072), ("tn", 256, 256, 131072),
+                                          ("nt", 2304, 2304, 8192), ("nt", 16, 512, 131072)])
+def test_sums_of_long_products_restart(layout, M, N, K):
+    """2^25, then K / 32 ones.  Beside the large term a 32-bit sum holds multiples of 4, and a one added to it is cut
+    off; so an accumulator that runs on loses all ones after it.  One that starts anew after 2048 values loses at most
+    the 64 of its own part: other parts' sums are exact, and, 4 to a block of 128, multiples of 4, so adding them to
+    the large one is exact too."""
+    a, b = one_large_many_small(K, 2.0 ** 13, 1.0), one_large_many_small(K, 2.0 ** 12, 1.0)
+    (qa, sa), (qb, sb) = same_rows(layout, M, *a), same_rows(layout, N, *b)
+    got = (fp64_emu.mm_fp8 if layout == "nt" else fp64_emu.mm_tn_fp8)(qa, qb, sa, sb, SF).double()
+    lost = 2.0 ** 25 + K // 32 - got
+    assert float(lost.min()) >= 0 and float(lost.max()) <= 64
+
+
+def test_sums_of_a_layer_over_long_k_restart():
+    """The same in a layer on few rows, in 32 bits, within the product's own quantisation and beyond it."""
+    for K in (131072, 442368, 524288):
+        x = torch.zeros(3, K, device="cuda")
+        x[:, 1::32], x[:, 0] = 1.0, 2.0 ** 13
+        q, s = one_large_many_small(K, 2.0 ** 12, 1.0)
+        lost = 2.0 ** 25 + K // 32 - fp64_emu.linear_fp8(x, q.expand(200, -1).contiguous().view(E4),
+                                                         s.expand(2, -1).contiguous().view(E8)).double()
+        assert float(lost.min()) >= 0 and float(lost.max()) <= 64
+
+
+@pytest.mark.parametrize("layout,M,N,K", [("tn", 256, 256, 2 ** 20), ("tn", 300, 136, 2 ** 20), ("nt", 512, 512, 2 ** 21),
+                                          ("nt", 1024, 1024, 2 ** 21), ("nt", 256, 256, 2 ** 22)])
+def test_sums_of_very_long_products_in_16_bits_restart(layout, M, N, K):
+    """2^14, then K / 32 times 2^-10, in float16, whose values are multiples of 16 there.  An accumulator holds
+    multiples of 2^-9 beside the large term and would lose all of the small ones; after 131072 values it starts anew,
+    and at most 4096 of them, 4 in all, are lost.  The sum, a multiple of 16, less 4 at most, rounds to itself."""
+    a, b = one_large_many_small(K, 2.0 ** 7, 2.0 ** -5), one_large_many_small(K, 2.0 ** 7, 2.0 ** -5)
+    (qa, sa), (qb, sb) = same_rows(layout, M, *a), same_rows(layout, N, *b)
+    got = (fp64_emu.mm_fp8 if layout == "nt" else fp64_emu.mm_tn_fp8)(qa, qb, sa, sb, HF)
+    assert torch.equal(got, torch.full_like(got, 2.0 ** 14 + K / 2 ** 15))
