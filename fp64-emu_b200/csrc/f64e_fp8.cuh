@@ -395,7 +395,7 @@ __device__ __forceinline__ void mma_mx_pair(uint32_t d_tmem, uint64_t a_desc, ui
       : "memory");
 }
 
-enum : int { kWaitScales = 6, kWaitScalesFree = 7 };   // status sites, beside kWait*
+enum : int { kWaitScales = 6, kWaitScalesFree = 7, kWaitSelfTestSplit = 10 };   // status sites, beside kWait*
 
 // --------------------------------------------------------------- scales --
 // Gathering the scales of `N` atoms (128 rows each, from r0) for blocks 4 j ..

@@ -117,5 +117,9 @@ int fp8_scale_mode(const Fp8Operand& o, int64_t rows, bool whole_squares);
 // The device's status words of these products, cleared by the read; synchronizes.
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s);
 cudaError_t read_fp8_status(int* status, cudaStream_t s);
+// One thread runs a bounded wait out, which records its site in the pairs' word
+// (kWaitSelfTest) or the split products' (kWaitSelfTestSplit).
+cudaError_t launch_fp8_wait_selftest(uint64_t limit_ns, cudaStream_t s);
+cudaError_t launch_fp8_split_wait_selftest(uint64_t limit_ns, cudaStream_t s);
 
 }  // namespace f64e

@@ -264,6 +264,17 @@ int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t ldx, const
   return e == cudaSuccess ? F64E_OK : cuda_error(e);
 }
 
+int f64e_fp8_wait_selftest(int32_t split, uint64_t limit_ns, void* stream) {
+  begin_call();
+  if (split != 0 && split != 1) return bad("fp8: split must be 0 or 1");
+  if (limit_ns == 0 || limit_ns > 10000000000ULL) return bad("fp8: limit must be in (0, 10 s]");
+  int sms = 0;
+  if (const int rc = device_sms(&sms)) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = split ? launch_fp8_split_wait_selftest(limit_ns, s) : launch_fp8_wait_selftest(limit_ns, s);
+  return e == cudaSuccess ? F64E_OK : cuda_error(e);
+}
+
 int f64e_fp8_status(void* stream, int32_t* status) {
   begin_call();
   if (!status) return bad("fp8: null argument");

@@ -790,6 +790,20 @@ cudaError_t launch_fp8_gemm(const Fp8GemmArgs& g, void* workspace, cudaStream_t 
   }
 }
 
+// Nothing arrives at the barrier and nothing else is in flight: the kernel returns.
+__global__ void fp8_wait_selftest_kernel(uint64_t limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  if (elect_one()) {
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+    mbar_wait_poll(&bar, 0, limit_ns, &g_fp8_status, kWaitSelfTest);
+  }
+}
+cudaError_t launch_fp8_wait_selftest(uint64_t limit_ns, cudaStream_t s) {
+  fp8_wait_selftest_kernel<<<1, 32, 0, s>>>(limit_ns);
+  return cudaGetLastError();
+}
+
 cudaError_t read_fp8_status(int* status, cudaStream_t s) {
   static const int zero = 0;
   int split = 0;

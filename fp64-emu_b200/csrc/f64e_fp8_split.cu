@@ -714,6 +714,20 @@ cudaError_t launch_fp8_linear_few(const Fp8LinearArgs& a, cudaStream_t s) {
   return e == cudaSuccess ? launch(k, a.x_type, a.x_type, g.K, plan, s) : e;
 }
 
+// Nothing arrives at the barrier and nothing else is in flight: the kernel returns.
+__global__ void fp8_split_wait_selftest_kernel(uint64_t limit_ns) {
+  __shared__ __align__(8) uint64_t bar;
+  if (elect_one()) {
+    mbar_init(&bar, 1);
+    fence_barrier_init();
+    mbar_wait_poll(&bar, 0, limit_ns, &g_fp8_split_status, kWaitSelfTestSplit);
+  }
+}
+cudaError_t launch_fp8_split_wait_selftest(uint64_t limit_ns, cudaStream_t s) {
+  fp8_split_wait_selftest_kernel<<<1, 32, 0, s>>>(limit_ns);
+  return cudaGetLastError();
+}
+
 cudaError_t read_fp8_split_status(int* status, cudaStream_t s) {
   static const int zero = 0;
   cudaError_t e = cudaMemcpyFromSymbolAsync(status, g_fp8_split_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s);

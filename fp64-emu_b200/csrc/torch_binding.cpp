@@ -544,6 +544,11 @@ int64_t fp8_status(int64_t device) {
   return st;
 }
 
+void fp8_wait_selftest(int64_t device, bool split, int64_t limit_ns) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  check(f64e_fp8_wait_selftest(split, (uint64_t)limit_ns, stream_of()));
+}
+
 // ---- a layer held in 8 bits ----
 // Sizes are read as symbols wherever the layer's autograd kernel comes by: it
 // also runs while a compiler traces it, and a number read there would tie the
@@ -774,6 +779,8 @@ TORCH_LIBRARY(fp64_emu_b200, ops) {
   ops.def("fp8_mm(Tensor a, Tensor b, Tensor sa, Tensor sb, int layout, ScalarType dtype) -> Tensor");
   ops.def("fp8_linear(Tensor x, Tensor w, Tensor? ws=None) -> Tensor");
   ops.def("fp8_status(int device) -> int");
+  ops.def("fp8_wait_selftest(int device, bool split, int limit_ns) -> ()");
+  ops.impl("fp8_wait_selftest", &fp8_wait_selftest);
   ops.impl("fp8_status", &fp8_status);
   ops.impl("fp64_emu_maxp", &maxp);
   ops.impl("fp64_emu_workspace_bytes", &workspace_bytes);

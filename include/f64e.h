@@ -312,6 +312,12 @@ F64E_API int f64e_fp8_linear(const f64e_fp8_problem* p, const void* x, int64_t l
  * on scales).  Reading clears it.  Synchronizes the stream. */
 F64E_API int f64e_fp8_status(void* stream, int32_t* status);
 
+/* Failure-detection self-test of that status (as f64e_wait_selftest): one
+ * device thread waits for what never comes, so that after limit_ns (0 <
+ * limit_ns <= 1e10) site 9 is recorded by the kernel of large products, or, with
+ * split = 1, site 10 by that of few rows or tiles.  f64e_fp8_status reads it. */
+F64E_API int f64e_fp8_wait_selftest(int32_t split, uint64_t limit_ns, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -456,3 +456,10 @@ def test_linear_abi_workspace_over_long_k(lib):
     p = Problem(4, 64, 442369, 0, 64, Operand(), Operand(442384, 0, 1, 1, 3457, 1))
     assert lib.f64e_fp8_linear(ctypes.byref(p), P, 442369, P, P, P, P, need - 1, None) == 2
     assert "workspace" in lib.f64e_last_error().decode()
+
+
+def test_wait_selftest_abi_refusals(lib):
+    lib.f64e_fp8_wait_selftest.argtypes = [ctypes.c_int32, ctypes.c_uint64, ctypes.c_void_p]
+    for split, limit, msg in ((2, 1000, "split must be"), (0, 0, "limit must be"), (1, 10 ** 10 + 1, "limit must be")):
+        assert lib.f64e_fp8_wait_selftest(split, limit, None) == 1
+        assert msg in lib.f64e_last_error().decode()

@@ -938,3 +938,23 @@ def test_sums_of_very_long_products_in_16_bits_restart(layout, M, N, K):
     (qa, sa), (qb, sb) = same_rows(layout, M, *a), same_rows(layout, N, *b)
     got = (fp64_emu.mm_fp8 if layout == "nt" else fp64_emu.mm_tn_fp8)(qa, qb, sa, sb, HF)
     assert torch.equal(got, torch.full_like(got, 2.0 ** 14 + K / 2 ** 15))
+
+
+def test_status_reports_a_wait_that_ran_out_once():
+    """Either kernel's word reaches the caller, the large products' first, and the read clears both; products after it
+    are right and leave it clear."""
+    run_out = lambda split: fp64_emu.ops.fp8_wait_selftest(0, split, 5_000_000)   # noqa: E731  5 ms
+    assert fp64_emu.fp8_status() == 0
+    for splits, site in (((False,), 9), ((True,), 10), ((True, False), 9), ((False, True), 9)):
+        for split in splits:
+            run_out(split)
+        assert fp64_emu.fp8_status() == site
+        assert fp64_emu.fp8_status() == 0
+    a, sa, av = operand(300, 1024, "row", E4, 1)
+    b, sb, bv = operand(2304, 1024, "tile", E4, 2)
+    for m in (300, 3):
+        R.check_product(fp64_emu.mm_fp8(a[:m], b, sa[:m], sb), av[:m], bv.t())
+    assert fp64_emu.fp8_status() == 0
+    for bad in (0, 10_000_000_001):
+        with pytest.raises(RuntimeError, match="limit must be"):
+            fp64_emu.ops.fp8_wait_selftest(0, False, bad)
