@@ -261,7 +261,9 @@ F64E_API int f64e_fp8_quantize_both(const void* x, int32_t x_type, int64_t rows,
                                     int32_t code, void* q_row, void* scale_row, int64_t ldq, void* q_col,
                                     void* scale_col, int32_t transposed, int64_t ld_col, void* stream);
 
-/* out [rows][cols] (contiguous, out_type) = code * scale, rounded once.
+/* out [rows][cols] (contiguous, out_type) = code * scale, rounded once: in F16
+ * a value whose code rounded up past 65504 (63488 and more in E4M3, 61440 in
+ * E5M2) becomes infinity.
  * scale_row / scale_col: strides of the scales in bytes; any ldq >= cols. */
 F64E_API int f64e_fp8_dequantize(const void* q, int32_t code, int64_t rows, int64_t cols, int64_t ldq,
                                  int32_t blocks, const void* scale, int64_t scale_row, int64_t scale_col,
@@ -292,7 +294,10 @@ typedef struct f64e_fp8_problem {
 F64E_API size_t f64e_fp8_workspace_size(const f64e_fp8_problem* p);
 
 /* The product of the values codes and scales stand for; sums are held in 32
- * bits and rounded once.  workspace: at least f64e_fp8_workspace_size() bytes
+ * bits and rounded once.  An addition into such a sum cuts off what it shifts
+ * out, and sums start anew every 2048 values of k (131072 for 16-bit outputs)
+ * and are then added with rounding: 32-bit outputs are 1e-7 of their norm off
+ * (4e-7 at K = 2^20), the sums behind 16-bit ones up to 2e-5.  workspace: at least f64e_fp8_workspace_size() bytes
  * of device memory, 256-byte aligned, or NULL where that is 0. */
 F64E_API int f64e_fp8_gemm(const f64e_fp8_problem* p, const void* A, const void* a_scale, const void* B,
                            const void* b_scale, void* out, void* workspace, size_t workspace_bytes, void* stream);

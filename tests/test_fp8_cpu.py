@@ -463,3 +463,17 @@ def test_wait_selftest_abi_refusals(lib):
     for split, limit, msg in ((2, 1000, "split must be"), (0, 0, "limit must be"), (1, 10 ** 10 + 1, "limit must be")):
         assert lib.f64e_fp8_wait_selftest(split, limit, None) == 1
         assert msg in lib.f64e_last_error().decode()
+
+
+def test_codes_and_products_are_detached():
+    """As documented: constants to autograd in both modes, whatever the inputs require."""
+    import torch.autograd.forward_ad as fw
+    x = torch.empty(6, 40, device="meta", requires_grad=True)
+    with fw.dual_level():
+        for t in (x, fw.make_dual(x.detach(), torch.empty(6, 40, device="meta"))):
+            q, s = fp64_emu.quantize_fp8(t)
+            results = (q, s, *fp64_emu.quantize_fp8_both(t), fp64_emu.dequantize_fp8(q, s), fp64_emu.mm_fp8(q, q, s, s))
+            for r in results:
+                assert not r.requires_grad and fw.unpack_dual(r).tangent is None
+    for f in (fp64_emu.quantize_fp8, fp64_emu.quantize_fp8_both, fp64_emu.dequantize_fp8):
+        assert "detached" in f.__doc__ or "without a\n    gradient" in f.__doc__

@@ -958,3 +958,31 @@ def test_status_reports_a_wait_that_ran_out_once():
     for bad in (0, 10_000_000_001):
         with pytest.raises(RuntimeError, match="limit must be"):
             fp64_emu.ops.fp8_wait_selftest(0, False, bad)
+
+
+@pytest.mark.parametrize("code,first", [(E4, 63488.0), (E5, 61440.0)])
+def test_restored_float16_overflows_where_documented(code, first):
+    x = torch.arange(57344, 65505, 1, device="cuda").to(HF).unique()[:, None]
+    back = fp64_emu.dequantize_fp8(*fp64_emu.quantize_fp8(x, "row", code), "row", HF)
+    assert torch.equal(torch.isinf(back), x >= first)
+    for dtype in (BF, SF):
+        assert torch.isfinite(fp64_emu.dequantize_fp8(*fp64_emu.quantize_fp8(x, "row", code), "row", dtype)).all()
+
+
+def test_layer_under_vmap_and_saved_tensor_hooks():
+    x, w, dy = data(4 * 30, 300, BF, 1, 1).view(4, 30, 300), data(64, 300, BF, 2, 1), data(30, 64, BF, 3, 1)
+    each = torch.stack([fp64_emu.linear_fp8(t, w) for t in x])
+    assert torch.equal(torch.vmap(lambda t: fp64_emu.linear_fp8(t, w))(x), each)
+    a, b = x[0].clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(fp64_emu.linear_fp8(a, b), (a, b), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = fp64_emu.linear_fp8(a, b)
+    for got, right in zip(torch.autograd.grad(y, (a, b), dy, retain_graph=True), want):
+        assert torch.equal(got, right)
+    # several gradients of the output at once
+    many = torch.stack([dy, 2 * dy, data(30, 64, BF, 4, 1)])
+    y = fp64_emu.linear_fp8(a, b)
+    batched = torch.autograd.grad(y, (a, b), many, is_grads_batched=True, retain_graph=True)
+    for i in range(3):
+        for got, right in zip(batched, torch.autograd.grad(y, (a, b), many[i], retain_graph=True)):
+            assert torch.equal(got[i], right)
