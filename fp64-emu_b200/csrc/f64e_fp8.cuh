@@ -263,17 +263,10 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity, u
 // What a wait gave, for the whole warp: true where all of its lanes have what
 // they waited for.  A lane that gives up, or reads the abort flag a moment
 // later than its neighbours, must not part from them: tcgen05 loads, barriers
-// and __syncwarp behind the wait need all 32.  Every wait that is not one
-// elected thread's goes through it, or is a mbar_wait_lane.
+// and __syncwarp behind the wait need all 32.  Nor may the lane that issues run
+// ahead of one that still waits, which could miss the phase it waits for.  So
+// every wait that is not one elected thread's goes through this vote.
 __device__ __forceinline__ bool warp_all(bool ok) { return __all_sync(0xFFFFFFFFu, ok) != 0; }
-// A wait in a loop that has no instruction for whole warps: its lanes may part
-// (one of them issues, the others keep its counters), and agree after the loop.
-// A vote on every block of k would cost 20 cycles (48 x 4096 x 4096 2 %).
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait_lane(uint64_t* bar, uint32_t parity, uint64_t limit_ns, int* status,
-                                               int site) {
-  return mbar_wait_poll<CLUSTER>(bar, parity, limit_ns, status, site);
-}
 
 // 128 x 128-byte box of a 2-D map at (x, y): x along the contiguous direction.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {

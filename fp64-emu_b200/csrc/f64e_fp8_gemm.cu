@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(PTHREADS, 1)
       bool ok = true;
       for (int tile = cluster; tile < ntiles && ok; tile += nclusters) {
         for (int kb = 0; kb < g.nkb && ok; it++) {   // an accumulator
-          if (!mbar_wait_lane(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) || *abort_flag) {
+          if (!warp_all(mbar_wait_poll(acc_empty, (it & 1) ^ 1, lim, status, kWaitAccEmpty) && !*abort_flag)) {
             ok = false;
             break;
           }
@@ -371,21 +371,21 @@ __global__ void __launch_bounds__(PTHREADS, 1)
             // Its scales, both CTAs' (group 0's came with the allocation's barrier).
             if (gr > 0) {
               const uint32_t par = sph ^ (ss == 0);
-              ok = mbar_wait_lane(&sf_full[ss], par, lim, status, kWaitScales) &&
-                   mbar_wait_lane<true>(&sf_peer[ss], par, lim, status, kWaitScales);
+              ok = warp_all(mbar_wait_poll(&sf_full[ss], par, lim, status, kWaitScales) &&
+                            mbar_wait_poll<true>(&sf_peer[ss], par, lim, status, kWaitScales));
             }
             // Two buffers in TMEM: the MMAs of the group before the last have
             // completed, by the ring (a stage is filled again only after
             // them) or, after short groups, by their own commit.
             if (ok && prev + STAGES > j + 1 && prev > 0) {
               const uint32_t p = prev - 1;
-              ok = mbar_wait_lane(&empty_bar[p % STAGES], (p / STAGES) & 1, lim, status, kWaitScales);
+              ok = warp_all(mbar_wait_poll(&empty_bar[p % STAGES], (p / STAGES) & 1, lim, status, kWaitScales));
             }
             prev = j;
             const uint32_t sf = tmem + SF_COL + (gr & 1) * SF_COLS;
             const int last = min(kb + 4, end);
             for (uint32_t i = 0; kb < last && ok; kb++, i++, j++) {
-              if (!mbar_wait_lane(&full_bar[s], ph, lim, status, kWaitFull)) {
+              if (!warp_all(mbar_wait_poll(&full_bar[s], ph, lim, status, kWaitFull))) {
                 ok = false;
                 break;
               }
@@ -421,7 +421,6 @@ __global__ void __launch_bounds__(PTHREADS, 1)
           if (ok && issuer) tc_commit_pair(acc_full, 0x3);
         }
       }
-      ok = warp_all(ok);
       if (!ok) *abort_flag = 1;
       // Every copy was waited for above and every MMA is waited for here: both
       // CTAs may then leave at the next barrier.
