@@ -510,13 +510,14 @@ cudaError_t launch_kernel(const CUtensorMap& tw, const CUtensorMap& tx, const Sp
     static std::map<int, bool> done;
     std::lock_guard<std::mutex> lk(mtx);
     if (!done[dev]) {
-      e = cudaFuncSetAttribute(fp8_split_kernel<OUT, XT, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+      e = cudaFuncSetAttribute(fp8_split_kernel<OUT, XT, TURNS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               227 * 1024);
       if (e != cudaSuccess) return e;
       done[dev] = true;
     }
   }
-  return fp8_launch(fp8_split_kernel<OUT, XT, TURNS>, (unsigned)(tiles * k.split), 32 * (4 + kQuantWarps<XT>), smem, k.split, s,
-                    tw, tx, k);
+  return fp8_launch(fp8_split_kernel<OUT, XT, TURNS>, (unsigned)(tiles * k.split), 32 * (4 + kQuantWarps<XT>), smem,
+                    k.split, s, tw, tx, k);
 }
 
 template <int OUT>
@@ -539,7 +540,8 @@ cudaError_t resident_clusters(int sms, const int** held) {
   if (it == known.end()) {
     std::array<int, kMaxSplit + 1> h{};
     const size_t smem = 200 * 1024;   // any amount above half an SM's gives the same answer
-    e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    e = cudaFuncSetAttribute(fp8_split_kernel<F64E_BF16, -1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             227 * 1024);
     if (e != cudaSuccess) return e;
     for (int n = 1; n <= kMaxSplit; n++) {
       cudaLaunchConfig_t cfg = {};
@@ -649,7 +651,8 @@ cudaError_t launch(SplitArgs k, int out_type, int x_type, int64_t K, const Plan&
   const int es = out_type == F64E_F32 ? 4 : 2;
   k.vec = k.out_r == 1 && reinterpret_cast<uintptr_t>(k.out) % (4 * es) == 0 && k.out_c % 4 == 0;
   k.ring = (uint32_t)std::max((size_t)k.nst * stage, (size_t)k.bn * kPitch * 4);
-  const size_t smem = std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * 2 * kAtom + (3 * kMaxStages + 5) * 8 + 16);
+  const size_t smem =
+      std::max(kMinSmem, 1024 + (size_t)k.ring + (size_t)k.nst * 2 * kAtom + (3 * kMaxStages + 5) * 8 + 16);
   if (x_type >= 0) {
     switch (x_type) {
       case F64E_F32: return launch_kernel<F64E_F32, F64E_F32, false>(tw, tx, k, tiles, smem, s);
@@ -670,7 +673,8 @@ cudaError_t launch_fp8_split(const Fp8GemmArgs& g, int64_t other_cost, bool* don
   *done = false;
   if (!(g.M <= g.N ? g.a : g.b).kmajor) return cudaSuccess;
   Plan plan;
-  const cudaError_t e = plan_tiles(std::max(g.M, g.N), std::min(g.M, g.N), (g.K + kBlock - 1) / kBlock, g.sms, 0, &plan);
+  const cudaError_t e =
+      plan_tiles(std::max(g.M, g.N), std::min(g.M, g.N), (g.K + kBlock - 1) / kBlock, g.sms, 0, &plan);
   if (e != cudaSuccess || plan.cost > other_cost) return e;
   *done = true;
   SplitArgs k = {};
