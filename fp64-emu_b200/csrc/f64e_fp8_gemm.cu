@@ -729,8 +729,11 @@ bool transpose_first(int64_t M, int64_t N, int64_t K, int sms) {
 
 }  // namespace
 
+// Decided for 148 SMs whatever the device: the size is asked for without one,
+// and the product decides by the same call.
 int64_t fp8_gemm_workspace(const Fp8GemmArgs& g) {
-  if (g.a.kmajor || g.b.kmajor || !transpose_first(g.M, g.N, g.K, 148)) return 0;
+  constexpr int kSms = 148;
+  if (g.a.kmajor || g.b.kmajor || !transpose_first(g.M, g.N, g.K, kSms)) return 0;
   return std::min(g.M, g.N) * round16(g.K);
 }
 

@@ -13,7 +13,8 @@
 // CTAs quantise the blocks of x they contract themselves: row blocks are 128
 // values of k, so a block is quantised within one step of the K loop.
 //   warp 0       TMA: 128 x 128 boxes of the wide operand (and the thin one's)
-//   warp 1       TMEM owner, scale copies and MMAs (tcgen05, cta_group::1)
+//   warp 1       TMEM owner; one thread issues scale copies and MMAs (tcgen05,
+//                cta_group::1)
 //   warps 2, 3   scales of the wide and the thin operand, four blocks of k a
 //                gather
 //   warps 4..    quantisation of x (eight warps); epilogue (four)

@@ -670,7 +670,9 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad()), kNoSecond);
+    // Asked for straight away; a gradient that comes with a graph of its own (a
+    // layer or a loss behind this one) is taken, see once().
+    TORCH_CHECK(!(at::GradMode::is_enabled() && grads[0].requires_grad() && grads[0].is_leaf()), kNoSecond);
     at::AutoDispatchBelowADInplaceOrView below;
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &wq = saved[0], &wsc = saved[1], &qc = saved[2], &sc = saved[3];
@@ -702,8 +704,8 @@ struct Fp8Linear : public torch::autograd::Function<Fp8Linear> {
  private:
   static constexpr const char* kNoSecond = "linear_fp8 has no second derivative";
   // Where a graph of the backward pass is asked for (create_graph): dx depends
-  // on w and dw on x, so a gradient is not a constant, and differentiating it
-  // ends with an error instead of leaving it out.
+  // on w and dy, dw on x and dy, so a gradient is not a constant, and
+  // differentiating it ends with an error instead of leaving it out.
   static at::Tensor once(at::Tensor grad) {
     if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
     grad.set_requires_grad(true);

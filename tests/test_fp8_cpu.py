@@ -466,3 +466,17 @@ def test_codes_and_products_are_detached():
                 assert not r.requires_grad and fw.unpack_dual(r).tangent is None
     for f in (fp64_emu.quantize_fp8, fp64_emu.quantize_fp8_both, fp64_emu.dequantize_fp8):
         assert "detached" in f.__doc__ or "without a\n    gradient" in f.__doc__
+
+
+@pytest.mark.parametrize("loss", [lambda y: y.sum(), lambda y: (y.float() ** 2).mean(), lambda y: torch.relu(y).sum()])
+def test_chain_of_layers_under_create_graph(loss):
+    """First derivatives of a chain come with create_graph too, whatever stands between and behind its layers; only
+    differentiating them is refused."""
+    x, w, _ = meta_layer()
+    w2 = torch.empty(30, 20, device="meta", requires_grad=True)
+    y = fp64_emu.linear_fp8(fp64_emu.linear_fp8(x, w), w2)
+    grads = torch.autograd.grad(loss(y), (x, w, w2), create_graph=True)
+    assert [g.shape for g in grads] == [x.shape, w.shape, w2.shape]
+    for g in grads:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            g.sum().backward(retain_graph=True)
